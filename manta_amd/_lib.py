@@ -19,11 +19,14 @@ LARGEST, SMALLEST = 0, 1
 Q8_ROWS, Q4_BLOCKS = 8, 4
 PROJ_F16, PROJ_Q8_COL, PROJ_F16_T, PROJ_Q8_COL_T = 0, 1, 2, 3
 DENSE_F32, DENSE_F16 = 32, 16
+F32, F16, BF16 = 32, 16, 17
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_NONE, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BLEND = 0, 1, 2, 3
 
 OPS = {"dot": DOT, "cosine": COSINE, "l2_distance": L2_DISTANCE}
 
-# Every exported symbol of include/manta_rocm.h, include/manta_mll.h and
-# include/manta_module.h:
+# Every exported symbol of include/manta_rocm.h, include/manta_cache.h,
+# include/manta_mll.h and include/manta_module.h:
 # name -> (restype, argtypes).
 _p = C.c_void_p
 _i64 = C.c_int64
@@ -48,6 +51,24 @@ class EncoderWeights(C.Structure):
         ("codes", C.c_void_p * 6),
         ("col_scales", C.c_void_p * 6),
     ]
+
+
+class Heads(C.Structure):
+    """MantaRocmHeads (include/manta_cache.h)."""
+    _fields_ = [("x_dev", C.c_void_p), ("out_dev", C.c_void_p), ("heads", C.c_int64), ("x_token", C.c_int64),
+                ("x_head", C.c_int64), ("out_token", C.c_int64), ("out_head", C.c_int64)]
+
+
+class CacheShape(C.Structure):
+    """MantaRocmCacheShape (include/manta_cache.h)."""
+    _fields_ = [(n, C.c_int64) for n in ("layers", "pages", "page_tokens", "kv_heads", "head_dim", "seqs",
+                                         "table_pages")]
+
+
+class CacheBuffers(C.Structure):
+    """MantaRocmCacheBuffers (include/manta_cache.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("k_codes", "v_codes", "k_max", "v_max", "book")] +
+                [(n, C.c_int64) for n in ("pitch", "code_bytes", "max_count", "book_count")])
 
 
 class Value(C.Structure):
@@ -173,6 +194,28 @@ SIGNATURES = {
     "manta_rocm_program_trace_count": (_i64, [_p]),
     "manta_rocm_program_trace_step": (
         C.c_int, [_p, _i64, C.POINTER(C.c_char_p), C.POINTER(C.c_char_p), C.POINTER(C.c_char_p)]),
+    "manta_rocm_rotary_freqs": (
+        C.c_int, [_i64, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double, _p, _err]),
+    "manta_rocm_rotary_bind": (C.c_int, [_p, _p, _i64, C.c_int, C.c_double, C.POINTER(_p), _err]),
+    "manta_rocm_rotary_unbind": (None, [_p]),
+    "manta_rocm_rotary": (C.c_int, [_p, _p, C.c_int, _p, _i64, _i64, C.POINTER(Heads), _i64, C.c_int, _err]),
+    "manta_rocm_cache_create": (C.c_int, [_p, C.POINTER(CacheShape), C.POINTER(_p), _err]),
+    "manta_rocm_cache_destroy": (None, [_p]),
+    "manta_rocm_cache_shape": (C.c_int, [_p, C.POINTER(CacheShape)]),
+    "manta_rocm_cache_buffers": (C.c_int, [_p, C.POINTER(CacheBuffers)]),
+    "manta_rocm_cache_extend": (C.c_int, [_p, _p, _p, _p, _i64, _err]),
+    "manta_rocm_cache_fork": (C.c_int, [_p, _p, _p, _p, _p, _i64, _err]),
+    "manta_rocm_cache_release": (C.c_int, [_p, _p, _p, _p, _i64, _err]),
+    "manta_rocm_cache_compact": (C.c_int, [_p, _p, _p, _err]),
+    "manta_rocm_cache_copy_pages": (C.c_int, [_p, _p, _p, _p, _i64, _err]),
+    "manta_rocm_cache_append": (
+        C.c_int, [_p, _p, _i64, C.c_int, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _err]),
+    "manta_rocm_cache_read": (
+        C.c_int, [_p, _p, _i64, C.c_int, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _err]),
+    "manta_rocm_cache_attention": (
+        C.c_int, [_p, _p, _i64, C.c_int, C.POINTER(Heads), _p, _p, _p, _i64, _i64, C.c_double, C.c_int, _i64, _i64,
+                  _err]),
+    "manta_rocm_copy": (C.c_int, [_p, _p, _p, C.c_size_t, _err]),
     "manta_rocm_embed_pooled": (
         C.c_int,
         [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, C.c_int, _p, _i64, _p, _err],

@@ -1,0 +1,118 @@
+// cache_kernels.hpp -- host-side launchers of the rotary and cache kernels,
+// and the element types they share (internal to libmanta_rocm.so; the public
+// surface is include/manta_cache.h).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "cache_layout.hpp"
+
+namespace manta {
+
+// ---- rotary ----
+constexpr int kRotaryParts = 4;
+struct RotaryPart {
+    const void* x;
+    void* out;
+    int heads;
+    int64_t x_token, x_head, out_token, out_head;
+};
+struct RotaryArgs {
+    RotaryPart part[kRotaryParts];
+    int parts, heads;      // tensors; heads of all of them
+    const double* turns;   // [rot / 2] turns a token
+    const int32_t* positions;
+    int64_t tokens;
+    int head_dim, rot, interleaved;
+    float magnitude;
+    int inverse;
+    int dtype;
+    int wide;  // every row starts on 16 bytes and splits into 16-byte pieces
+};
+hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s);
+
+// ---- cache ----
+struct RaggedRows {
+    const int32_t* offsets;  // [n + 1]
+    const int32_t* seqs;     // [n] or nullptr
+    int n;
+    int tokens;
+};
+struct KvRows {  // k and v [tokens, kv_heads, head_dim], in or out
+    void* k;
+    void* v;
+    int64_t k_token, k_head, v_token, v_head;
+    int dtype;
+    int wide;  // every row starts on 16 bytes
+};
+hipError_t launch_cache_append(const CacheView& c, int64_t layer, const RaggedRows& r, const KvRows& x, hipStream_t s);
+hipError_t launch_cache_read(const CacheView& c, int64_t layer, const RaggedRows& r, const KvRows& x, hipStream_t s);
+
+// scratch of the page calls: pairs (from, to) to copy, their count first
+struct PageScratch {
+    int32_t* count;
+    int32_t* from;
+    int32_t* to;
+    int32_t* remap;  // [pages]
+};
+hipError_t launch_cache_extend(const CacheView& c, const PageScratch& w, const int32_t* seqs, const int32_t* counts,
+                               int n, int32_t* free_list, hipStream_t s);
+hipError_t launch_cache_fork(const CacheView& c, const int32_t* parents, const int32_t* children,
+                             const int32_t* tokens, int n, hipStream_t s);
+hipError_t launch_cache_release(const CacheView& c, const int32_t* seqs, const int32_t* keep, int n, hipStream_t s);
+hipError_t launch_cache_compact(const CacheView& c, const PageScratch& w, int32_t* live, hipStream_t s);
+hipError_t launch_cache_remap(const CacheView& c, const PageScratch& w, hipStream_t s);
+// copy pages from[i] -> to[i], i < *count (count in device memory) or n
+hipError_t launch_cache_copy(const CacheView& c, const int32_t* from, const int32_t* to, const int32_t* count, int n,
+                             hipStream_t s);
+
+struct AttendArgs {
+    const void* q;
+    void* out;
+    float* lse;
+    int64_t q_token, q_head, o_token, o_head;
+    int dtype;
+    int heads, group;
+    float scale;  // of q k, in units of exp2
+    int causal;
+    int window;
+    int longest;
+    int wide;
+    float* partial;
+    int64_t partial_bytes;
+    uint32_t* tickets;
+    int cus;
+};
+hipError_t launch_cache_attention(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a,
+                                  hipStream_t s);
+
+#ifdef __HIP__
+// ---- elements ----
+struct F32 {
+    typedef float T;
+    static constexpr int kWide = 4;  // elements of 16 bytes
+    static __device__ __forceinline__ float load(T x) { return x; }
+    static __device__ __forceinline__ T store(float x) { return x; }
+};
+struct F16 {
+    typedef _Float16 T;
+    static constexpr int kWide = 8;
+    static __device__ __forceinline__ float load(T x) { return (float)x; }
+    static __device__ __forceinline__ T store(float x) { return (T)x; }
+};
+struct Bf16 {
+    typedef __bf16 T;
+    static constexpr int kWide = 8;
+    static __device__ __forceinline__ float load(T x) {
+        return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, x) << 16);
+    }
+    static __device__ __forceinline__ T store(float x) { return (T)x; }
+};
+
+__device__ __forceinline__ void cache_report(const CacheView& c, int kind, int64_t a, int64_t b) {
+    atomicMax(c.err, cache_error(kind, a, b));
+}
+#endif
+
+}  // namespace manta

@@ -20,11 +20,13 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <new>
 #include <set>
 #include <string>
 #include <thread>
 #include <vector>
 
+#include "cache_layout.hpp"
 #include "device_common.hpp"
 #include "kernels.hpp"
 #include "mq_plan.hpp"
@@ -68,6 +70,10 @@ struct MantaRocm {
     // candidate sets bound on this runtime and not yet unbound: destroy
     // releases their device memory and detaches them
     std::set<MantaRocmCandidates*> bound;
+    // rotary tables and caches, likewise
+    std::set<manta_rt::Attached*> attached;
+    // a cache was made: err_word[1] may hold what its kernels found wrong
+    bool cache_errors = false;
 };
 
 struct MantaRocmCandidates {
@@ -281,6 +287,25 @@ int check_gather_error(MantaRocm* rt, char** err) {
     return fail(err, MANTA_ROCM_ERROR, "gather index %d out of range", manta_rt::gather_error_index(w));
 }
 
+// What a cache kernel found wrong (cache_layout.hpp), reported and cleared by
+// the next synchronizing call.  Looked at on every such call once a cache
+// exists: a graph's replays leave no other sign.
+int check_cache_error(MantaRocm* rt, char** err) {
+    if (!rt->cache_errors) return MANTA_ROCM_OK;
+    unsigned long long w = 0;
+    HIP_TRY(hipMemcpyAsync(&w, rt->err_word + 1, sizeof(w), hipMemcpyDeviceToHost, rt->stream),
+            "hipMemcpy(error word)");
+    HIP_TRY(hipStreamSynchronize(rt->stream), "hipStreamSynchronize");
+    if (w == 0) return MANTA_ROCM_OK;
+    const unsigned long long zero = 0;
+    HIP_TRY(hipMemcpyAsync(rt->err_word + 1, &zero, sizeof(zero), hipMemcpyHostToDevice, rt->stream),
+            "hipMemcpy(error word)");
+    HIP_TRY(hipStreamSynchronize(rt->stream), "hipStreamSynchronize");
+    char text[160];
+    manta::describe_cache_error(w, text, sizeof(text));
+    return fail(err, MANTA_ROCM_ERROR, "%s", text);
+}
+
 #define RT_CHECK(rt)                                                          \
     do {                                                                      \
         if (!(rt)) return fail(err, MANTA_ROCM_ERROR, "nil rocm runtime");    \
@@ -371,8 +396,8 @@ int manta_rocm_create(int device, MantaRocm** out, char** err) {
     }
     // the allocation-free entry point's scratch address on this device
     manta_rt::noalloc_init(device);
-    e = hipMalloc((void**)&rt->err_word, sizeof(unsigned long long));
-    if (e == hipSuccess) e = hipMemset(rt->err_word, 0, sizeof(unsigned long long));
+    e = hipMalloc((void**)&rt->err_word, 2 * sizeof(unsigned long long));  // gathers', caches'
+    if (e == hipSuccess) e = hipMemset(rt->err_word, 0, 2 * sizeof(unsigned long long));
     if (e == hipSuccess) e = hipMalloc((void**)&rt->tickets, kTickets * sizeof(uint32_t));
     if (e == hipSuccess) e = hipMemset(rt->tickets, 0, kTickets * sizeof(uint32_t));
     if (e != hipSuccess) {
@@ -407,6 +432,8 @@ void manta_rocm_destroy(MantaRocm* rt) {
         c->rt = nullptr;
     }
     rt->bound.clear();
+    for (manta_rt::Attached* a : rt->attached) a->release();
+    rt->attached.clear();
     if (rt->own_stream) (void)hipStreamDestroy(rt->own_stream);
     delete rt;
 }
@@ -421,7 +448,8 @@ int manta_rocm_set_stream(MantaRocm* rt, void* hip_stream, char** err) {
 int manta_rocm_synchronize(MantaRocm* rt, char** err) {
     RT_CHECK(rt);
     HIP_TRY(hipStreamSynchronize(rt->stream), "hipStreamSynchronize");
-    return check_gather_error(rt, err);
+    int rc = check_gather_error(rt, err);
+    return rc ? rc : check_cache_error(rt, err);
 }
 
 int manta_rocm_malloc(MantaRocm* rt, void** out_dev, size_t bytes, char** err) {
@@ -459,7 +487,8 @@ int manta_rocm_download(MantaRocm* rt, void* dst, const void* src_dev, size_t by
             "hipMemcpyDtoH");
     HIP_TRY(hipStreamSynchronize(rt->stream), "hipStreamSynchronize");
     rt->stats.bytes_downloaded += bytes;
-    return check_gather_error(rt, err);
+    int rc = check_gather_error(rt, err);
+    return rc ? rc : check_cache_error(rt, err);
 }
 
 int manta_rocm_set_timing(MantaRocm* rt, int on, char** err) {
@@ -1395,6 +1424,62 @@ int manta_rt::score_topk_impl(MantaRocm* rt, const MantaRocmCandidates* c, int o
 int manta_rt::runtime_device(const MantaRocm* rt) { return rt ? rt->device : -1; }
 
 void* manta_rt::runtime_stream(const MantaRocm* rt) { return rt ? (void*)rt->stream : nullptr; }
+
+int manta_rt::runtime_cus(const MantaRocm* rt) { return rt->cus; }
+
+int manta_rt::fail(char** err, int code, const char* fmt, ...) {
+    if (err) {
+        va_list ap;
+        va_start(ap, fmt);
+        *err = dup_printf(fmt, ap);
+        va_end(ap);
+    }
+    return code;
+}
+
+int manta_rt::use(MantaRocm* rt, char** err) {
+    RT_CHECK(rt);
+    return MANTA_ROCM_OK;
+}
+
+void* manta_rt::launch_begin(MantaRocm* rt) {
+    if (!rt->timing) return nullptr;
+    hipEvent_t e = pooled_event(rt);
+    if (e) (void)hipEventRecord(e, rt->stream);
+    return e;
+}
+
+void manta_rt::launch_end(MantaRocm* rt, const char* what, void* start) {
+    rt->stats.kernel_launches++;
+    if (!start) return;
+    hipEvent_t e = pooled_event(rt);
+    if (e) {
+        (void)hipEventRecord(e, rt->stream);
+        rt->pending.push_back(TimedLaunch{what, (hipEvent_t)start, e});
+    } else {
+        rt->event_pool.push_back((hipEvent_t)start);
+    }
+}
+
+bool manta_rt::attach(MantaRocm* rt, Attached* a) {
+    try {
+        rt->attached.insert(a);
+    } catch (const std::bad_alloc&) {
+        return false;
+    }
+    return true;
+}
+
+void manta_rt::detach(MantaRocm* rt, Attached* a) {
+    (void)hipSetDevice(rt->device);
+    (void)hipStreamSynchronize(rt->stream);
+    a->release();
+    rt->attached.erase(a);
+}
+
+unsigned long long* manta_rt::cache_error_word(const MantaRocm* rt) { return rt->err_word + 1; }
+
+void manta_rt::cache_errors_possible(MantaRocm* rt) { rt->cache_errors = true; }
 
 int manta_rt::pack_candidates_into(MantaRocm* rt, const MantaRocmCandidates* c, const int32_t* top, int64_t nq,
                                    int64_t k, const int64_t* candidate_ids, int64_t* out_ids, void* out_rows,

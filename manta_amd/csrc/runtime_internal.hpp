@@ -36,6 +36,35 @@ int pack_candidates_into(MantaRocm* rt, const MantaRocmCandidates* c, const int3
                          const int64_t* candidate_ids, int64_t* out_ids, void* out_rows, void* out_scales,
                          unsigned long long* err_word, char** err);
 
+// ---- for entry points in other files (cache.cpp) ----
+
+// An error code with a malloc'd message (printf-style).
+int fail(char** err, int code, const char* fmt, ...);
+
+// Checks the runtime and makes its device current.
+int use(MantaRocm* rt, char** err);
+
+int runtime_cus(const MantaRocm* rt);
+
+// Bracket a launch: counted, and timed when timing is on.
+void* launch_begin(MantaRocm* rt);
+void launch_end(MantaRocm* rt, const char* what, void* start);
+
+// A handle whose device memory goes with its runtime: manta_rocm_destroy
+// calls release() on those still attached (the handle itself stays), and
+// detach() waits for the runtime's stream and releases one.
+struct Attached {
+    virtual ~Attached() {}
+    virtual void release() = 0;
+};
+bool attach(MantaRocm* rt, Attached* a);  // false: out of memory
+void detach(MantaRocm* rt, Attached* a);
+
+// The device word the cache kernels report into, and the flag that makes
+// synchronizing calls look at it.
+unsigned long long* cache_error_word(const MantaRocm* rt);
+void cache_errors_possible(MantaRocm* rt);
+
 // The index a gather error word holds (report_gather_error's encoding).
 inline int gather_error_index(unsigned long long w) { return (int)(uint32_t)(~w & 0xFFFFFFFFull); }
 

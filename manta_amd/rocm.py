@@ -78,6 +78,27 @@ class DeviceArray:
             pass
 
 
+class View:
+    """Part of a device array, strided: shape and strides (in elements), the
+    first element at `offset`.  The last axis is contiguous.  For the calls
+    that take strides (rotary, Cache): q inside a fused q/k/v buffer, heads
+    before tokens."""
+
+    def __init__(self, array: DeviceArray, shape, strides, offset: int = 0):
+        self.array = array
+        self.rt, self.dtype = array.rt, array.dtype
+        self.shape = tuple(int(s) for s in shape)
+        self.strides = tuple(int(s) for s in strides)
+        if len(self.shape) != len(self.strides) or not self.shape or self.strides[-1] != 1:
+            raise ValueError("a view needs a stride per axis, the last of them 1")
+        if offset < 0 or min(self.strides) < 0 or min(self.shape) < 0:
+            raise ValueError("a view's offset, shape and strides must not be negative")
+        last = offset + sum((n - 1) * s for n, s in zip(self.shape, self.strides))
+        if 0 not in self.shape and (last + 1) * self.dtype.itemsize > array.nbytes:
+            raise ValueError("view %s of strides %s at %d leaves its array" % (self.shape, self.strides, offset))
+        self.addr = array.addr + offset * self.dtype.itemsize
+
+
 class Candidates:
     """Device-resident packed candidate matrix ([sets, n, d])."""
 
@@ -157,6 +178,36 @@ class Runtime:
         s = _lib.Stats()
         load().manta_rocm_stats(self.handle, C.byref(s))
         return {f: getattr(s, f) for f, _ in _lib.Stats._fields_}
+
+    def copy(self, dst: DeviceArray, src: DeviceArray) -> None:
+        """Copy src over dst (the same size) on the runtime's stream."""
+        if dst.nbytes != src.nbytes:
+            raise ValueError("copy size mismatch: %d vs %d" % (dst.nbytes, src.nbytes))
+        call("manta_rocm_copy", self.handle, dst.addr, src.addr, dst.nbytes)
+
+    # ------------------------------------------- rotary positions, the cache
+    def rotary_bind(self, freqs, layout: str = "half", magnitude: float = 1.0):
+        """Frequencies (radians a token, one a pair; rotary_freqs) as rotary
+        takes them; layout "half" or "interleaved"."""
+        from . import cache
+
+        return cache.Rotary(self, freqs, layout, magnitude)
+
+    def rotary(self, rot, positions: DeviceArray, parts, inverse: bool = False, dtype: Optional[str] = None) -> None:
+        """Rotate the tensors of parts [(x, out), ...], each [tokens, heads,
+        head_dim] (out may be x), by the tokens' positions (int32);
+        inverse=True is the gradient.  dtype "f32", "f16" or "bf16" (by default
+        the array's; 16-bit arrays are f16)."""
+        from . import cache
+
+        cache.rotary(self, rot, positions, parts, inverse, dtype)
+
+    def cache(self, pages: int, kv_heads: int, head_dim: int, seqs: int, table_pages: int, page_tokens: int = 64,
+              layers: int = 1):
+        """An empty 8-bit key/value cache of pages (cache.Cache)."""
+        from . import cache
+
+        return cache.Cache(self, layers, pages, page_tokens, kv_heads, head_dim, seqs, table_pages)
 
     # ------------------------------------------------------------ binding
     def bind_q8(self, codes: np.ndarray, scales: np.ndarray) -> Candidates:
@@ -438,6 +489,20 @@ class Runtime:
         call("manta_rocm_encoder_pooled_layers", self.handle, tokens.ptr, mask.ptr, C.c_int64(b), C.c_int64(t),
              C.byref(w), C.c_int64(vocab), C.c_int64(d), C.c_int64(h), C.c_int64(layers), out.ptr)
         return out
+
+
+def rotary_freqs(rot: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, low: float = 1.0,
+                 high: float = 4.0, original: float = 8192.0) -> np.ndarray:
+    """Frequencies of rot/2 pairs in radians a token; scaling "none",
+    "linear", "base" or "blend" (include/manta_cache.h has the formulas)."""
+    kinds = {"none": _lib.ROTARY_NONE, "linear": _lib.ROTARY_LINEAR, "base": _lib.ROTARY_BASE,
+             "blend": _lib.ROTARY_BLEND}
+    if scaling not in kinds:
+        raise ValueError("unknown rotary scaling %r (none, linear, base, blend)" % (scaling,))
+    out = np.empty((max(rot, 0) // 2,), np.float64)
+    call("manta_rocm_rotary_freqs", rot, base, kinds[scaling], factor, low, high, original,
+         out.ctypes.data_as(C.c_void_p))
+    return out
 
 
 def pack_q8_rows(x: np.ndarray):
