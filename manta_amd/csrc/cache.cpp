@@ -170,7 +170,7 @@ int manta_rocm_rotary(MantaRocm* rt, const MantaRocmRotary* rot, int dtype, cons
                       int64_t tokens, int64_t head_dim, const MantaRocmHeads* parts, int64_t nparts, int inverse,
                       char** err) {
     if (!manta::element_type(dtype)) return fail(err, MANTA_ROCM_ERROR, "rotary: unknown element type %d", dtype);
-    if (tokens < 0 || tokens > manta::kMaxInt32 / 2)
+    if (tokens < 0 || tokens > manta::kMaxTokens)
         return fail(err, MANTA_ROCM_ERROR, "rotary: bad token count %lld", (long long)tokens);
     if (nparts < 1 || nparts > manta::kRotaryParts || !parts)
         return fail(err, MANTA_ROCM_ERROR, "rotary: 1 to %d tensors (got %lld)", manta::kRotaryParts,

@@ -19,6 +19,10 @@ namespace manta {
 
 constexpr int kMaxHeadDim = 256;
 constexpr int64_t kMaxInt32 = 0x7FFFFFFF;
+// A launch has less than 2^32 threads: a workgroup a sequence, or one a slot
+// of a ragged batch (tokens / 16 + 2 n of them).
+constexpr int64_t kMaxSeqs = 1 << 21;
+constexpr int64_t kMaxTokens = 1 << 25;
 
 // What the kernels know of a cache.
 struct CacheView {
@@ -113,7 +117,7 @@ inline const char* check_cache_shape(const MantaRocmCacheShape& s) {
         return "page_tokens must be 16, 32, 64 or 128";
     if (s.head_dim <= 0 || s.head_dim > kMaxHeadDim) return "head_dim must be 1 to 256";
     if (s.kv_heads > 65535 || s.layers > 65535) return "at most 65535 kv_heads and layers";
-    if (s.pages > (kMaxInt32 >> 2) || s.seqs > (kMaxInt32 >> 2)) return "too many pages or sequences";
+    if (s.pages > (kMaxInt32 >> 2) || s.seqs > kMaxSeqs) return "too many pages or sequences";
     if (s.table_pages > kMaxInt32 / s.page_tokens) return "table_pages * page_tokens exceeds int32 lengths";
     if (s.pages + s.seqs + s.seqs * s.table_pages > (kMaxInt32 >> 1)) return "the book exceeds int32 entries";
     return nullptr;
@@ -130,7 +134,7 @@ inline const char* check_strides(int64_t tokens, int64_t heads, int64_t head_dim
 
 inline const char* check_batch(int64_t n, int64_t tokens, int64_t seqs, bool listed) {
     if (n < 0 || tokens < 0) return "negative count";
-    if (n > (kMaxInt32 >> 2) || tokens > (kMaxInt32 >> 2)) return "too many sequences or tokens";
+    if (n > kMaxSeqs || tokens > kMaxTokens) return "too many sequences or tokens";
     if (!listed && n > seqs) return "more sequences than the cache has";
     return nullptr;
 }

@@ -253,7 +253,8 @@ __global__ __launch_bounds__(kBook) void extend_kernel(CacheView c, PageScratch 
         taken += total;
         copies += copied;
         __syncthreads();  // every growth() of this step has read the book
-        if (g.ok) {
+        // (a list that names a sequence twice could ask for more than was counted)
+        if (g.ok && at >= 0 && at + mine <= need && copy < need) {
             int32_t* row = c.tables + (int64_t)g.seq * c.table_pages;
             if (g.last >= 0) {
                 const int page = free_list[at++];

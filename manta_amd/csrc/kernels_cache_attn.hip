@@ -34,7 +34,7 @@ __global__ __launch_bounds__(64) void attend_kernel(CacheView c, int64_t layer, 
     else if (lane == 0) cache_report(c, kCacheBadSeq, seq, 0);
     const int pos = length - (hi - lo) + (row - lo);
     const int end = a.causal ? min(length, pos + 1) : length;
-    const int begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const int begin = a.window > 0 ? (int)max((int64_t)0, (int64_t)pos - a.window + 1) : 0;
     const int d = c.head_dim, kv = head / a.group;
     const T* q = (const T*)a.q + row * a.q_token + head * a.q_head;
     for (int k = lane; k < d; k += 64) qs[k] = E::load(q[k]);

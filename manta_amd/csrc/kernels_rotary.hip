@@ -27,8 +27,9 @@ template <class E, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     typedef typename E::T T;
     __shared__ float cs[kMaxHeadDim / 2], sn[kMaxHeadDim / 2];
-    const int64_t token = blockIdx.x;
     const int half = a.rot >> 1;
+  for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+    __syncthreads();  // an earlier token's angles have been used
     const double pos = (double)a.positions[token];
     for (int p = threadIdx.x; p < half; p += kThreads) {
         const double t = pos * a.turns[p];
@@ -91,6 +92,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
             *(Pack<E, V>*)(y + half + p) = yhi;
         }
     }
+  }
 }
 
 template <class E>
@@ -99,7 +101,7 @@ hipError_t launch(const RotaryArgs& a, hipStream_t s) {
     // is full
     int split = 1;
     while (split < 8 && split * 2 <= a.heads && a.tokens * split < 512) split *= 2;
-    const dim3 grid((unsigned)a.tokens, split);
+    const dim3 grid((unsigned)(a.tokens < (1 << 20) ? a.tokens : 1 << 20), split);
     if (a.wide) {
         if (a.interleaved) rotary_kernel<E, E::kWide, true><<<grid, kThreads, 0, s>>>(a);
         else rotary_kernel<E, E::kWide, false><<<grid, kThreads, 0, s>>>(a);
