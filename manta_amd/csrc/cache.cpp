@@ -459,6 +459,9 @@ int manta_rocm_cache_attention(MantaRocm* rt, const MantaRocmCache* c, int64_t l
     if (window < 0 || (window > 0 && !causal))
         return fail(err, MANTA_ROCM_ERROR, "cache_attention: a window must be positive and causal");
     if (longest < 0) return fail(err, MANTA_ROCM_ERROR, "cache_attention: negative length");
+    if (tokens * q->heads > ((int64_t)1 << 28))
+        return fail(err, MANTA_ROCM_ERROR, "cache_attention: too many rows (%lld tokens of %lld heads)", (long long)tokens,
+                    (long long)q->heads);
     if (n == 0 || tokens == 0) return MANTA_ROCM_OK;
     manta::AttendArgs a{};
     a.q = q->x_dev;
@@ -471,7 +474,7 @@ int manta_rocm_cache_attention(MantaRocm* rt, const MantaRocmCache* c, int64_t l
     a.dtype = dtype;
     a.heads = (int)q->heads;
     a.group = (int)(q->heads / c->shape.kv_heads);
-    a.scale = (float)(scale * M_LOG2E);
+    a.scale = (float)(scale * M_LOG2E / 127.0);
     a.causal = causal != 0;
     a.window = window > manta::kMaxInt32 ? 0 : (int)window;
     a.longest = (int)(longest < manta::kMaxInt32 ? longest : manta::kMaxInt32);
@@ -479,6 +482,7 @@ int manta_rocm_cache_attention(MantaRocm* rt, const MantaRocmCache* c, int64_t l
     a.partial = c->partial;
     a.partial_bytes = (int64_t)kPartialBytes;
     a.tickets = c->tickets;
+    a.ntickets = (int64_t)kAttendTickets;
     a.cus = manta_rt::runtime_cus(rt);
     const manta::RaggedRows r{offsets, seqs, (int)n, (int)tokens};
     return launch(rt, "cache_attention", err,

@@ -74,15 +74,19 @@ struct AttendArgs {
     int64_t q_token, q_head, o_token, o_head;
     int dtype;
     int heads, group;
-    float scale;  // of q k, in units of exp2
+    float scale;  // scale * log2 e / 127: of q . codes * k_max, in units of exp2
     int causal;
     int window;
     int longest;
     int wide;
-    float* partial;
+    float* partial;  // what split tiles leave for their last workgroup
     int64_t partial_bytes;
-    uint32_t* tickets;
+    uint32_t* tickets;  // ntickets, zero between calls
+    int64_t ntickets;
     int cus;
+    // the launcher's plan
+    int splits;  // workgroups that may share a tile's keys
+    int rounds;  // steps over the keys that are worth a workgroup
 };
 hipError_t launch_cache_attention(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a,
                                   hipStream_t s);
@@ -109,6 +113,27 @@ struct Bf16 {
     }
     static __device__ __forceinline__ T store(float x) { return (T)x; }
 };
+
+__device__ __forceinline__ int clamp_row(int x, int tokens) { return x < 0 ? 0 : x > tokens ? tokens : x; }
+
+// The sequence whose slots hold `slot`: the last i < n with base(i) <= slot.
+// Every wave of the workgroup finds it, 64 candidates a step.
+template <class Base>
+__device__ __forceinline__ int find_slot(int n, int64_t slot, Base base) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = n;  // the answer lies in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) / 64;
+        const int i = lo + lane * step;
+        const bool below = i < hi && base(i) <= slot;
+        // (lane 0's candidate counts as below even where the bases do not ascend)
+        const unsigned long long m = __ballot(below) | 1ull;
+        const int last = 63 - __clzll(m);
+        lo += last * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
 
 __device__ __forceinline__ void cache_report(const CacheView& c, int kind, int64_t a, int64_t b) {
     atomicMax(c.err, cache_error(kind, a, b));

@@ -104,6 +104,13 @@ MANTA_HD bool ragged_piece(int a, int b, int length, int64_t local, int shift, P
     return true;
 }
 
+// ---- a ragged batch in tiles of query rows ----
+// Row r of sequence i and kv head h is query head h * group + r % group of
+// the sequence's token r / group.  A tile is `rows` of them; ceil(count *
+// group / rows) tiles fit the slots [tile_base(a, i), tile_base(b, i + 1)).
+MANTA_HD int64_t tile_slots(int64_t tokens, int64_t n, int64_t group, int rows) { return tokens * group / rows + n; }
+MANTA_HD int64_t tile_base(int offset, int64_t i, int64_t group, int rows) { return offset * group / rows + i; }
+
 // ---- checks (nullptr: nothing wrong) ----
 
 MANTA_HD bool element_type(int dtype) {

@@ -14,31 +14,12 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ int clamp_row(int x, int tokens) { return x < 0 ? 0 : x > tokens ? tokens : x; }
-
-// The sequence whose slots hold `slot`: the last i with ragged_base(i) <=
-// slot.  Every wave of the workgroup finds it, 64 candidates a step.
-__device__ int find_sequence(const RaggedRows& r, int64_t slot, int shift) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, hi = r.n;  // the answer lies in [lo, hi)
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 63) / 64;
-        const int i = lo + lane * step;
-        const bool below = i < hi && ragged_base(clamp_row(r.offsets[i], r.tokens), i, shift) <= slot;
-        // (lane 0's candidate counts as below even where the offsets do not ascend)
-        const unsigned long long m = __ballot(below) | 1ull;
-        const int last = 63 - __clzll(m);
-        lo += last * step;
-        hi = min(hi, lo + step);
-    }
-    return lo;
-}
-
 // This workgroup's piece of the ragged batch and its page: false if there is
 // none.
 __device__ bool my_piece(const CacheView& c, const RaggedRows& r, Piece* p, int* page) {
     const int64_t slot = blockIdx.x;
-    const int i = find_sequence(r, slot, c.page_shift);
+    const int i = find_slot(
+        r.n, slot, [&](int j) { return ragged_base(clamp_row(r.offsets[j], r.tokens), j, c.page_shift); });
     const int a = clamp_row(r.offsets[i], r.tokens), b = clamp_row(r.offsets[i + 1], r.tokens);
     const int seq = r.seqs ? r.seqs[i] : i;
     if ((unsigned)seq >= (unsigned)c.seqs) {
