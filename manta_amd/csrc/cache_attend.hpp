@@ -7,6 +7,7 @@
 
 namespace manta {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
@@ -110,18 +111,38 @@ __device__ __forceinline__ int key_begin(const AttendArgs& a, int pos) {
 __device__ __forceinline__ Tile my_tile(const CacheView& c, const RaggedRows& r, const AttendArgs& a, int64_t slot,
                                         int rows) {
     Tile t{};
-    const int i = __builtin_amdgcn_readfirstlane(
-        r.n == 1 ? 0 : find_slot(r.n, slot, [&](int j) {
+    int i, from, to, length = 0;
+    if (r.n <= 64) {
+        // every sequence's offsets and length at once, the one wanted picked
+        // from the lanes: one wait where a search, its result's offsets and
+        // its length are three
+        const int lane = threadIdx.x & 63, j = min(lane, r.n - 1);
+        const int o0 = clamp_row(r.offsets[j], r.tokens), o1 = clamp_row(r.offsets[j + 1], r.tokens);
+        int seq = r.seqs ? r.seqs[j] : j;
+        const bool good = (unsigned)seq < (unsigned)c.seqs;
+        const int len = good ? c.lengths[seq] : -1;
+        const unsigned long long m = __ballot(lane < r.n && tile_base(o0, j, a.group, rows) <= slot) | 1ull;
+        i = 63 - __clzll(m);
+        from = __builtin_amdgcn_readlane(o0, i);
+        to = __builtin_amdgcn_readlane(o1, i);
+        t.seq = __builtin_amdgcn_readlane(seq, i);
+        length = __builtin_amdgcn_readlane(len, i);
+    } else {
+        i = __builtin_amdgcn_readfirstlane(find_slot(r.n, slot, [&](int j) {
             return tile_base(clamp_row(r.offsets[j], r.tokens), j, a.group, rows);
         }));
-    t.row0 = clamp_row(r.offsets[i], r.tokens);
-    t.count = clamp_row(r.offsets[i + 1], r.tokens) - t.row0;
+        from = clamp_row(r.offsets[i], r.tokens);
+        to = clamp_row(r.offsets[i + 1], r.tokens);
+        t.seq = r.seqs ? r.seqs[i] : i;
+        if ((unsigned)t.seq < (unsigned)c.seqs) length = c.lengths[t.seq];
+    }
+    t.row0 = from;
+    t.count = to - from;
     const int64_t r0 = (slot - tile_base(t.row0, i, a.group, rows)) * rows;
     if (t.count <= 0 || r0 < 0 || r0 >= (int64_t)t.count * a.group) return t;
     t.r0 = (int)r0;
     t.rows = (int)min((int64_t)rows, (int64_t)t.count * a.group - r0);
-    t.seq = r.seqs ? r.seqs[i] : i;
-    if ((unsigned)t.seq < (unsigned)c.seqs) t.length = c.clamp_length(c.lengths[t.seq]);
+    if ((unsigned)t.seq < (unsigned)c.seqs) t.length = c.clamp_length(length);
     else {
         if (threadIdx.x == 0) cache_report(c, kCacheBadSeq, t.seq, 0);
         t.seq = 0;  // length 0: none of its table is read
@@ -133,14 +154,135 @@ __device__ __forceinline__ Tile my_tile(const CacheView& c, const RaggedRows& r,
     return t;
 }
 
-// Results of a tile's part of the keys, in global memory: [row][pitch + 4],
-// the weighted mean of v, then the largest score and the sum of weights.
-// Written with agent-scope stores, which the last workgroup's ticket follows.
-__device__ __forceinline__ void part_store(float* at, float x) {
-    __hip_atomic_store((uint32_t*)at, __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// What the workgroups of a tile leave for the last of them, in global memory.
+// Agent scope (sc1): written through, and read past this die's caches; the
+// ticket is taken after the stores are done.  Offsets are in bytes, and the
+// buffer's size is checked by the access itself.
+struct Parts {
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ explicit Parts(const AttendArgs& a)
+        : rsrc(__builtin_amdgcn_make_buffer_rsrc(a.partial, 0, (int)a.partial_bytes, 0x00020000)) {}
+    static constexpr int kAgent = 16;
+    __device__ __forceinline__ void store(int at, f32x4 x) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), rsrc, at, 0, kAgent);
+    }
+    __device__ __forceinline__ void store(int at, f32x2 x) const {
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), rsrc, at, 0, kAgent);
+    }
+    __device__ __forceinline__ f32x4 load4(int at) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, kAgent));
+    }
+    __device__ __forceinline__ f32x2 load2(int at) const {
+        return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, 0, kAgent));
+    }
+};
+
+// The end of a tile's part: true in the last of its `parts` workgroups, which
+// sees what all of them stored.  The ticket is zero again.
+__device__ __forceinline__ bool last_part(uint32_t* ticket, int parts) {
+    __shared__ int last;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(parts - 1);
+        if (last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return last;
 }
-__device__ __forceinline__ float part_load(const float* at) {
-    return __uint_as_float(__hip_atomic_load((const uint32_t*)at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+
+// Columns k .. k + 3 of a tile's row, and with the first of them its lse.
+template <class T>
+__device__ __forceinline__ void store_out(const AttendArgs& a, const Tile& t, int kv, int d, int row, int k, f32x4 y,
+                                          float big, float sum) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const int r = t.r0 + row, token = r / a.group, head = kv * a.group + r % a.group;
+    const int pos = t.length - t.count + token;
+    const bool none = key_begin(a, pos) >= key_end(a, t.length, pos);
+    if (none) y = f32x4{0, 0, 0, 0};
+    T* dst = (T*)a.out + (int64_t)(t.row0 + token) * a.o_token + (int64_t)head * a.o_head + k;
+    const T4 z = {(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
+    if (a.wide && k + 4 <= d) {
+        *(T4*)dst = z;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (k + j < d) dst[j] = z[j];
+    }
+    if (a.lse && k == 0)
+        a.lse[(int64_t)(t.row0 + token) * a.heads + head] =
+            none ? -INFINITY : (big + __builtin_amdgcn_logf(sum)) * 0.693147180559945f;
+}
+
+// In a tile's last workgroup: its parts joined in their order, whichever
+// workgroup came last, and stored.  so: 4 * THREADS floats, weight: MOST * RT.
+template <class T, int RT, int D, int THREADS, int MOST>
+__device__ __forceinline__ void join_parts(const AttendArgs& a, const Tile& t, int kv, int d, const Parts& mem,
+                                           int base_at, int parts, float* so, float* weight) {
+    constexpr int OP = D + 4;
+    __shared__ float top_m[RT], top_l[RT];
+    {
+        // the parts' weights, by PER threads a row
+        constexpr int PER = THREADS / RT, EACH = MOST / PER;
+        const int row = min((int)threadIdx.x / PER, t.rows - 1), j = threadIdx.x % PER;
+        f32x2 e[EACH];
+        float big = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < EACH; u++)
+            if (u * PER < parts) e[u] = mem.load2(base_at + (min(j + u * PER, parts - 1) * RT + row) * (OP * 4) + 4 * D);
+#pragma unroll
+        for (int u = 0; u < EACH; u++)
+            if (u * PER < parts) big = fmaxf(big, e[u][0]);
+#pragma unroll
+        for (int x = 1; x < PER; x <<= 1) big = fmaxf(big, __shfl_xor(big, x));
+        const float base = big == -INFINITY ? 0.0f : big;
+#pragma unroll
+        for (int u = 0; u < EACH; u++) {
+            if (j + u * PER < parts) {
+                const float w = e[u][1] * __builtin_amdgcn_exp2f(e[u][0] - base);
+                weight[(j + u * PER) * RT + row] = w;
+                sum += w;
+            }
+        }
+#pragma unroll
+        for (int x = 1; x < PER; x <<= 1) sum += __shfl_xor(sum, x);
+        if (j == 0) {
+            top_m[row] = big;
+            top_l[row] = sum;
+        }
+    }
+    __syncthreads();
+    // 4 columns a thread; where those are few, several threads share one's parts
+    const int items = t.rows * (D / 4);
+    const int groups = items < THREADS ? min(THREADS / items, parts) : 1;
+    const int group = groups > 1 ? (int)threadIdx.x / items : 0;
+    const int s1 = parts * (group + 1) / groups;
+    for (int i = groups > 1 ? (int)threadIdx.x % items : (int)threadIdx.x; i < items; i += THREADS) {
+        const int row = i / (D / 4), k = 4 * (i % (D / 4));
+        f32x4 y = {0, 0, 0, 0};
+        constexpr int AHEAD = 16;
+        if (group < groups) {
+            for (int s0 = parts * group / groups; s0 < s1; s0 += AHEAD) {
+                f32x4 e[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+                    if (s0 + u < s1) e[u] = mem.load4(base_at + ((s0 + u) * RT + row) * (OP * 4) + 4 * k);
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+                    if (s0 + u < s1) y += e[u] * weight[(s0 + u) * RT + row];
+            }
+        }
+        if (groups == 1) store_out<T>(a, t, kv, d, row, k, y / top_l[row], top_m[row], top_l[row]);
+        else if (group < groups) *(f32x4*)&so[4 * threadIdx.x] = y;
+    }
+    if (groups == 1) return;
+    __syncthreads();
+    if ((int)threadIdx.x < items) {
+        const int row = threadIdx.x / (D / 4), k = 4 * (threadIdx.x % (D / 4));
+        f32x4 y = {0, 0, 0, 0};
+        for (int h = 0; h < groups; h++) y += *(const f32x4*)&so[4 * (h * items + threadIdx.x)];
+        store_out<T>(a, t, kv, d, row, k, y / top_l[row], top_m[row], top_l[row]);
+    }
 }
 
 }  // namespace manta

@@ -13,6 +13,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kMaxSplits = 128;
 
+
 // A tile of 16 QT rows (the query heads of a kv head, and tokens); 64 keys a
 // wave at a time.  Scores are k q^T: lane (g, c) = (lane / 16, lane % 16)
 // holds row c's scores of the 16 keys of block g, and those are what the
@@ -36,7 +37,8 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
     typedef typename M::V V8;
     constexpr int D = 32 * DP, DC = DP / 2, DT = 2 * DP, RT = 16 * QT, OP = D + 4;
     constexpr bool ODD = DP % 2 != 0;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
+    const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv = blockIdx.y, split = blockIdx.z;
     const Tile t = my_tile(c, r, a, blockIdx.x, RT);
     if (t.rows == 0) return;
@@ -69,7 +71,7 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[j] = at + j < d ? src[at + j] : (T)0.0f;
             }
-            q[n][s] = x;
+            q[n][s] = a.scale < 0.0f ? -x : x;  // (the scores' order is that of the products)
         }
     }
     {
@@ -109,10 +111,10 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
             if (ODD) k8[i] = *(const u32x2*)(p + 4 * i * c.pitch + 64 * DC + 8 * g);
         }
     };
-    auto load_v = [&](int x) {
-        bad = (unsigned)page_v >= (unsigned)c.pages;
-        const int page = bad ? 0 : page_v;
-        if (bad) cache_report(c, kCacheBadPage, page_v, 0);
+    auto load_v = [&](int x, int entry) {
+        bad = (unsigned)entry >= (unsigned)c.pages;
+        const int page = bad ? 0 : entry;
+        if (bad) cache_report(c, kCacheBadPage, entry, 0);
         ks = kmax[(int64_t)page * c.kv_heads];
         vs = vmax[(int64_t)page * c.kv_heads];
         const int8_t* p = vbase + page * page_codes + ((64 * x + 16 * g) & mask) + col * c.page_tokens;
@@ -135,8 +137,9 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
     if (x < c1) {
         look(x);
         load_k(x);
-        load_v(x);
+        const int entry = page_v;
         look(x + step);
+        load_v(x, entry);
     }
     for (; x < c1; x += step) {
         f32x4 s[QT][4];
@@ -155,7 +158,7 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
         const bool more = x + step < c1;
         if (more) load_k(x + step);
 
-        const float kscale = ks * a.scale;
+        const float kscale = ks * fabsf(a.scale);
         const bool any_bad = __any(bad);
         const bool whole = 64 * x >= lo_all && 64 * x + 63 < hi_all && !any_bad;
         const float R2 = fmaxf(R, max_quarters(finite_or_zero(bad ? 0.0f : vs)));
@@ -165,16 +168,19 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
         half8 p[QT][2];
 #pragma unroll
         for (int n = 0; n < QT; n++) {
-            float e[16], top = -INFINITY;
+            float e[16], top = -INFINITY, factor = kscale;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                e[k] = s[n][k >> 2][k & 3] * kscale;
-                if (!whole) {
-                    const int key = 64 * x + 16 * g + k;
-                    if (key < lo[n] || key >= hi[n] || bad) e[k] = -INFINITY;
-                }
-                top = fmaxf(top, e[k]);
+            for (int k = 0; k < 16; k++) e[k] = s[n][k >> 2][k & 3];
+            const int from = bad ? 16 : lo[n] - (64 * x + 16 * g), to = hi[n] - (64 * x + 16 * g);
+            if (!whole) {
+                // (the scale first: it may be zero or NaN, which a key that is not seen must not meet)
+#pragma unroll
+                for (int k = 0; k < 16; k++) e[k] = k >= from && k < to ? e[k] * kscale : -INFINITY;
+                factor = 1.0f;
             }
+#pragma unroll
+            for (int k = 0; k < 16; k++) top = fmaxf(top, e[k]);
+            top *= factor;
             const float m2 = fmaxf(m[n], max_quarters(top));
             const float base = m2 == -INFINITY ? 0.0f : m2;
             const float keep = __builtin_amdgcn_exp2f(m[n] - base);
@@ -186,15 +192,15 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
             float sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                e[k] = __builtin_amdgcn_exp2f(e[k] - base);
+                e[k] = __builtin_amdgcn_exp2f(e[k] * factor - base);
                 sum += e[k];
-                float f = e[k] * w;
-                if (!whole) {
-                    // nothing of a page that the row does not see, not even its NaN
-                    const int key = 64 * x + 16 * g + k;
-                    if (key < lo[n] || key >= hi[n] || bad) f = 0.0f;
-                }
-                p[n][k >> 3][k & 7] = (_Float16)f;
+                p[n][k >> 3][k & 7] = (_Float16)(e[k] * w);
+            }
+            if (!whole) {
+                // nothing of a page that the row does not see, not even its NaN
+#pragma unroll
+                for (int k = 0; k < 16; k++)
+                    p[n][k >> 3][k & 7] = k >= from && k < to ? p[n][k >> 3][k & 7] : (_Float16)0.0f;
             }
             l[n] = l[n] * keep + sum;
         }
@@ -209,16 +215,17 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
             __builtin_amdgcn_sched_barrier(0);
         }
         if (more) {
-            load_v(x + step);
+            // loads return in order: table entries ahead of the codes, so that
+            // the next k need not wait for this v
+            const int entry = page_v;
             look(x + 2 * step);
+            load_v(x + step, entry);
         }
     }
 
-    // the waves' results joined, one after the other
-    __shared__ float so[RT * OP];
+    // the waves' results joined
+    __shared__ float so[kWaves * RT * OP];
     __shared__ float sm[kWaves][RT], sl[kWaves][RT], sR[kWaves];
-    __shared__ float top_m[RT], top_l[RT];
-    __shared__ int last;
 #pragma unroll
     for (int n = 0; n < QT; n++) {
         l[n] = sum_quarters(l[n]);
@@ -226,120 +233,66 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
             sm[wave][16 * n + col] = m[n];
             sl[wave][16 * n + col] = l[n];
         }
+#pragma unroll
+        for (int i = 0; i < DT; i++) *(f32x4*)&so[(wave * RT + 16 * n + col) * OP + 16 * i + 4 * g] = o[n][i];
     }
     if (lane == 0) sR[wave] = R;
     __syncthreads();
-    float R2 = sR[0];
+    R = sR[0];
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) R2 = fmaxf(R2, sR[w]);
-    if (threadIdx.x < RT) {
-        float big = sm[0][threadIdx.x], sum = 0.0f;
-        for (int w = 1; w < kWaves; w++) big = fmaxf(big, sm[w][threadIdx.x]);
-        const float base = big == -INFINITY ? 0.0f : big;
-        for (int w = 0; w < kWaves; w++) sum += sl[w][threadIdx.x] * __builtin_amdgcn_exp2f(sm[w][threadIdx.x] - base);
-        top_m[threadIdx.x] = big;
-        top_l[threadIdx.x] = sum;
-    }
-    __syncthreads();
-    for (int w = 0; w < kWaves; w++) {
-        if (w == wave) {
-#pragma unroll
-            for (int n = 0; n < QT; n++) {
-                const float big = top_m[16 * n + col];
-                const float f = __builtin_amdgcn_exp2f(m[n] - (big == -INFINITY ? 0.0f : big)) * (R2 > 0.0f ? R / R2 : 1.0f);
-#pragma unroll
-                for (int i = 0; i < DT; i++) {
-                    f32x4* at = (f32x4*)&so[(16 * n + col) * OP + 16 * i + 4 * g];
-                    const f32x4 y = o[n][i] * f;
-                    *at = w == 0 ? y : *at + y;
-                }
-            }
-        }
-        __syncthreads();
-    }
+    for (int w = 1; w < kWaves; w++) R = fmaxf(R, sR[w]);
 
+    // 4 columns a thread: of the output, or of this part
     const int64_t tile = (int64_t)blockIdx.x * gridDim.y + kv;
-    const float unit = R2 / 127.0f;
-    if (parts > 1) {
-        float* part = a.partial + (tile * a.splits + split) * RT * OP;
-        for (int i = threadIdx.x; i < t.rows * D; i += kThreads) {
-            const int row = i / D, k = i % D;
-            const float sum = top_l[row];
-            part_store(part + row * OP + k, sum == 0.0f ? 0.0f : so[row * OP + k] / sum * unit);
-        }
-        if (threadIdx.x < t.rows) {
-            part_store(part + threadIdx.x * OP + D, top_m[threadIdx.x]);
-            part_store(part + threadIdx.x * OP + D + 1, top_l[threadIdx.x]);
-        }
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (threadIdx.x == 0)
-            last = __hip_atomic_fetch_add(&a.tickets[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                   (uint32_t)(parts - 1);
-        __syncthreads();
-        if (!last) return;
-        if (threadIdx.x == 0)
-            __hip_atomic_store(&a.tickets[tile], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // the parts in their order, whichever workgroup came last
-        __shared__ float weight[kMaxSplits * RT];
-        part = a.partial + tile * a.splits * RT * OP;
-        if (threadIdx.x < t.rows) {
-            float big = -INFINITY, sum = 0.0f;
-            for (int s = 0; s < parts; s++) big = fmaxf(big, part_load(part + (s * RT + threadIdx.x) * OP + D));
-            const float base = big == -INFINITY ? 0.0f : big;
-            for (int s = 0; s < parts; s++) {
-                const float* e = part + (s * RT + threadIdx.x) * OP + D;
-                const float w = part_load(e + 1) * __builtin_amdgcn_exp2f(part_load(e) - base);
-                weight[s * RT + threadIdx.x] = w;
-                sum += w;
-            }
-            top_m[threadIdx.x] = big;
-            top_l[threadIdx.x] = sum;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < t.rows * D; i += kThreads) {
-            const int row = i / D, k = i % D;
-            float sum = 0.0f;
-            for (int s = 0; s < parts; s++) sum += weight[s * RT + row] * part_load(part + (s * RT + row) * OP + k);
-            so[row * OP + k] = sum;
-        }
-        __syncthreads();
-    }
-    const float factor = parts > 1 ? 1.0f : unit;
-    constexpr int WIDE = 8;
-    const int pieces = (d + WIDE - 1) / WIDE;
-    for (int i = threadIdx.x; i < t.rows * pieces; i += kThreads) {
-        const int row = i / pieces, at = WIDE * (i % pieces);
-        const int rr = t.r0 + row, token = rr / a.group, head = kv * a.group + rr % a.group;
-        const int pos = t.length - t.count + token;
-        const bool none = key_begin(a, pos) >= key_end(a, t.length, pos);
-        T* dst = (T*)a.out + (int64_t)(t.row0 + token) * a.o_token + (int64_t)head * a.o_head + at;
-        const float sum = top_l[row];
-        V8 y;
+    const Parts parts_mem(a);
+    const int base_at = parts > 1 ? (int)(tile * a.splits) * (RT * OP * 4) : 0;
+    for (int i = threadIdx.x; i < t.rows * (D / 4); i += kThreads) {
+        const int row = i / (D / 4), k = 4 * (i % (D / 4));
+        float big = sm[0][row];
 #pragma unroll
-        for (int j = 0; j < WIDE; j++) {
-            const float v = so[row * OP + at + j] / sum * factor;
-            y[j] = E::store(none ? 0.0f : v);
+        for (int w = 1; w < kWaves; w++) big = fmaxf(big, sm[w][row]);
+        const float base = big == -INFINITY ? 0.0f : big;
+        float sum = 0.0f;
+        f32x4 y = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float f = __builtin_amdgcn_exp2f(sm[w][row] - base);
+            sum += f * sl[w][row];
+            y += *(const f32x4*)&so[(w * RT + row) * OP + k] * (R > 0.0f ? f * (sR[w] / R) : f);
         }
-        if (a.wide && at + WIDE <= d) {
-            *(V8*)dst = y;
+        const float unit = R / 127.0f;
+        if (parts > 1) {
+            const int at = base_at + (split * RT + row) * (OP * 4);
+            parts_mem.store(at + 4 * k, sum == 0.0f ? f32x4{0, 0, 0, 0} : y / sum * unit);
+            if (k == 0) parts_mem.store(at + 4 * D, f32x2{big, sum});
         } else {
-            for (int j = 0; j < WIDE; j++)
-                if (at + j < d) dst[j] = y[j];
+            store_out<T>(a, t, kv, d, row, k, y / sum * unit, big, sum);
         }
-        if (a.lse && at == 0)
-            a.lse[(int64_t)(t.row0 + token) * a.heads + head] =
-                none ? -INFINITY : (top_m[row] + __builtin_amdgcn_logf(sum)) * 0.693147180559945f;
     }
+    if (parts == 1) return;
+    if (!last_part(&a.tickets[tile], parts)) return;
+
+    __shared__ float weight[kMaxSplits * RT];
+    join_parts<T, RT, D, kThreads, kMaxSplits>(a, t, kv, d, parts_mem, base_at, parts, so, weight);
 }
 
 template <class E, int DP, int QT>
 hipError_t launch_few(const CacheView& c, int64_t layer, const RaggedRows& r, AttendArgs a, hipStream_t s) {
     constexpr int RT = 16 * QT, OP = 32 * DP + 4;
     const int64_t slots = tile_slots(r.tokens, r.n, a.group, RT), tiles = slots * c.kv_heads;
-    const int64_t chunks = ((int64_t)a.longest + 63) / 64;
-    int64_t splits = (4 * a.cus + tiles - 1) / tiles;
-    splits = splits < (chunks + kWaves - 1) / kWaves ? splits : (chunks + kWaves - 1) / kWaves;
+    // about: keys that a tile sees in steps of 64, tiles that hold rows
+    const int64_t each = (r.tokens + r.n - 1) / r.n;
+    const int64_t keys = a.window > 0 && a.window + each < a.longest ? a.window + each : a.longest;
+    const int64_t chunks = (keys + 63) / 64;
+    int64_t live = r.n * ((each * a.group + RT - 1) / RT) * c.kv_heads;
+    if (live > tiles) live = tiles;
+    // Two workgroups fit a compute unit.  One sequence: as many as that, all
+    // with the same work (262145 keys of 8 heads of 128: 104 us, with twice as
+    // many 113).  Several, of lengths that the host does not know: twice as
+    // many, so that what the longest leave is small (64 of up to 8192: 155 us
+    // against 167).
+    int64_t splits = ((r.n == 1 ? 2 : 4) * a.cus + live - 1) / live;
+    if (splits > (chunks + kWaves - 1) / kWaves) splits = (chunks + kWaves - 1) / kWaves;
     const int64_t fit = a.partial_bytes / (tiles * RT * OP * 4);
     if (splits > fit) splits = fit;
     if (splits > kMaxSplits) splits = kMaxSplits;
