@@ -88,6 +88,8 @@ struct AttendArgs {
     int splits;  // workgroups that may share a tile's keys
     int rounds;  // steps over the keys that are worth a workgroup
 };
+hipError_t launch_attend_many(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a,
+                              hipStream_t s);
 hipError_t launch_cache_attention(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a,
                                   hipStream_t s);
 

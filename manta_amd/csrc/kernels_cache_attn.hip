@@ -322,7 +322,8 @@ template <class E>
 hipError_t launch_rows(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a, hipStream_t s) {
     const int64_t rows = ((int64_t)r.tokens * a.group + r.n - 1) / r.n;  // a sequence's, about
     if (rows <= 16) return launch_width<E, 1>(c, layer, r, a, s);
-    return launch_width<E, 2>(c, layer, r, a, s);
+    if (rows <= 64) return launch_width<E, 2>(c, layer, r, a, s);
+    return launch_attend_many(c, layer, r, a, s);
 }
 
 }  // namespace

@@ -1,0 +1,380 @@
+// kernels_cache_prompt.hip -- softmax(scale q k^T) v over the 8-bit cache,
+// many rows of a sequence at a time: prompts, and passages after a cached
+// prefix.
+//
+// Bound by the matrix cores and by the softmax between the two products.  A
+// workgroup takes 4 * 32 NB rows (the query heads of a kv head, and tokens)
+// and goes over the keys 64 at a time: the codes become f16 (bf16 for k of
+// bf16 queries) once per workgroup, in LDS, and its four waves multiply them
+// with 32 NB rows each.
+#include "cache_attend.hpp"
+
+namespace manta {
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kMaxSplits = 16;
+constexpr int kKeys = 64;  // of a step
+
+// Scores are k q^T in tiles of 32 keys by 32 rows: lane (h, c) = (lane / 32,
+// lane % 32) holds 16 scores of row c.  Row 8 i + 4 h + j of the k operand is
+// key 16 h + 4 i + j of the 32, so those 16 are keys of one block (of one
+// page, with one scale), and the product v^T p takes its p from the registers
+// that hold them.
+//
+// v is staged as code * (v_max / R), R the largest v_max of the keys, each
+// factor and their product rounded to f16: at most 127, whatever the pages'
+// scales.  The running maximum that weights are taken against moves when a
+// score exceeds it by 8 or more (a weight is at most 256, in f16), so most
+// steps leave the sums alone.
+template <class E, int DP, int NB>
+__global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, int64_t layer, RaggedRows r,
+                                                                  AttendArgs a) {
+    typedef typename E::T T;
+    typedef typename MmaOf<E>::M M;
+    typedef typename M::V V8;
+    constexpr int D = 32 * DP, KS = 2 * DP, RT = kWaves * 32 * NB, OP = D + 4;
+    constexpr int KPITCH = D + 8, VPITCH = kKeys + 8;  // (elements: rows start 4 banks apart)
+    constexpr int CHUNKS = kKeys * D / 16, EACH = (CHUNKS + kThreads - 1) / kThreads;
+    __shared__ T k_lds0[kKeys * KPITCH], k_lds1[kKeys * KPITCH];
+    __shared__ _Float16 v_lds0[D * VPITCH], v_lds1[D * VPITCH];
+    __shared__ float ks_lds0[4], ks_lds1[4];
+    __shared__ int flag_lds0[4], flag_lds1[4];  // 1: no such page, 2: a largest v that is not finite
+    __shared__ float wave_max[kWaves];
+
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // kv heads first: workgroups go round the dies, so a head's stay on one
+    // (of 8 heads), whose cache then holds its keys.  The last rows see the
+    // most keys: they go first.
+    const int kv = blockIdx.x % c.kv_heads, split = blockIdx.y;
+    const int64_t slot = gridDim.x / c.kv_heads - 1 - blockIdx.x / c.kv_heads;
+    const Tile t = my_tile(c, r, a, slot, RT);
+    if (t.rows == 0) return;
+    int c0 = t.begin >> 6, c1 = t.end > t.begin ? (t.end + 63) >> 6 : c0;
+    const int parts = min(max((c1 - c0 + a.rounds - 1) / a.rounds, 1), a.splits);
+    if (split >= parts) return;
+    {
+        const int n = c1 - c0, first = c0;
+        c0 = first + (int)((int64_t)n * split / parts);
+        c1 = first + (int)((int64_t)n * (split + 1) / parts);
+    }
+
+    const int32_t* table = c.tables + (int64_t)t.seq * c.table_pages;
+    const int mask = c.page_tokens - 1, last_page = (t.end - 1) >> c.page_shift;
+    const int64_t page_codes = c.page_codes(), slab0 = c.slab(layer, 0), head_codes = (int64_t)kv * c.page_tokens * c.pitch;
+    const int8_t* kbase = c.k_codes + slab0 * page_codes + head_codes;
+    const int8_t* vbase = c.v_codes + slab0 * page_codes + head_codes;
+    const float* kmax = c.k_max + slab0 * c.kv_heads + kv;
+    const float* vmax = c.v_max + slab0 * c.kv_heads + kv;
+
+    // R
+    float R = 0.0f;
+    if (c1 > c0) {
+        const int to = min((64 * (c1 - 1) + 63) >> c.page_shift, last_page);
+        for (int p = ((64 * c0) >> c.page_shift) + tid; p <= to; p += kThreads) {
+            const int page = table[p];
+            if ((unsigned)page < (unsigned)c.pages) R = fmaxf(R, finite_or_zero(vmax[(int64_t)page * c.kv_heads]));
+        }
+        R = max_quarters(R);
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) R = fmaxf(R, __shfl_xor(R, x));
+        if (lane == 0) wave_max[wave] = R;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) R = fmaxf(R, wave_max[w]);
+    }
+
+    // the wave's rows, clamped (the doubles are not stored), as operands
+    const int d = c.head_dim, wave_row = wave * 32 * NB;
+    V8 q[NB][KS];
+    int lo[NB], hi[NB];
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+        const int row = t.r0 + min(wave_row + 32 * n + col, t.rows - 1);
+        const int token = row / a.group, head = kv * a.group + row % a.group;
+        const int pos = t.length - t.count + token;
+        lo[n] = key_begin(a, pos);
+        hi[n] = key_end(a, t.length, pos);
+        const T* src = (const T*)a.q + (int64_t)(t.row0 + token) * a.q_token + (int64_t)head * a.q_head;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const int at = 16 * s + 8 * h;
+            V8 x;
+            if (a.wide && at + 8 <= d) {
+                x = *(const V8*)(src + at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = at + j < d ? src[at + j] : (T)0.0f;
+            }
+            q[n][s] = a.scale < 0.0f ? -x : x;  // (the scores' order is that of the products)
+        }
+    }
+    // keys that some of the wave's rows see, and that all of them do
+    int some_lo, some_hi, all_lo, all_hi;
+    {
+        const int first = t.length - t.count + (t.r0 + min(wave_row, t.rows - 1)) / a.group;
+        const int last = t.length - t.count + (t.r0 + min(wave_row + 32 * NB - 1, t.rows - 1)) / a.group;
+        some_lo = key_begin(a, first);
+        all_lo = key_begin(a, last);
+        all_hi = key_end(a, t.length, first);
+        some_hi = wave_row < t.rows ? key_end(a, t.length, last) : 0;
+    }
+
+    // codes on their way to LDS
+    u32x4 kc[EACH], vc[EACH];
+    float v_big = 0.0f, k_big = 0.0f;  // block tid % 4: largest v, largest k
+    int flag = 0;
+    auto page_of = [&](int x, int block) { return table[min((64 * x + 16 * block) >> c.page_shift, last_page)]; };
+    int page_k[EACH], page_v;
+    auto look = [&](int x) {
+        x = min(x, c1 - 1);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int key = min((tid + kThreads * i) / KS, kKeys - 1);
+            page_k[i] = page_of(x, key >> 4);
+        }
+        page_v = page_of(x, tid & 3);
+    };
+    auto fetch = [&](int x) {
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int at = tid + kThreads * i, key = at / KS, part = at % KS;
+            const int page = (unsigned)page_k[i] < (unsigned)c.pages ? page_k[i] : 0;
+            if (CHUNKS % kThreads == 0 || at < CHUNKS)
+                kc[i] = *(const u32x4*)(kbase + page * page_codes + ((64 * x + key) & mask) * c.pitch + 16 * part);
+        }
+        const bool bad = (unsigned)page_v >= (unsigned)c.pages;
+        const int page = bad ? 0 : page_v;
+        if (bad && tid < 4) cache_report(c, kCacheBadPage, page_v, 0);
+        k_big = kmax[(int64_t)page * c.kv_heads];
+        v_big = vmax[(int64_t)page * c.kv_heads];
+        flag = bad ? 1 : 0;
+        const int8_t* p = vbase + page * page_codes + ((64 * x + 16 * (tid & 3)) & mask);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int at = tid + kThreads * i;
+            if (CHUNKS % kThreads == 0 || at < CHUNKS) vc[i] = *(const u32x4*)(p + (at >> 2) * c.page_tokens);
+        }
+    };
+    auto stage = [&](T* kl, _Float16* vl, float* ksl, int* fl) {
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int at = tid + kThreads * i, key = at / KS, part = at % KS;
+            const int row = (key & 32) + 8 * ((key >> 2) & 3) + 4 * ((key >> 4) & 1) + (key & 3);
+            if (CHUNKS % kThreads == 0 || at < CHUNKS) {
+                V8* dst = (V8*)(kl + row * KPITCH + 16 * part);
+                dst[0] = M::codes(kc[i][0], kc[i][1]);
+                dst[1] = M::codes(kc[i][2], kc[i][3]);
+            }
+        }
+        // a largest v that is not finite: its codes are left out here, and its weights are made NaN
+        const bool poison = !(v_big < INFINITY);
+        const _Float16 w = (_Float16)(poison || R == 0.0f ? 0.0f : v_big / R);
+        const half8 w8 = {w, w, w, w, w, w, w, w};
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int at = tid + kThreads * i;
+            if (CHUNKS % kThreads == 0 || at < CHUNKS) {
+                half8* dst = (half8*)(vl + (at >> 2) * VPITCH + 16 * (at & 3));
+                dst[0] = codes_f16(vc[i][0], vc[i][1]) * w8;
+                dst[1] = codes_f16(vc[i][2], vc[i][3]) * w8;
+            }
+        }
+        if (tid < 4) {
+            ksl[tid] = k_big * fabsf(a.scale);
+            fl[tid] = flag ? 1 : poison ? 2 : 0;
+        }
+    };
+
+    float m[NB], l[NB];
+    f32x16 o[NB][DP];
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DP; i++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[n][i][k] = 0.0f;
+    }
+
+    auto compute = [&](int x, const T* kl, const _Float16* vl, const float* ksl, const int* fl) {
+        if (64 * x >= some_hi || 64 * x + 63 < some_lo) return;  // (the wave's rows see none of them)
+        f32x16 s[2][NB];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                const V8 k = *(const V8*)(kl + (32 * b + col) * KPITCH + 16 * j + 8 * h);
+#pragma unroll
+                for (int n = 0; n < NB; n++) s[b][n] = M::mma(k, q[n][j], j ? s[b][n] : f32x16{});
+            }
+        }
+        const float ks0 = ksl[h], ks1 = ksl[2 + h];
+        const int f0 = fl[h], f1 = fl[2 + h];
+        const int flags = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
+        const bool whole = 64 * x >= all_lo && 64 * x + 63 < all_hi && flags == 0;
+        half8 p[NB][2][2];
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            float factor0 = ks0, factor1 = ks1, top;
+            const int from = lo[n] - 64 * x - 16 * h, to = hi[n] - 64 * x - 16 * h;
+            if (!whole) {
+                // (the scale first: it may be zero or NaN, which a key that is not seen must not meet)
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    s[0][n][k] = k >= from && k < to && !(f0 & 1) ? s[0][n][k] * ks0 : -INFINITY;
+                    s[1][n][k] = k + 32 >= from && k + 32 < to && !(f1 & 1) ? s[1][n][k] * ks1 : -INFINITY;
+                }
+                factor0 = factor1 = 1.0f;
+            }
+            float top0 = s[0][n][0], top1 = s[1][n][0];
+#pragma unroll
+            for (int k = 1; k < 16; k++) {
+                top0 = fmaxf(top0, s[0][n][k]);
+                top1 = fmaxf(top1, s[1][n][k]);
+            }
+            top = max_halves(fmaxf(top0 * factor0, top1 * factor1));
+            if (__any(top > m[n] + 8.0f)) {
+                const float m2 = fmaxf(m[n], top);
+                const float keep = __builtin_amdgcn_exp2f(m[n] - (m2 == -INFINITY ? 0.0f : m2));
+#pragma unroll
+                for (int i = 0; i < DP; i++) o[n][i] *= keep;
+                l[n] *= keep;
+                m[n] = m2;
+            }
+            const float base = m[n] == -INFINITY ? 0.0f : m[n];
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const float e = __builtin_amdgcn_exp2f(s[b][n][k] * (b ? factor1 : factor0) - base);
+                    sum += e;
+                    p[n][b][k >> 3][k & 7] = (_Float16)e;
+                }
+            }
+            l[n] += sum;
+            if (flags & 2) {
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    if (k >= from && k < to && f0 == 2) p[n][0][k >> 3][k & 7] = (_Float16)NAN;
+                    if (k + 32 >= from && k + 32 < to && f1 == 2) p[n][1][k >> 3][k & 7] = (_Float16)NAN;
+                }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int i = 0; i < DP; i++) {
+                    const half8 v = *(const half8*)(vl + (32 * i + col) * VPITCH + 32 * b + 16 * h + 8 * u);
+#pragma unroll
+                    for (int n = 0; n < NB; n++) o[n][i] = MmaF16::mma(v, p[n][b][u], o[n][i]);
+                }
+            }
+        }
+    };
+
+    if (c0 < c1) {
+        look(c0);
+        fetch(c0);
+        look(c0 + 1);
+        stage(k_lds0, v_lds0, ks_lds0, flag_lds0);
+        if (c0 + 1 < c1) fetch(c0 + 1);
+        for (int x = c0; x < c1; x += 2) {
+            // one barrier a step: what a step stages, the step before it has read
+            look(x + 2);
+            __syncthreads();
+            if (x + 1 < c1) stage(k_lds1, v_lds1, ks_lds1, flag_lds1);
+            if (x + 2 < c1) fetch(x + 2);
+            compute(x, k_lds0, v_lds0, ks_lds0, flag_lds0);
+            if (x + 1 >= c1) break;
+            look(x + 3);
+            __syncthreads();
+            if (x + 2 < c1) stage(k_lds0, v_lds0, ks_lds0, flag_lds0);
+            if (x + 3 < c1) fetch(x + 3);
+            compute(x + 1, k_lds1, v_lds1, ks_lds1, flag_lds1);
+        }
+    }
+
+    const Parts mem(a);
+    const int64_t tile = slot * c.kv_heads + kv;
+    const int base_at = parts > 1 ? (int)(tile * a.splits) * (RT * OP * 4) : 0;
+    const float unit = R / 127.0f;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+        l[n] = sum_halves(l[n]);
+        const int row = wave_row + 32 * n + col;
+        if (row >= t.rows) continue;
+        // (a part that saw no key joins as zeros)
+        const float inv = parts > 1 && l[n] == 0.0f ? 0.0f : unit / l[n];
+        const int at = base_at + (split * RT + row) * (OP * 4);
+#pragma unroll
+        for (int i = 0; i < DP; i++) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int k = 32 * i + 8 * u + 4 * h;
+                const f32x4 y = f32x4{o[n][i][4 * u], o[n][i][4 * u + 1], o[n][i][4 * u + 2], o[n][i][4 * u + 3]} * inv;
+                if (parts > 1) mem.store(at + 4 * k, y);
+                else store_out<T>(a, t, kv, d, row, k, y, m[n], l[n]);
+            }
+        }
+        if (parts > 1 && h == 0) mem.store(at + 4 * D, f32x2{m[n], l[n]});
+    }
+    if (parts == 1) return;
+    if (!last_part(&a.tickets[tile], parts)) return;
+    __shared__ float so[4 * kThreads], weight[kMaxSplits * RT];
+    join_parts<T, RT, D, kThreads, kMaxSplits>(a, t, kv, d, mem, base_at, parts, so, weight);
+}
+
+template <class E, int DP>
+hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, AttendArgs a, hipStream_t s) {
+    constexpr int NB = DP <= 4 ? 2 : 1, RT = kWaves * 32 * NB, OP = 32 * DP + 4;
+    const int64_t slots = tile_slots(r.tokens, r.n, a.group, RT), tiles = slots * c.kv_heads;
+    // about: keys that a tile sees in steps of 64, tiles that hold rows
+    const int64_t each = (r.tokens + r.n - 1) / r.n;
+    const int64_t keys = a.window > 0 && a.window + RT / a.group < a.longest ? a.window + RT / a.group : a.longest;
+    const int64_t chunks = (keys + 63) / 64;
+    int64_t live = r.n * ((each * a.group + RT - 1) / RT) * c.kv_heads;
+    if (live > tiles) live = tiles;
+    int64_t splits = a.cus / live;
+    if (splits > chunks / 8) splits = chunks / 8;
+    const int64_t fit = a.partial_bytes / (tiles * RT * OP * 4);
+    if (splits > fit) splits = fit;
+    if (splits > kMaxSplits) splits = kMaxSplits;
+    if (splits < 1 || tiles > a.ntickets) splits = 1;
+    a.splits = (int)splits;
+    const int64_t rounds = (chunks + splits - 1) / splits;
+    a.rounds = rounds < 8 ? 8 : (int)rounds;
+    attend_many_kernel<E, DP, NB><<<dim3((unsigned)tiles, (unsigned)splits), kThreads, 0, s>>>(c, layer, r, a);
+    return hipGetLastError();
+}
+
+template <class E>
+hipError_t launch_width(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a, hipStream_t s) {
+    switch (c.pitch / 32) {
+        case 1: return launch_many<E, 1>(c, layer, r, a, s);
+        case 2: return launch_many<E, 2>(c, layer, r, a, s);
+        case 3: return launch_many<E, 3>(c, layer, r, a, s);
+        case 4: return launch_many<E, 4>(c, layer, r, a, s);
+        case 5: return launch_many<E, 5>(c, layer, r, a, s);
+        case 6: return launch_many<E, 6>(c, layer, r, a, s);
+        case 7: return launch_many<E, 7>(c, layer, r, a, s);
+        default: return launch_many<E, 8>(c, layer, r, a, s);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_attend_many(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a,
+                              hipStream_t s) {
+    if (a.dtype == MANTA_ROCM_F16) return launch_width<F16>(c, layer, r, a, s);
+    return launch_width<Bf16>(c, layer, r, a, s);
+}
+
+}  // namespace manta
