@@ -13,9 +13,11 @@ namespace manta {
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
 constexpr int kMaxSplits = 16;
+#ifndef KW
+#define KW 8
+#endif
+
 constexpr int kKeys = 64;  // of a step
 
 // Scores are k q^T in tiles of 32 keys by 32 rows: lane (h, c) = (lane / 32,
@@ -29,19 +31,20 @@ constexpr int kKeys = 64;  // of a step
 // scales.  The running maximum that weights are taken against moves when a
 // score exceeds it by 8 or more (a weight is at most 256, in f16), so most
 // steps leave the sums alone.
-template <class E, int DP, int NB>
-__global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, int64_t layer, RaggedRows r,
+template <class E, int DP, int NB, int WAVES, int OCC, bool ONE_PAGE>
+__global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView c, int64_t layer, RaggedRows r,
                                                                   AttendArgs a) {
     typedef typename E::T T;
     typedef typename MmaOf<E>::M M;
     typedef typename M::V V8;
+    constexpr int kThreads = 64 * WAVES, kWaves = WAVES;
     constexpr int D = 32 * DP, KS = 2 * DP, RT = kWaves * 32 * NB, OP = D + 4;
     constexpr int KPITCH = D + 8, VPITCH = kKeys + 8;  // (elements: rows start 4 banks apart)
     constexpr int CHUNKS = kKeys * D / 16, EACH = (CHUNKS + kThreads - 1) / kThreads;
-    __shared__ T k_lds0[kKeys * KPITCH], k_lds1[kKeys * KPITCH];
-    __shared__ _Float16 v_lds0[D * VPITCH], v_lds1[D * VPITCH];
-    __shared__ float ks_lds0[4], ks_lds1[4];
-    __shared__ int flag_lds0[4], flag_lds1[4];  // 1: no such page, 2: a largest v that is not finite
+    __shared__ T k_lds[2][kKeys * KPITCH];
+    __shared__ _Float16 v_lds[2][D * VPITCH];
+    __shared__ float ks_lds[2][4];
+    __shared__ int flag_lds[2][4];  // 1: no such page, 2: a largest v that is not finite
     __shared__ float wave_max[kWaves];
 
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
@@ -64,7 +67,8 @@ __global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, i
 
     const int32_t* table = c.tables + (int64_t)t.seq * c.table_pages;
     const int mask = c.page_tokens - 1, last_page = (t.end - 1) >> c.page_shift;
-    const int64_t page_codes = c.page_codes(), slab0 = c.slab(layer, 0), head_codes = (int64_t)kv * c.page_tokens * c.pitch;
+    const uint32_t page_codes = (uint32_t)c.page_codes();  // (at most 65535 * 128 * 256)
+    const int64_t slab0 = c.slab(layer, 0), head_codes = (int64_t)kv * c.page_tokens * c.pitch;
     const int8_t* kbase = c.k_codes + slab0 * page_codes + head_codes;
     const int8_t* vbase = c.v_codes + slab0 * page_codes + head_codes;
     const float* kmax = c.k_max + slab0 * c.kv_heads + kv;
@@ -128,9 +132,17 @@ __global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, i
     float v_big = 0.0f, k_big = 0.0f;  // block tid % 4: largest v, largest k
     int flag = 0;
     auto page_of = [&](int x, int block) { return table[min((64 * x + 16 * block) >> c.page_shift, last_page)]; };
+    // Vector loads, though their addresses are the same for all: a scalar load
+    // on its way would make every wait for LDS a wait for memory.
+    int zero = 0;
+    asm("" : "+v"(zero));
     int page_k[EACH], page_v;
     auto look = [&](int x) {
         x = min(x, c1 - 1);
+        if (ONE_PAGE) {
+            page_v = page_of(x, zero);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
             const int key = min((tid + kThreads * i) / KS, kKeys - 1);
@@ -139,27 +151,42 @@ __global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, i
         page_v = page_of(x, tid & 3);
     };
     auto fetch = [&](int x) {
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int at = tid + kThreads * i, key = at / KS, part = at % KS;
-            const int page = (unsigned)page_k[i] < (unsigned)c.pages ? page_k[i] : 0;
-            if (CHUNKS % kThreads == 0 || at < CHUNKS)
-                kc[i] = *(const u32x4*)(kbase + page * page_codes + ((64 * x + key) & mask) * c.pitch + 16 * part);
-        }
-        const bool bad = (unsigned)page_v >= (unsigned)c.pages;
-        const int page = bad ? 0 : page_v;
+        x = min(x, c1 - 1);
+        bool bad = (unsigned)page_v >= (unsigned)c.pages;
         if (bad && tid < 4) cache_report(c, kCacheBadPage, page_v, 0);
+        flag = bad;
+        const unsigned page = bad ? 0 : page_v;
         k_big = kmax[(int64_t)page * c.kv_heads];
         v_big = vmax[(int64_t)page * c.kv_heads];
-        flag = bad ? 1 : 0;
-        const int8_t* p = vbase + page * page_codes + ((64 * x + 16 * (tid & 3)) & mask);
+        if (ONE_PAGE) {
+            // one address for the workgroup, and offsets that stay
+            const uint64_t at0 = (uint64_t)__builtin_amdgcn_readfirstlane(page) * page_codes;
+            const int8_t* k = kbase + at0 + ((64 * x) & mask) * c.pitch;
+            const int8_t* v = vbase + at0 + ((64 * x) & mask);
 #pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int at = tid + kThreads * i;
-            if (CHUNKS % kThreads == 0 || at < CHUNKS) vc[i] = *(const u32x4*)(p + (at >> 2) * c.page_tokens);
+            for (int i = 0; i < EACH; i++) {
+                const unsigned at = tid + kThreads * i;
+                if (CHUNKS % kThreads == 0 || at < CHUNKS) {
+                    kc[i] = *(const u32x4*)(k + at * 16u);
+                    vc[i] = *(const u32x4*)(v + ((at >> 2) * (unsigned)c.page_tokens + 16u * (at & 3)));
+                }
+            }
+        } else {
+            const int8_t* v = vbase + (uint64_t)page * page_codes + ((64 * x + 16 * (tid & 3)) & mask);
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const int at = tid + kThreads * i, key = at / KS, part = at % KS;
+                const unsigned pk = (unsigned)page_k[i] < (unsigned)c.pages ? page_k[i] : 0;
+                if (CHUNKS % kThreads == 0 || at < CHUNKS) {
+                    kc[i] = *(const u32x4*)(kbase + (uint64_t)pk * page_codes + ((64 * x + key) & mask) * c.pitch + 16 * part);
+                    vc[i] = *(const u32x4*)(v + (at >> 2) * c.page_tokens);
+                }
+            }
         }
     };
-    auto stage = [&](T* kl, _Float16* vl, float* ksl, int* fl) {
+    auto stage = [&](int buf) {
+        T* kl = k_lds[buf];
+        _Float16* vl = v_lds[buf];
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
             const int at = tid + kThreads * i, key = at / KS, part = at % KS;
@@ -184,8 +211,8 @@ __global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, i
             }
         }
         if (tid < 4) {
-            ksl[tid] = k_big * fabsf(a.scale);
-            fl[tid] = flag ? 1 : poison ? 2 : 0;
+            ks_lds[buf][tid] = k_big * fabsf(a.scale);
+            flag_lds[buf][tid] = flag ? 1 : poison ? 2 : 0;
         }
     };
 
@@ -201,18 +228,45 @@ __global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, i
             for (int k = 0; k < 16; k++) o[n][i][k] = 0.0f;
     }
 
-    auto compute = [&](int x, const T* kl, const _Float16* vl, const float* ksl, const int* fl) {
+    auto compute = [&](int x, int buf) {
+        const T* kl = k_lds[buf];
+        const _Float16* vl = v_lds[buf];
+        const float* ksl = ks_lds[buf];
+        const int* fl = flag_lds[buf];
         if (64 * x >= some_hi || 64 * x + 63 < some_lo) return;  // (the wave's rows see none of them)
+        // Operands are read a group ahead of the products that use them.  (The
+        // scheduler on its own reads two ahead, and every product then waits
+        // for LDS.)
         f32x16 s[2][NB];
+        V8 kf[2][4];
+        auto read_k = [&](int j) {
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < 2; b++)
 #pragma unroll
-            for (int j = 0; j < KS; j++) {
-                const V8 k = *(const V8*)(kl + (32 * b + col) * KPITCH + 16 * j + 8 * h);
+                for (int u = 0; u < 2; u++)
+                    kf[j & 1][2 * u + b] = *(const V8*)(kl + (32 * b + col) * KPITCH + 16 * (2 * j + u) + 8 * h);
+        };
+        read_k(0);
 #pragma unroll
-                for (int n = 0; n < NB; n++) s[b][n] = M::mma(k, q[n][j], j ? s[b][n] : f32x16{});
-            }
+        for (int j = 0; j < DP; j++) {
+            if (j + 1 < DP) read_k(j + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+                        s[b][n] = M::mma(kf[j & 1][2 * u + b], q[n][2 * j + u], j + u ? s[b][n] : f32x16{});
+            __builtin_amdgcn_sched_barrier(0);
         }
+        half8 vf[2][DP];
+        auto read_v = [&](int g) {
+#pragma unroll
+            for (int i = 0; i < DP; i++)
+                vf[g & 1][i] = *(const half8*)(vl + (32 * i + col) * VPITCH + 32 * (g >> 1) + 16 * h + 8 * (g & 1));
+        };
+        read_v(0);
         const float ks0 = ksl[h], ks1 = ksl[2 + h];
         const int f0 = fl[h], f1 = fl[2 + h];
         const int flags = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
@@ -259,24 +313,24 @@ __global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, i
             }
             l[n] += sum;
             if (flags & 2) {
+                int from2 = from, to2 = to;
+                asm("" : "+v"(from2), "+v"(to2));  // (compared anew: nothing of this is kept for the usual step)
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
-                    if (k >= from && k < to && f0 == 2) p[n][0][k >> 3][k & 7] = (_Float16)NAN;
-                    if (k + 32 >= from && k + 32 < to && f1 == 2) p[n][1][k >> 3][k & 7] = (_Float16)NAN;
+                    if (k >= from2 && k < to2 && f0 == 2) p[n][0][k >> 3][k & 7] = (_Float16)NAN;
+                    if (k + 32 >= from2 && k + 32 < to2 && f1 == 2) p[n][1][k >> 3][k & 7] = (_Float16)NAN;
                 }
             }
         }
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
+        for (int g = 0; g < 4; g++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (g < 3) read_v(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+            for (int i = 0; i < DP; i++)
 #pragma unroll
-                for (int i = 0; i < DP; i++) {
-                    const half8 v = *(const half8*)(vl + (32 * i + col) * VPITCH + 32 * b + 16 * h + 8 * u);
-#pragma unroll
-                    for (int n = 0; n < NB; n++) o[n][i] = MmaF16::mma(v, p[n][b][u], o[n][i]);
-                }
-            }
+                for (int n = 0; n < NB; n++) o[n][i] = MmaF16::mma(vf[g & 1][i], p[n][g >> 1][g & 1], o[n][i]);
         }
     };
 
@@ -284,22 +338,21 @@ __global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, i
         look(c0);
         fetch(c0);
         look(c0 + 1);
-        stage(k_lds0, v_lds0, ks_lds0, flag_lds0);
-        if (c0 + 1 < c1) fetch(c0 + 1);
-        for (int x = c0; x < c1; x += 2) {
-            // one barrier a step: what a step stages, the step before it has read
+        stage(0);
+        fetch(c0 + 1);
+        for (int x = c0; x < c1; x++) {
+            // One barrier a step: what a step stages, the step before it has
+            // read.  The last steps fetch and stage the last keys once more:
+            // no branch here, after which every load on its way would be
+            // waited for.
+            const int buf = (x - c0) & 1;
             look(x + 2);
             __syncthreads();
-            if (x + 1 < c1) stage(k_lds1, v_lds1, ks_lds1, flag_lds1);
-            if (x + 2 < c1) fetch(x + 2);
-            compute(x, k_lds0, v_lds0, ks_lds0, flag_lds0);
-            if (x + 1 >= c1) break;
-            look(x + 3);
-            __syncthreads();
-            if (x + 2 < c1) stage(k_lds0, v_lds0, ks_lds0, flag_lds0);
-            if (x + 3 < c1) fetch(x + 3);
-            compute(x + 1, k_lds1, v_lds1, ks_lds1, flag_lds1);
+            stage(buf ^ 1);
+            fetch(x + 2);
+            compute(x, buf);
         }
+        __syncthreads();  // (the staged keys have been used)
     }
 
     const Parts mem(a);
@@ -328,13 +381,17 @@ __global__ __launch_bounds__(kThreads, 1) void attend_many_kernel(CacheView c, i
     }
     if (parts == 1) return;
     if (!last_part(&a.tickets[tile], parts)) return;
-    __shared__ float so[4 * kThreads], weight[kMaxSplits * RT];
-    join_parts<T, RT, D, kThreads, kMaxSplits>(a, t, kv, d, mem, base_at, parts, so, weight);
+    static_assert(sizeof(k_lds) >= (4 * kThreads + kMaxSplits * RT) * 4 || D < 96, "");
+    constexpr bool OVER = D >= 96;
+    __shared__ float join_lds[OVER ? 1 : 4 * kThreads + kMaxSplits * RT];
+    float* so = OVER ? (float*)k_lds : join_lds;
+    join_parts<T, RT, D, kThreads, kMaxSplits>(a, t, kv, d, mem, base_at, parts, so, so + 4 * kThreads);
 }
 
 template <class E, int DP>
 hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, AttendArgs a, hipStream_t s) {
-    constexpr int NB = DP <= 4 ? 2 : 1, RT = kWaves * 32 * NB, OP = 32 * DP + 4;
+    constexpr int NB = 1, WAVES = DP <= 4 ? KW : 4, OCC = DP <= 4 ? 2 : 1;
+    constexpr int kThreads = 64 * WAVES, RT = WAVES * 32 * NB, OP = 32 * DP + 4;
     const int64_t slots = tile_slots(r.tokens, r.n, a.group, RT), tiles = slots * c.kv_heads;
     // about: keys that a tile sees in steps of 64, tiles that hold rows
     const int64_t each = (r.tokens + r.n - 1) / r.n;
@@ -342,7 +399,7 @@ hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, A
     const int64_t chunks = (keys + 63) / 64;
     int64_t live = r.n * ((each * a.group + RT - 1) / RT) * c.kv_heads;
     if (live > tiles) live = tiles;
-    int64_t splits = a.cus / live;
+    int64_t splits = OCC * 4 / WAVES * a.cus / live;
     if (splits > chunks / 8) splits = chunks / 8;
     const int64_t fit = a.partial_bytes / (tiles * RT * OP * 4);
     if (splits > fit) splits = fit;
@@ -351,7 +408,9 @@ hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, A
     a.splits = (int)splits;
     const int64_t rounds = (chunks + splits - 1) / splits;
     a.rounds = rounds < 8 ? 8 : (int)rounds;
-    attend_many_kernel<E, DP, NB><<<dim3((unsigned)tiles, (unsigned)splits), kThreads, 0, s>>>(c, layer, r, a);
+    const dim3 grid((unsigned)tiles, (unsigned)splits);
+    if (c.page_tokens >= kKeys) attend_many_kernel<E, DP, NB, WAVES, OCC, true><<<grid, kThreads, 0, s>>>(c, layer, r, a);
+    else attend_many_kernel<E, DP, NB, WAVES, OCC, false><<<grid, kThreads, 0, s>>>(c, layer, r, a);
     return hipGetLastError();
 }
 
