@@ -286,20 +286,27 @@ hipError_t launch_few(const CacheView& c, int64_t layer, const RaggedRows& r, At
     const int64_t chunks = (keys + 63) / 64;
     int64_t live = r.n * ((each * a.group + RT - 1) / RT) * c.kv_heads;
     if (live > tiles) live = tiles;
-    // Two workgroups fit a compute unit.  One sequence: as many as that, all
-    // with the same work (262145 keys of 8 heads of 128: 104 us, with twice as
-    // many 113).  Several, of lengths that the host does not know: twice as
-    // many, so that what the longest leave is small (64 of up to 8192: 155 us
-    // against 167).
-    int64_t splits = ((r.n == 1 ? 2 : 4) * a.cus + live - 1) / live;
+    // Two workgroups fit a compute unit (of heads wider than 128 or 32 rows,
+    // one).  One sequence: as many as that, all with the same work (262145
+    // keys of 8 heads of 128: 104 us, with twice as many 113).  Several, of
+    // lengths that the host does not know: twice as many, so that what the
+    // longest leave is small (64 of up to 8192: 155 us against 167).
+    constexpr int RESIDENT = DP * QT <= 6 ? 2 : 1;
+    int64_t splits = ((r.n == 1 ? 1 : 2) * RESIDENT * a.cus + live - 1) / live;
     if (splits > (chunks + kWaves - 1) / kWaves) splits = (chunks + kWaves - 1) / kWaves;
+    // joining costs as much as two steps (300 keys: 8.5 us alone, 9.7 in two
+    // parts; 1000: 9.8 in two, 8.8 in four)
+    if (chunks <= 2 * kWaves) splits = 1;
     const int64_t fit = a.partial_bytes / (tiles * RT * OP * 4);
     if (splits > fit) splits = fit;
     if (splits > kMaxSplits) splits = kMaxSplits;
     if (splits < 1 || tiles > a.ntickets) splits = 1;
     a.splits = (int)splits;
     const int64_t rounds = (chunks + kWaves * splits - 1) / (kWaves * splits);
-    a.rounds = rounds < 1 ? 1 : (int)rounds;
+    // wide heads have more to join (16 sequences of up to 8000, 2 heads of 256:
+    // 58 us with steps of 1, 50 of 2, 45 of 3)
+    constexpr int LEAST = DP <= 4 ? 1 : 3;
+    a.rounds = rounds < LEAST ? LEAST : (int)rounds;
     attend_few_kernel<E, DP, QT><<<dim3((unsigned)slots, c.kv_heads, (unsigned)splits), kThreads, 0, s>>>(c, layer, r, a);
     return hipGetLastError();
 }
@@ -322,7 +329,9 @@ template <class E>
 hipError_t launch_rows(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a, hipStream_t s) {
     const int64_t rows = ((int64_t)r.tokens * a.group + r.n - 1) / r.n;  // a sequence's, about
     if (rows <= 16) return launch_width<E, 1>(c, layer, r, a, s);
-    if (rows <= 64) return launch_width<E, 2>(c, layer, r, a, s);
+    // (8 sequences of up to 16000, 64 rows each: 133 us in two tiles here, 106
+    // staged once there; 32 of up to 8000, 40 rows each: 166 either way)
+    if (rows <= 32) return launch_width<E, 2>(c, layer, r, a, s);
     return launch_attend_many(c, layer, r, a, s);
 }
 

@@ -3,10 +3,10 @@
 // prefix.
 //
 // Bound by the matrix cores and by the softmax between the two products.  A
-// workgroup takes 4 * 32 NB rows (the query heads of a kv head, and tokens)
-// and goes over the keys 64 at a time: the codes become f16 (bf16 for k of
-// bf16 queries) once per workgroup, in LDS, and its four waves multiply them
-// with 32 NB rows each.
+// workgroup takes 256 rows (128 of heads wider than 128; the query heads of a
+// kv head, and tokens) and goes over the keys 64 at a time: the codes become
+// f16 (bf16 for k of bf16 queries) once per workgroup, in LDS, and its waves
+// multiply them with 32 rows each.
 #include "cache_attend.hpp"
 
 namespace manta {
@@ -14,9 +14,6 @@ namespace manta {
 namespace {
 
 constexpr int kMaxSplits = 16;
-#ifndef KW
-#define KW 8
-#endif
 
 constexpr int kKeys = 64;  // of a step
 
@@ -31,21 +28,21 @@ constexpr int kKeys = 64;  // of a step
 // scales.  The running maximum that weights are taken against moves when a
 // score exceeds it by 8 or more (a weight is at most 256, in f16), so most
 // steps leave the sums alone.
-template <class E, int DP, int NB, int WAVES, int OCC, bool ONE_PAGE>
+template <class E, int DP, int WAVES, int OCC, bool ONE_PAGE>
 __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView c, int64_t layer, RaggedRows r,
                                                                   AttendArgs a) {
     typedef typename E::T T;
     typedef typename MmaOf<E>::M M;
     typedef typename M::V V8;
-    constexpr int kThreads = 64 * WAVES, kWaves = WAVES;
-    constexpr int D = 32 * DP, KS = 2 * DP, RT = kWaves * 32 * NB, OP = D + 4;
+    constexpr int kThreads = 64 * WAVES;
+    constexpr int D = 32 * DP, KS = 2 * DP, RT = WAVES * 32, OP = D + 4;
     constexpr int KPITCH = D + 8, VPITCH = kKeys + 8;  // (elements: rows start 4 banks apart)
     constexpr int CHUNKS = kKeys * D / 16, EACH = (CHUNKS + kThreads - 1) / kThreads;
     __shared__ T k_lds[2][kKeys * KPITCH];
     __shared__ _Float16 v_lds[2][D * VPITCH];
     __shared__ float ks_lds[2][4];
     __shared__ int flag_lds[2][4];  // 1: no such page, 2: a largest v that is not finite
-    __shared__ float wave_max[kWaves];
+    __shared__ float wave_max[WAVES];
 
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -88,20 +85,19 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
         if (lane == 0) wave_max[wave] = R;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) R = fmaxf(R, wave_max[w]);
+        for (int w = 0; w < WAVES; w++) R = fmaxf(R, wave_max[w]);
     }
 
     // the wave's rows, clamped (the doubles are not stored), as operands
-    const int d = c.head_dim, wave_row = wave * 32 * NB;
-    V8 q[NB][KS];
-    int lo[NB], hi[NB];
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-        const int row = t.r0 + min(wave_row + 32 * n + col, t.rows - 1);
+    const int d = c.head_dim, wave_row = wave * 32;
+    V8 q[KS];
+    int lo, hi;
+    {
+        const int row = t.r0 + min(wave_row + col, t.rows - 1);
         const int token = row / a.group, head = kv * a.group + row % a.group;
         const int pos = t.length - t.count + token;
-        lo[n] = key_begin(a, pos);
-        hi[n] = key_end(a, t.length, pos);
+        lo = key_begin(a, pos);
+        hi = key_end(a, t.length, pos);
         const T* src = (const T*)a.q + (int64_t)(t.row0 + token) * a.q_token + (int64_t)head * a.q_head;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
@@ -113,14 +109,14 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[j] = at + j < d ? src[at + j] : (T)0.0f;
             }
-            q[n][s] = a.scale < 0.0f ? -x : x;  // (the scores' order is that of the products)
+            q[s] = a.scale < 0.0f ? -x : x;  // (the scores' order is that of the products)
         }
     }
     // keys that some of the wave's rows see, and that all of them do
     int some_lo, some_hi, all_lo, all_hi;
     {
         const int first = t.length - t.count + (t.r0 + min(wave_row, t.rows - 1)) / a.group;
-        const int last = t.length - t.count + (t.r0 + min(wave_row + 32 * NB - 1, t.rows - 1)) / a.group;
+        const int last = t.length - t.count + (t.r0 + min(wave_row + 31, t.rows - 1)) / a.group;
         some_lo = key_begin(a, first);
         all_lo = key_begin(a, last);
         all_hi = key_end(a, t.length, first);
@@ -128,6 +124,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     }
 
     // codes on their way to LDS
+    const float inv_R = R > 0.0f ? 1.0f / R : 0.0f;
     u32x4 kc[EACH], vc[EACH];
     float v_big = 0.0f, k_big = 0.0f;  // block tid % 4: largest v, largest k
     int flag = 0;
@@ -199,7 +196,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
         }
         // a largest v that is not finite: its codes are left out here, and its weights are made NaN
         const bool poison = !(v_big < INFINITY);
-        const _Float16 w = (_Float16)(poison || R == 0.0f ? 0.0f : v_big / R);
+        const _Float16 w = (_Float16)(poison ? 0.0f : v_big * inv_R);
         const half8 w8 = {w, w, w, w, w, w, w, w};
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
@@ -216,17 +213,10 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
         }
     };
 
-    float m[NB], l[NB];
-    f32x16 o[NB][DP];
+    float m = -INFINITY, l = 0.0f;
+    f32x16 o[DP];
 #pragma unroll
-    for (int n = 0; n < NB; n++) {
-        m[n] = -INFINITY;
-        l[n] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DP; i++)
-#pragma unroll
-            for (int k = 0; k < 16; k++) o[n][i][k] = 0.0f;
-    }
+    for (int i = 0; i < DP; i++) o[i] = f32x16{};
 
     auto compute = [&](int x, int buf) {
         const T* kl = k_lds[buf];
@@ -237,7 +227,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
         // Operands are read a group ahead of the products that use them.  (The
         // scheduler on its own reads two ahead, and every product then waits
         // for LDS.)
-        f32x16 s[2][NB];
+        f32x16 s[2];
         V8 kf[2][4];
         auto read_k = [&](int j) {
 #pragma unroll
@@ -255,9 +245,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int b = 0; b < 2; b++)
-#pragma unroll
-                    for (int n = 0; n < NB; n++)
-                        s[b][n] = M::mma(kf[j & 1][2 * u + b], q[n][2 * j + u], j + u ? s[b][n] : f32x16{});
+                    s[b] = M::mma(kf[j & 1][2 * u + b], q[2 * j + u], j + u ? s[b] : f32x16{});
             __builtin_amdgcn_sched_barrier(0);
         }
         half8 vf[2][DP];
@@ -271,55 +259,52 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
         const int f0 = fl[h], f1 = fl[2 + h];
         const int flags = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
         const bool whole = 64 * x >= all_lo && 64 * x + 63 < all_hi && flags == 0;
-        half8 p[NB][2][2];
+        half8 p[2][2];
+        float factor0 = ks0, factor1 = ks1;
+        const int from = lo - 64 * x - 16 * h, to = hi - 64 * x - 16 * h;
+        if (!whole) {
+            // (the scale first: it may be zero or NaN, which a key that is not seen must not meet)
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-            float factor0 = ks0, factor1 = ks1, top;
-            const int from = lo[n] - 64 * x - 16 * h, to = hi[n] - 64 * x - 16 * h;
-            if (!whole) {
-                // (the scale first: it may be zero or NaN, which a key that is not seen must not meet)
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    s[0][n][k] = k >= from && k < to && !(f0 & 1) ? s[0][n][k] * ks0 : -INFINITY;
-                    s[1][n][k] = k + 32 >= from && k + 32 < to && !(f1 & 1) ? s[1][n][k] * ks1 : -INFINITY;
-                }
-                factor0 = factor1 = 1.0f;
+            for (int k = 0; k < 16; k++) {
+                s[0][k] = k >= from && k < to && !(f0 & 1) ? s[0][k] * ks0 : -INFINITY;
+                s[1][k] = k + 32 >= from && k + 32 < to && !(f1 & 1) ? s[1][k] * ks1 : -INFINITY;
             }
-            float top0 = s[0][n][0], top1 = s[1][n][0];
+            factor0 = factor1 = 1.0f;
+        }
+        float top0 = s[0][0], top1 = s[1][0];
 #pragma unroll
-            for (int k = 1; k < 16; k++) {
-                top0 = fmaxf(top0, s[0][n][k]);
-                top1 = fmaxf(top1, s[1][n][k]);
+        for (int k = 1; k < 16; k++) {
+            top0 = fmaxf(top0, s[0][k]);
+            top1 = fmaxf(top1, s[1][k]);
+        }
+        const float top = max_halves(fmaxf(top0 * factor0, top1 * factor1));
+        if (__any(top > m + 8.0f)) {
+            const float m2 = fmaxf(m, top);
+            const float keep = __builtin_amdgcn_exp2f(m - (m2 == -INFINITY ? 0.0f : m2));
+#pragma unroll
+            for (int i = 0; i < DP; i++) o[i] *= keep;
+            l *= keep;
+            m = m2;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const float e = __builtin_amdgcn_exp2f(s[b][k] * (b ? factor1 : factor0) - base);
+                sum += e;
+                p[b][k >> 3][k & 7] = (_Float16)e;
             }
-            top = max_halves(fmaxf(top0 * factor0, top1 * factor1));
-            if (__any(top > m[n] + 8.0f)) {
-                const float m2 = fmaxf(m[n], top);
-                const float keep = __builtin_amdgcn_exp2f(m[n] - (m2 == -INFINITY ? 0.0f : m2));
+        }
+        l += sum;
+        if (flags & 2) {
+            int from2 = from, to2 = to;
+            asm("" : "+v"(from2), "+v"(to2));  // (compared anew: nothing of this is kept for the usual step)
 #pragma unroll
-                for (int i = 0; i < DP; i++) o[n][i] *= keep;
-                l[n] *= keep;
-                m[n] = m2;
-            }
-            const float base = m[n] == -INFINITY ? 0.0f : m[n];
-            float sum = 0.0f;
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const float e = __builtin_amdgcn_exp2f(s[b][n][k] * (b ? factor1 : factor0) - base);
-                    sum += e;
-                    p[n][b][k >> 3][k & 7] = (_Float16)e;
-                }
-            }
-            l[n] += sum;
-            if (flags & 2) {
-                int from2 = from, to2 = to;
-                asm("" : "+v"(from2), "+v"(to2));  // (compared anew: nothing of this is kept for the usual step)
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    if (k >= from2 && k < to2 && f0 == 2) p[n][0][k >> 3][k & 7] = (_Float16)NAN;
-                    if (k + 32 >= from2 && k + 32 < to2 && f1 == 2) p[n][1][k >> 3][k & 7] = (_Float16)NAN;
-                }
+            for (int k = 0; k < 16; k++) {
+                if (k >= from2 && k < to2 && f0 == 2) p[0][k >> 3][k & 7] = (_Float16)NAN;
+                if (k + 32 >= from2 && k + 32 < to2 && f1 == 2) p[1][k >> 3][k & 7] = (_Float16)NAN;
             }
         }
 #pragma unroll
@@ -329,8 +314,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < DP; i++)
-#pragma unroll
-                for (int n = 0; n < NB; n++) o[n][i] = MmaF16::mma(vf[g & 1][i], p[n][g >> 1][g & 1], o[n][i]);
+                o[i] = MmaF16::mma(vf[g & 1][i], p[g >> 1][g & 1], o[i]);
         }
     };
 
@@ -359,25 +343,23 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     const int64_t tile = slot * c.kv_heads + kv;
     const int base_at = parts > 1 ? (int)(tile * a.splits) * (RT * OP * 4) : 0;
     const float unit = R / 127.0f;
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-        l[n] = sum_halves(l[n]);
-        const int row = wave_row + 32 * n + col;
-        if (row >= t.rows) continue;
+    l = sum_halves(l);
+    const int row = wave_row + col;
+    if (row < t.rows) {
         // (a part that saw no key joins as zeros)
-        const float inv = parts > 1 && l[n] == 0.0f ? 0.0f : unit / l[n];
+        const float inv = parts > 1 && l == 0.0f ? 0.0f : unit / l;
         const int at = base_at + (split * RT + row) * (OP * 4);
 #pragma unroll
         for (int i = 0; i < DP; i++) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const int k = 32 * i + 8 * u + 4 * h;
-                const f32x4 y = f32x4{o[n][i][4 * u], o[n][i][4 * u + 1], o[n][i][4 * u + 2], o[n][i][4 * u + 3]} * inv;
+                const f32x4 y = f32x4{o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]} * inv;
                 if (parts > 1) mem.store(at + 4 * k, y);
-                else store_out<T>(a, t, kv, d, row, k, y, m[n], l[n]);
+                else store_out<T>(a, t, kv, d, row, k, y, m, l);
             }
         }
-        if (parts > 1 && h == 0) mem.store(at + 4 * D, f32x2{m[n], l[n]});
+        if (parts > 1 && h == 0) mem.store(at + 4 * D, f32x2{m, l});
     }
     if (parts == 1) return;
     if (!last_part(&a.tickets[tile], parts)) return;
@@ -390,8 +372,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
 
 template <class E, int DP>
 hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, AttendArgs a, hipStream_t s) {
-    constexpr int NB = 1, WAVES = DP <= 4 ? KW : 4, OCC = DP <= 4 ? 2 : 1;
-    constexpr int kThreads = 64 * WAVES, RT = WAVES * 32 * NB, OP = 32 * DP + 4;
+    constexpr int WAVES = DP <= 4 ? 8 : 4, OCC = DP <= 4 ? 2 : 1;
+    constexpr int kThreads = 64 * WAVES, RT = WAVES * 32, OP = 32 * DP + 4;
     const int64_t slots = tile_slots(r.tokens, r.n, a.group, RT), tiles = slots * c.kv_heads;
     // about: keys that a tile sees in steps of 64, tiles that hold rows
     const int64_t each = (r.tokens + r.n - 1) / r.n;
@@ -399,7 +381,7 @@ hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, A
     const int64_t chunks = (keys + 63) / 64;
     int64_t live = r.n * ((each * a.group + RT - 1) / RT) * c.kv_heads;
     if (live > tiles) live = tiles;
-    int64_t splits = OCC * 4 / WAVES * a.cus / live;
+    int64_t splits = a.cus / live;  // (one workgroup fits a compute unit)
     if (splits > chunks / 8) splits = chunks / 8;
     const int64_t fit = a.partial_bytes / (tiles * RT * OP * 4);
     if (splits > fit) splits = fit;
@@ -409,8 +391,8 @@ hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, A
     const int64_t rounds = (chunks + splits - 1) / splits;
     a.rounds = rounds < 8 ? 8 : (int)rounds;
     const dim3 grid((unsigned)tiles, (unsigned)splits);
-    if (c.page_tokens >= kKeys) attend_many_kernel<E, DP, NB, WAVES, OCC, true><<<grid, kThreads, 0, s>>>(c, layer, r, a);
-    else attend_many_kernel<E, DP, NB, WAVES, OCC, false><<<grid, kThreads, 0, s>>>(c, layer, r, a);
+    if (c.page_tokens >= kKeys) attend_many_kernel<E, DP, WAVES, OCC, true><<<grid, kThreads, 0, s>>>(c, layer, r, a);
+    else attend_many_kernel<E, DP, WAVES, OCC, false><<<grid, kThreads, 0, s>>>(c, layer, r, a);
     return hipGetLastError();
 }
 
