@@ -198,7 +198,7 @@ SIGNATURES = {
         C.c_int, [_i64, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double, _p, _err]),
     "manta_rocm_rotary_bind": (C.c_int, [_p, _p, _i64, C.c_int, C.c_double, C.POINTER(_p), _err]),
     "manta_rocm_rotary_unbind": (None, [_p]),
-    "manta_rocm_rotary": (C.c_int, [_p, _p, C.c_int, _p, _i64, _i64, C.POINTER(Heads), _i64, C.c_int, _err]),
+    "manta_rocm_rotary": (C.c_int, [_p, _p, C.c_int, _p, _i64, _i64, _p, _i64, C.c_int, _err]),
     "manta_rocm_cache_create": (C.c_int, [_p, C.POINTER(CacheShape), C.POINTER(_p), _err]),
     "manta_rocm_cache_destroy": (None, [_p]),
     "manta_rocm_cache_shape": (C.c_int, [_p, C.POINTER(CacheShape)]),
@@ -213,7 +213,7 @@ SIGNATURES = {
     "manta_rocm_cache_read": (
         C.c_int, [_p, _p, _i64, C.c_int, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _err]),
     "manta_rocm_cache_attention": (
-        C.c_int, [_p, _p, _i64, C.c_int, C.POINTER(Heads), _p, _p, _p, _i64, _i64, C.c_double, C.c_int, _i64, _i64,
+        C.c_int, [_p, _p, _i64, C.c_int, _p, _p, _p, _p, _i64, _i64, C.c_double, C.c_int, _i64, _i64,
                   _err]),
     "manta_rocm_copy": (C.c_int, [_p, _p, _p, C.c_size_t, _err]),
     "manta_rocm_embed_pooled": (

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional
 
 import numpy as np
@@ -22,8 +23,19 @@ from ._lib import call, load
 _KINDS = {"f32": (_lib.F32, 4), "f16": (_lib.F16, 2), "bf16": (_lib.BF16, 2)}
 
 
+_HEADS = struct.Struct("=QQqqqqq").pack  # MantaRocmHeads
+_SEEN: dict = {}  # (name, array type) -> element type
+
+
 def _kind(a, dtype: Optional[str]) -> int:
     """The element type of a device array: given by name, else its own."""
+    known = _SEEN.get((dtype, a.dtype))
+    if known is None:
+        known = _SEEN[(dtype, a.dtype)] = _find_kind(a, dtype)
+    return known
+
+
+def _find_kind(a, dtype: Optional[str]) -> int:
     if dtype is None:
         dtype = {"f": {4: "f32", 2: "f16"}, "u": {2: "f16"}}.get(a.dtype.kind, {}).get(a.dtype.itemsize)
     kind = _KINDS.get(dtype)
@@ -41,7 +53,10 @@ def _rows(name: str, a, heads: Optional[int] = None, dim: Optional[int] = None):
     t, h, d = a.shape
     if (heads is not None and h != heads) or (dim is not None and d != dim):
         raise ValueError("%s must be [tokens, %s, %s] (got %s)" % (name, heads, dim, a.shape))
-    strides = getattr(a, "strides", None)
+    try:
+        strides = a.strides
+    except AttributeError:
+        strides = None
     return (a.addr, t, h, d, h * d, d) if strides is None else (a.addr, t, h, d, strides[0], strides[1])
 
 
@@ -82,26 +97,29 @@ def rotary(rt, rot: Rotary, positions, parts, inverse: bool, dtype: Optional[str
     parts = list(parts)
     if not parts:
         raise ValueError("rotary needs at least one tensor")
-    structs = (_lib.Heads * len(parts))()
+    packed = b""
     kind = _kind(parts[0][0], dtype)
     tokens = dim = None
-    for s, (x, out) in zip(structs, parts):
+    for x, out in parts:
         if _kind(x, dtype) != kind or _kind(out, dtype) != kind:
             raise TypeError("rotary tensors must have one element type")
-        s.x_dev, t, s.heads, d, s.x_token, s.x_head = _rows("x", x)
+        xp, t, h, d, xt, xh = _rows("x", x)
         if tuple(out.shape) != tuple(x.shape):
             raise ValueError("rotary out must be %s (got %s)" % (x.shape, out.shape))
-        s.out_dev, _, _, _, s.out_token, s.out_head = _rows("out", out)
+        op, _, _, _, ot, oh = _rows("out", out)
+        packed += _HEADS(xp, op, h, xt, xh, ot, oh)
         if tokens is None:
             tokens, dim = t, d
         elif (t, d) != (tokens, dim):
             raise ValueError("rotary tensors must agree on tokens and head_dim")
-    call("manta_rocm_rotary", rt.handle, rot.handle, kind, _ints("positions", positions, tokens), tokens, dim, structs,
+    call("manta_rocm_rotary", rt.handle, rot.handle, kind, _ints("positions", positions, tokens), tokens, dim, packed,
          len(parts), 1 if inverse else 0)
 
 
 class _Part:
     """Device memory that a Cache owns, as an array (download, rt.copy)."""
+
+    strides = None
 
     def __init__(self, cache: "Cache", addr: int, shape, dtype):
         self.cache, self.rt, self.addr = cache, cache.rt, addr
@@ -226,14 +244,14 @@ class Cache:
             out = self.rt.empty(q.shape, q.dtype)
         elif tuple(out.shape) != tuple(q.shape) or _kind(out, dtype) != kind:
             raise ValueError("attention out must be %s like q" % (q.shape,))
-        s = _lib.Heads()
-        s.x_dev, t, s.heads, _, s.x_token, s.x_head = _rows("q", q, None, self.head_dim)
-        s.out_dev, _, _, _, s.out_token, s.out_head = _rows("out", out)
+        qp, t, heads, _, qt, qh = _rows("q", q, None, self.head_dim)
+        op, _, _, _, ot, oh = _rows("out", out)
+        packed = _HEADS(qp, op, heads, qt, qh, ot, oh)
         if lse is not None and (lse.dtype != np.float32 or tuple(lse.shape) != tuple(q.shape[:2])
-                                or getattr(lse, "strides", None) is not None):
+                                or lse.strides is not None):
             raise ValueError("attention lse must be a whole f32 array %s" % (q.shape[:2],))
         off, sq, n = self._batch(offsets, seqs)
-        call("manta_rocm_cache_attention", self.rt.handle, self.handle, layer, kind, C.byref(s),
+        call("manta_rocm_cache_attention", self.rt.handle, self.handle, layer, kind, packed,
              None if lse is None else lse.addr, off, sq, n, t,
              1.0 / math.sqrt(self.head_dim) if scale is None else scale, 1 if causal else 0, window,
              self.table_pages * self.page_tokens if longest is None else longest)

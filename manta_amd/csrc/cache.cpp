@@ -319,7 +319,7 @@ int manta_rocm_cache_extend(MantaRocm* rt, MantaRocmCache* c, const int32_t* seq
     });
     if (rc) return rc;
     return launch(rt, "cache_copy", err, [&](hipStream_t s) {
-        return manta::launch_cache_copy(c->view, c->scratch.from, c->scratch.to, c->scratch.count, (int)n, s);
+        return manta::launch_cache_copy(c->view, c->scratch.from, c->scratch.to, c->scratch.count, (int)n, nullptr, s);
     });
 }
 
@@ -354,13 +354,10 @@ int manta_rocm_cache_compact(MantaRocm* rt, MantaRocmCache* c, int32_t* live, ch
     rc = launch(rt, "cache_pages", err,
                 [&](hipStream_t s) { return manta::launch_cache_compact(c->view, c->scratch, live, s); });
     if (rc) return rc;
-    rc = launch(rt, "cache_copy", err, [&](hipStream_t s) {
+    return launch(rt, "cache_copy", err, [&](hipStream_t s) {
         return manta::launch_cache_copy(c->view, c->scratch.from, c->scratch.to, c->scratch.count, (int)c->view.pages,
-                                        s);
+                                        c->scratch.remap, s);
     });
-    if (rc) return rc;
-    return launch(rt, "cache_pages", err,
-                  [&](hipStream_t s) { return manta::launch_cache_remap(c->view, c->scratch, s); });
 }
 
 int manta_rocm_cache_copy_pages(MantaRocm* rt, MantaRocmCache* c, const int32_t* src, const int32_t* dst, int64_t n,
@@ -372,7 +369,7 @@ int manta_rocm_cache_copy_pages(MantaRocm* rt, MantaRocmCache* c, const int32_t*
     if (n == 0) return MANTA_ROCM_OK;
     if (!src || !dst) return fail(err, MANTA_ROCM_ERROR, "cache_copy_pages: nil pointer");
     return launch(rt, "cache_copy", err, [&](hipStream_t s) {
-        return manta::launch_cache_copy(c->view, src, dst, nullptr, (int)n, s);
+        return manta::launch_cache_copy(c->view, src, dst, nullptr, (int)n, nullptr, s);
     });
 }
 

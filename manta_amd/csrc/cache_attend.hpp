@@ -111,39 +111,17 @@ __device__ __forceinline__ int key_begin(const AttendArgs& a, int pos) {
 __device__ __forceinline__ Tile my_tile(const CacheView& c, const RaggedRows& r, const AttendArgs& a, int64_t slot,
                                         int rows) {
     Tile t{};
-    int i, from, to, length = 0;
-    if (r.n <= 64) {
-        // every sequence's offsets and length at once, the one wanted picked
-        // from the lanes: one wait where a search, its result's offsets and
-        // its length are three
-        const int lane = threadIdx.x & 63, j = min(lane, r.n - 1);
-        const int o0 = clamp_row(r.offsets[j], r.tokens), o1 = clamp_row(r.offsets[j + 1], r.tokens);
-        int seq = r.seqs ? r.seqs[j] : j;
-        const bool good = (unsigned)seq < (unsigned)c.seqs;
-        const int len = good ? c.lengths[seq] : -1;
-        const unsigned long long m = __ballot(lane < r.n && tile_base(o0, j, a.group, rows) <= slot) | 1ull;
-        i = 63 - __clzll(m);
-        from = __builtin_amdgcn_readlane(o0, i);
-        to = __builtin_amdgcn_readlane(o1, i);
-        t.seq = __builtin_amdgcn_readlane(seq, i);
-        length = __builtin_amdgcn_readlane(len, i);
-    } else {
-        i = __builtin_amdgcn_readfirstlane(find_slot(r.n, slot, [&](int j) {
-            return tile_base(clamp_row(r.offsets[j], r.tokens), j, a.group, rows);
-        }));
-        from = clamp_row(r.offsets[i], r.tokens);
-        to = clamp_row(r.offsets[i + 1], r.tokens);
-        t.seq = r.seqs ? r.seqs[i] : i;
-        if ((unsigned)t.seq < (unsigned)c.seqs) length = c.lengths[t.seq];
-    }
-    t.row0 = from;
-    t.count = to - from;
-    const int64_t r0 = (slot - tile_base(t.row0, i, a.group, rows)) * rows;
+    const Owner o = find_owner(c, r, slot, [&](int offset, int j) { return tile_base(offset, j, a.group, rows); });
+    t.row0 = o.from;
+    t.count = o.to - o.from;
+    t.seq = o.seq;
+    const int64_t r0 = (slot - tile_base(t.row0, o.i, a.group, rows)) * rows;
     if (t.count <= 0 || r0 < 0 || r0 >= (int64_t)t.count * a.group) return t;
     t.r0 = (int)r0;
     t.rows = (int)min((int64_t)rows, (int64_t)t.count * a.group - r0);
-    if ((unsigned)t.seq < (unsigned)c.seqs) t.length = c.clamp_length(length);
-    else {
+    if (o.length >= 0) {
+        t.length = c.clamp_length(o.length);
+    } else {
         if (threadIdx.x == 0) cache_report(c, kCacheBadSeq, t.seq, 0);
         t.seq = 0;  // length 0: none of its table is read
     }

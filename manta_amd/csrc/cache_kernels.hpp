@@ -62,10 +62,10 @@ hipError_t launch_cache_fork(const CacheView& c, const int32_t* parents, const i
                              const int32_t* tokens, int n, hipStream_t s);
 hipError_t launch_cache_release(const CacheView& c, const int32_t* seqs, const int32_t* keep, int n, hipStream_t s);
 hipError_t launch_cache_compact(const CacheView& c, const PageScratch& w, int32_t* live, hipStream_t s);
-hipError_t launch_cache_remap(const CacheView& c, const PageScratch& w, hipStream_t s);
-// copy pages from[i] -> to[i], i < *count (count in device memory) or n
+// copy pages from[i] -> to[i], i < *count (count in device memory) or n, and
+// with remap [pages] replace the pages that the tables name
 hipError_t launch_cache_copy(const CacheView& c, const int32_t* from, const int32_t* to, const int32_t* count, int n,
-                             hipStream_t s);
+                             const int32_t* remap, hipStream_t s);
 
 struct AttendArgs {
     const void* q;
@@ -135,6 +135,38 @@ __device__ __forceinline__ int find_slot(int n, int64_t slot, Base base) {
         hi = min(hi, lo + step);
     }
     return lo;
+}
+
+struct Owner {  // the sequence that owns a workgroup's slot, as the device arrays have it
+    int i, from, to;  // its place in the batch, its rows
+    int seq, length;  // (length: -1 where seq is out of range)
+};
+template <class Base>
+__device__ __forceinline__ Owner find_owner(const CacheView& c, const RaggedRows& r, int64_t slot, Base base) {
+    Owner o;
+    if (r.n <= 64) {
+        // every sequence's offsets and length at once, the one wanted picked
+        // from the lanes: one wait where a search, its result's offsets and
+        // its length are three
+        const int lane = threadIdx.x & 63, j = min(lane, r.n - 1);
+        const int o0 = clamp_row(r.offsets[j], r.tokens), o1 = clamp_row(r.offsets[j + 1], r.tokens);
+        const int seq = r.seqs ? r.seqs[j] : j;
+        const int length = (unsigned)seq < (unsigned)c.seqs ? max(c.lengths[seq], 0) : -1;
+        const unsigned long long m = __ballot(lane < r.n && base(o0, j) <= slot) | 1ull;
+        o.i = 63 - __clzll(m);
+        o.from = __builtin_amdgcn_readlane(o0, o.i);
+        o.to = __builtin_amdgcn_readlane(o1, o.i);
+        o.seq = __builtin_amdgcn_readlane(seq, o.i);
+        o.length = __builtin_amdgcn_readlane(length, o.i);
+    } else {
+        o.i = __builtin_amdgcn_readfirstlane(
+            find_slot(r.n, slot, [&](int j) { return base(clamp_row(r.offsets[j], r.tokens), j); }));
+        o.from = clamp_row(r.offsets[o.i], r.tokens);
+        o.to = clamp_row(r.offsets[o.i + 1], r.tokens);
+        o.seq = r.seqs ? r.seqs[o.i] : o.i;
+        o.length = (unsigned)o.seq < (unsigned)c.seqs ? max(c.lengths[o.seq], 0) : -1;
+    }
+    return o;
 }
 
 __device__ __forceinline__ void cache_report(const CacheView& c, int kind, int64_t a, int64_t b) {

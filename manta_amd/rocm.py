@@ -38,6 +38,8 @@ class PreparedProjection:
 class DeviceArray:
     """A device allocation with a numpy dtype and shape."""
 
+    strides = None  # C order (View has them)
+
     def __init__(self, rt: "Runtime", shape, dtype):
         self.rt = rt
         self.shape = tuple(int(s) for s in shape)
