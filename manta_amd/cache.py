@@ -141,7 +141,8 @@ class _Part:
 
 class Cache:
     """Keys and values in 8 bits, in pages that sequences share.  k_codes,
-    v_codes, k_max, v_max and book are its device memory."""
+    v_codes, k_max, v_max and book are its device memory, lengths the part of
+    book that a loop on the device takes positions from."""
 
     def __init__(self, rt, layers, pages, page_tokens, kv_heads, head_dim, seqs, table_pages):
         self.rt = rt
@@ -161,6 +162,7 @@ class Cache:
         self.k_max = _Part(self, b.k_max, lead, np.float32)
         self.v_max = _Part(self, b.v_max, lead, np.float32)
         self.book = _Part(self, b.book, (b.book_count,), np.int32)
+        self.lengths = _Part(self, b.book + 4 * self.pages, (self.seqs,), np.int32)
 
     def close(self) -> None:
         if self.handle is not None and self.handle.value:
