@@ -23,9 +23,11 @@ constexpr int kKeys = 64;  // of a step
 // page, with one scale), and the product v^T p takes its p from the registers
 // that hold them.
 //
-// v is staged as code * (v_max / R), R the largest v_max of the keys, each
-// factor and their product rounded to f16: at most 127, whatever the pages'
-// scales.  The running maximum that weights are taken against moves when a
+// A weight is multiplied by v_max / R, R the largest v_max of the keys, and
+// the product is rounded to f16 (half a step, 2^-11, as the operand of an f32
+// sum): whatever the pages' scales, codes stay exact.  (Codes scaled as they
+// are staged would be rounded with their scale: 1.8 times the error of an f16
+// result.)  The running maximum that weights are taken against moves when a
 // score exceeds it by 8 or more (a weight is at most 256, in f16), so most
 // steps leave the sums alone.
 template <class E, int DP, int WAVES, int OCC, bool ONE_PAGE>
@@ -40,7 +42,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     constexpr int CHUNKS = kKeys * D / 16, EACH = (CHUNKS + kThreads - 1) / kThreads;
     __shared__ T k_lds[2][kKeys * KPITCH];
     __shared__ _Float16 v_lds[2][D * VPITCH];
-    __shared__ float ks_lds[2][4];
+    __shared__ float ks_lds[2][4], vs_lds[2][4];
     __shared__ int flag_lds[2][4];  // 1: no such page, 2: a largest v that is not finite
     __shared__ float wave_max[WAVES];
 
@@ -194,21 +196,20 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
                 dst[1] = M::codes(kc[i][2], kc[i][3]);
             }
         }
-        // a largest v that is not finite: its codes are left out here, and its weights are made NaN
-        const bool poison = !(v_big < INFINITY);
-        const _Float16 w = (_Float16)(poison ? 0.0f : v_big * inv_R);
-        const half8 w8 = {w, w, w, w, w, w, w, w};
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
             const int at = tid + kThreads * i;
             if (CHUNKS % kThreads == 0 || at < CHUNKS) {
                 half8* dst = (half8*)(vl + (at >> 2) * VPITCH + 16 * (at & 3));
-                dst[0] = codes_f16(vc[i][0], vc[i][1]) * w8;
-                dst[1] = codes_f16(vc[i][2], vc[i][3]) * w8;
+                dst[0] = codes_f16(vc[i][0], vc[i][1]);
+                dst[1] = codes_f16(vc[i][2], vc[i][3]);
             }
         }
         if (tid < 4) {
+            // (a largest v that is not finite: weights of 0, which become NaN where they are seen)
+            const bool poison = !(v_big < INFINITY);
             ks_lds[buf][tid] = k_big * fabsf(a.scale);
+            vs_lds[buf][tid] = poison ? 0.0f : v_big * inv_R;
             flag_lds[buf][tid] = flag ? 1 : poison ? 2 : 0;
         }
     };
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
                 vf[g & 1][i] = *(const half8*)(vl + (32 * i + col) * VPITCH + 32 * (g >> 1) + 16 * h + 8 * (g & 1));
         };
         read_v(0);
-        const float ks0 = ksl[h], ks1 = ksl[2 + h];
+        const float ks0 = ksl[h], ks1 = ksl[2 + h], w0 = vs_lds[buf][h], w1 = vs_lds[buf][2 + h];
         const int f0 = fl[h], f1 = fl[2 + h];
         const int flags = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
         const bool whole = 64 * x >= all_lo && 64 * x + 63 < all_hi && flags == 0;
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             for (int k = 0; k < 16; k++) {
                 const float e = __builtin_amdgcn_exp2f(s[b][k] * (b ? factor1 : factor0) - base);
                 sum += e;
-                p[b][k >> 3][k & 7] = (_Float16)e;
+                p[b][k >> 3][k & 7] = (_Float16)(e * (b ? w1 : w0));
             }
         }
         l += sum;
