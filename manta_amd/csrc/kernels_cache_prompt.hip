@@ -23,11 +23,11 @@ constexpr int kKeys = 64;  // of a step
 // page, with one scale), and the product v^T p takes its p from the registers
 // that hold them.
 //
-// A weight is multiplied by v_max / R, R the largest v_max of the keys, and
-// the product is rounded to f16 (half a step, 2^-11, as the operand of an f32
-// sum): whatever the pages' scales, codes stay exact.  (Codes scaled as they
-// are staged would be rounded with their scale: 1.8 times the error of an f16
-// result.)  The running maximum that weights are taken against moves when a
+// A weight carries v_max / R, R the largest v_max of the keys, in its exponent
+// (the sum of the weights is freed of it block by block), and is rounded to
+// f16 (half a step, 2^-11, as the operand of an f32 sum): whatever the pages'
+// scales, codes stay exact.  (Codes scaled as they are staged would be rounded
+// with their scale: 1.8 times the rounding error of an f16 result, not 1.4.)  The running maximum that weights are taken against moves when a
 // score exceeds it by 8 or more (a weight is at most 256, in f16), so most
 // steps leave the sums alone.
 template <class E, int DP, int WAVES, int OCC, bool ONE_PAGE>
@@ -42,8 +42,9 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     constexpr int CHUNKS = kKeys * D / 16, EACH = (CHUNKS + kThreads - 1) / kThreads;
     __shared__ T k_lds[2][kKeys * KPITCH];
     __shared__ _Float16 v_lds[2][D * VPITCH];
-    __shared__ float ks_lds[2][4], vs_lds[2][4];
-    __shared__ int flag_lds[2][4];  // 1: no such page, 2: a largest v that is not finite
+    // of each block of 16 keys: the factor of its scores; log2 of its weights'
+    // v_max / R, and the inverse of that; 1: no such page, 2: a largest v that is not finite
+    __shared__ f32x4 block_lds[2][4];
     __shared__ float wave_max[WAVES];
 
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
@@ -206,11 +207,13 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             }
         }
         if (tid < 4) {
-            // (a largest v that is not finite: weights of 0, which become NaN where they are seen)
+            // (a largest v below 2^-40 R, or 0: as if it were 2^-40 R, whose
+            // weights are zero in f16 too.  One that is not finite: the same,
+            // and its weights become NaN where they are seen.)
             const bool poison = !(v_big < INFINITY);
-            ks_lds[buf][tid] = k_big * fabsf(a.scale);
-            vs_lds[buf][tid] = poison ? 0.0f : v_big * inv_R;
-            flag_lds[buf][tid] = flag ? 1 : poison ? 2 : 0;
+            const float log_w = poison ? 0.0f : __builtin_amdgcn_logf(fmaxf(v_big * inv_R, 0x1p-40f));
+            block_lds[buf][tid] = f32x4{k_big * fabsf(a.scale), log_w, __builtin_amdgcn_exp2f(-log_w),
+                                        flag ? 1.0f : poison ? 2.0f : 0.0f};
         }
     };
 
@@ -222,8 +225,6 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     auto compute = [&](int x, int buf) {
         const T* kl = k_lds[buf];
         const _Float16* vl = v_lds[buf];
-        const float* ksl = ks_lds[buf];
-        const int* fl = flag_lds[buf];
         if (64 * x >= some_hi || 64 * x + 63 < some_lo) return;  // (the wave's rows see none of them)
         // Operands are read a group ahead of the products that use them.  (The
         // scheduler on its own reads two ahead, and every product then waits
@@ -256,10 +257,10 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
                 vf[g & 1][i] = *(const half8*)(vl + (32 * i + col) * VPITCH + 32 * (g >> 1) + 16 * h + 8 * (g & 1));
         };
         read_v(0);
-        const float ks0 = ksl[h], ks1 = ksl[2 + h], w0 = vs_lds[buf][h], w1 = vs_lds[buf][2 + h];
-        const int f0 = fl[h], f1 = fl[2 + h];
-        const int flags = __builtin_amdgcn_readfirstlane(fl[0] | fl[1] | fl[2] | fl[3]);
-        const bool whole = 64 * x >= all_lo && 64 * x + 63 < all_hi && flags == 0;
+        const f32x4 block0 = block_lds[buf][h], block1 = block_lds[buf][2 + h];
+        const float ks0 = block0[0], ks1 = block1[0];
+        const bool odd = __any(block0[3] != 0.0f || block1[3] != 0.0f);
+        const bool whole = 64 * x >= all_lo && 64 * x + 63 < all_hi && !odd;
         half8 p[2][2];
         float factor0 = ks0, factor1 = ks1;
         const int from = lo - 64 * x - 16 * h, to = hi - 64 * x - 16 * h;
@@ -267,8 +268,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             // (the scale first: it may be zero or NaN, which a key that is not seen must not meet)
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                s[0][k] = k >= from && k < to && !(f0 & 1) ? s[0][k] * ks0 : -INFINITY;
-                s[1][k] = k + 32 >= from && k + 32 < to && !(f1 & 1) ? s[1][k] * ks1 : -INFINITY;
+                s[0][k] = k >= from && k < to && block0[3] != 1.0f ? s[0][k] * ks0 : -INFINITY;
+                s[1][k] = k + 32 >= from && k + 32 < to && block1[3] != 1.0f ? s[1][k] * ks1 : -INFINITY;
             }
             factor0 = factor1 = 1.0f;
         }
@@ -288,24 +289,25 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             m = m2;
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f;
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < 2; b++) {
+            const float factor = b ? factor1 : factor0, shift = (b ? block1[1] : block0[1]) - base;
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                const float e = __builtin_amdgcn_exp2f(s[b][k] * (b ? factor1 : factor0) - base);
-                sum += e;
-                p[b][k >> 3][k & 7] = (_Float16)(e * (b ? w1 : w0));
+                const float e = __builtin_amdgcn_exp2f(s[b][k] * factor + shift);
+                sum[b] += e;
+                p[b][k >> 3][k & 7] = (_Float16)e;
             }
         }
-        l += sum;
-        if (flags & 2) {
+        l += sum[0] * block0[2] + sum[1] * block1[2];
+        if (odd) {
             int from2 = from, to2 = to;
             asm("" : "+v"(from2), "+v"(to2));  // (compared anew: nothing of this is kept for the usual step)
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                if (k >= from2 && k < to2 && f0 == 2) p[0][k >> 3][k & 7] = (_Float16)NAN;
-                if (k + 32 >= from2 && k + 32 < to2 && f1 == 2) p[1][k >> 3][k & 7] = (_Float16)NAN;
+                if (k >= from2 && k < to2 && block0[3] == 2.0f) p[0][k >> 3][k & 7] = (_Float16)NAN;
+                if (k + 32 >= from2 && k + 32 < to2 && block1[3] == 2.0f) p[1][k >> 3][k & 7] = (_Float16)NAN;
             }
         }
 #pragma unroll
