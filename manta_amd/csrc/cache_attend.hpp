@@ -194,9 +194,9 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, const Tile& t, in
 
 // In a tile's last workgroup: its parts joined in their order, whichever
 // workgroup came last, and stored.  so: 4 * THREADS floats, weight: MOST * RT.
-template <class T, int RT, int D, int THREADS, int MOST>
+template <class T, int RT, int D, int THREADS, int MOST, class At>
 __device__ __forceinline__ void join_parts(const AttendArgs& a, const Tile& t, int kv, int d, const Parts& mem,
-                                           int base_at, int parts, float* so, float* weight) {
+                                           At part_at, int parts, float* so, float* weight) {
     constexpr int OP = D + 4;
     __shared__ float top_m[RT], top_l[RT];
     {
@@ -207,7 +207,7 @@ __device__ __forceinline__ void join_parts(const AttendArgs& a, const Tile& t, i
         float big = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < EACH; u++)
-            if (u * PER < parts) e[u] = mem.load2(base_at + (min(j + u * PER, parts - 1) * RT + row) * (OP * 4) + 4 * D);
+            if (u * PER < parts) e[u] = mem.load2(part_at(min(j + u * PER, parts - 1)) + row * (OP * 4) + 4 * D);
 #pragma unroll
         for (int u = 0; u < EACH; u++)
             if (u * PER < parts) big = fmaxf(big, e[u][0]);
@@ -244,7 +244,7 @@ __device__ __forceinline__ void join_parts(const AttendArgs& a, const Tile& t, i
                 f32x4 e[AHEAD];
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++)
-                    if (s0 + u < s1) e[u] = mem.load4(base_at + ((s0 + u) * RT + row) * (OP * 4) + 4 * k);
+                    if (s0 + u < s1) e[u] = mem.load4(part_at(s0 + u) + row * (OP * 4) + 4 * k);
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++)
                     if (s0 + u < s1) y += e[u] * weight[(s0 + u) * RT + row];

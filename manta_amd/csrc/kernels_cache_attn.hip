@@ -37,8 +37,19 @@ __device__ __forceinline__ V stream(const V* p) {
 // (v_max / R) is at most 1 and is rounded to f16 (half a step, 2^-11, as the
 // operand of an f32 sum; codes are exact).  The pages' own scales would leave
 // f16's range, and the codes times them would be rounded once more.
+struct Share {  // a workgroup's part of a tile's keys
+    int kv;
+    int c0, c1;         // the keys 64 c0 .. 64 c1 - 1,
+    int first, step;    // of which wave w takes c0 + first + w, that + step, ...
+    int part, parts;    // which of the tile's parts this is
+    uint32_t* ticket;
+    int at0, at1, pitch;  // where part 0 goes in a.partial (bytes), and parts 1, 2, ...
+    __device__ __forceinline__ int at(int s) const { return s == 0 ? at0 : at1 + (s - 1) * pitch; }
+};
+
 template <class E, int DP, int QT>
-__global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_kernel(CacheView c, int64_t layer, RaggedRows r, AttendArgs a) {
+__device__ __forceinline__ void attend_share(const CacheView& c, int64_t layer, const AttendArgs& a, const Tile& t,
+                                             const Share& sh) {
     typedef typename E::T T;
     typedef typename MmaOf<E>::M M;
     typedef typename M::V V8;
@@ -46,14 +57,7 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
     constexpr bool ODD = DP % 2 != 0;
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kv = blockIdx.y, split = blockIdx.z;
-    const Tile t = my_tile(c, r, a, blockIdx.x, RT);
-    if (t.rows == 0) return;
-    const int c0 = t.begin >> 6, c1 = t.end > t.begin ? (t.end + 63) >> 6 : c0;
-    // workgroups that share the keys, `rounds` steps of theirs or more for each
-    const int want = (c1 - c0 + kWaves * a.rounds - 1) / (kWaves * a.rounds);
-    const int parts = min(max(want, 1), a.splits);
-    if (split >= parts) return;
+    const int kv = sh.kv, c1 = sh.c1, parts = sh.parts;
 
     // the rows, clamped (the doubles are not stored), as operands
     const int d = c.head_dim;
@@ -91,7 +95,8 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
 
     const int32_t* table = c.tables + (int64_t)t.seq * c.table_pages;
     const int mask = c.page_tokens - 1, last_page = (t.end - 1) >> c.page_shift;
-    const int64_t page_codes = c.page_codes(), slab0 = c.slab(layer, 0), head_codes = (int64_t)kv * c.page_tokens * c.pitch;
+    const uint32_t page_codes = (uint32_t)c.page_codes();  // (at most 65535 * 128 * 256)
+    const int64_t slab0 = c.slab(layer, 0), head_codes = (int64_t)kv * c.page_tokens * c.pitch;
     const int8_t* kbase = c.k_codes + slab0 * page_codes + head_codes;
     const int8_t* vbase = c.v_codes + slab0 * page_codes + head_codes;
     const float* kmax = c.k_max + slab0 * c.kv_heads + kv;
@@ -109,8 +114,8 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
         page_v = table[min((64 * x + 16 * g) >> c.page_shift, last_page)];
     };
     auto load_k = [&](int x) {
-        const int page = (unsigned)page_k < (unsigned)c.pages ? page_k : 0;
-        const int8_t* p = kbase + page * page_codes + (((64 * x + 16 * kb) & mask) + (col & 3)) * c.pitch;
+        const unsigned page = (unsigned)page_k < (unsigned)c.pages ? page_k : 0;
+        const int8_t* p = kbase + (uint64_t)page * page_codes + (((64 * x + 16 * kb) & mask) + (col & 3)) * c.pitch;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
 #pragma unroll
@@ -120,11 +125,11 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
     };
     auto load_v = [&](int x, int entry) {
         bad = (unsigned)entry >= (unsigned)c.pages;
-        const int page = bad ? 0 : entry;
+        const unsigned page = bad ? 0 : entry;
         if (bad) cache_report(c, kCacheBadPage, entry, 0);
         ks = kmax[(int64_t)page * c.kv_heads];
         vs = vmax[(int64_t)page * c.kv_heads];
-        const int8_t* p = vbase + page * page_codes + ((64 * x + 16 * g) & mask) + col * c.page_tokens;
+        const int8_t* p = vbase + (uint64_t)page * page_codes + ((64 * x + 16 * g) & mask) + col * c.page_tokens;
 #pragma unroll
         for (int i = 0; i < DT; i++) v16[i] = stream<QT == 1>((const u32x4*)(p + 16 * i * c.page_tokens));
     };
@@ -139,8 +144,8 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
         for (int i = 0; i < DT; i++) o[n][i] = f32x4{0, 0, 0, 0};
     }
 
-    const int step = kWaves * parts;
-    int x = c0 + wave + kWaves * split;
+    const int step = sh.step;
+    int x = sh.c0 + sh.first + wave;
     if (x < c1) {
         look(x);
         load_k(x);
@@ -250,9 +255,7 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
     for (int w = 1; w < kWaves; w++) R = fmaxf(R, sR[w]);
 
     // 4 columns a thread: of the output, or of this part
-    const int64_t tile = (int64_t)blockIdx.x * gridDim.y + kv;
     const Parts parts_mem(a);
-    const int base_at = parts > 1 ? (int)(tile * a.splits) * (RT * OP * 4) : 0;
     for (int i = threadIdx.x; i < t.rows * (D / 4); i += kThreads) {
         const int row = i / (D / 4), k = 4 * (i % (D / 4));
         float big = sm[0][row];
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
         }
         const float unit = R / 127.0f;
         if (parts > 1) {
-            const int at = base_at + (split * RT + row) * (OP * 4);
+            const int at = sh.at(sh.part) + row * (OP * 4);
             parts_mem.store(at + 4 * k, sum == 0.0f ? f32x4{0, 0, 0, 0} : y / sum * unit);
             if (k == 0) parts_mem.store(at + 4 * D, f32x2{big, sum});
         } else {
@@ -277,10 +280,140 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
         }
     }
     if (parts == 1) return;
-    if (!last_part(&a.tickets[tile], parts)) return;
+    if (!last_part(sh.ticket, parts)) return;
 
     __shared__ float weight[kMaxSplits * RT];
-    join_parts<T, RT, D, kThreads, kMaxSplits>(a, t, kv, d, parts_mem, base_at, parts, so, weight);
+    join_parts<T, RT, D, kThreads, kMaxSplits>(a, t, kv, d, parts_mem, [&](int s) { return sh.at(s); }, parts, so, weight);
+}
+
+// A workgroup a tile and part: parts of `rounds` steps or more.
+template <class E, int DP, int QT>
+__global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_kernel(CacheView c, int64_t layer,
+                                                                                  RaggedRows r, AttendArgs a) {
+    constexpr int RT = 16 * QT, BYTES = RT * (32 * DP + 4) * 4;
+    const Tile t = my_tile(c, r, a, blockIdx.x, RT);
+    if (t.rows == 0) return;
+    Share sh;
+    sh.kv = blockIdx.y;
+    sh.c0 = t.begin >> 6;
+    sh.c1 = t.end > t.begin ? (t.end + 63) >> 6 : sh.c0;
+    const int want = (sh.c1 - sh.c0 + kWaves * a.rounds - 1) / (kWaves * a.rounds);
+    sh.parts = min(max(want, 1), a.splits);
+    sh.part = blockIdx.z;
+    if (sh.part >= sh.parts) return;
+    sh.first = kWaves * sh.part;
+    sh.step = kWaves * sh.parts;
+    const int64_t tile = (int64_t)blockIdx.x * gridDim.y + sh.kv;
+    sh.ticket = a.tickets + (sh.parts > 1 ? tile : 0);
+    sh.at0 = sh.parts > 1 ? (int)(tile * a.splits) * BYTES : 0;
+    sh.at1 = sh.at0 + BYTES;
+    sh.pitch = BYTES;
+    attend_share<E, DP, QT>(c, layer, a, t, sh);
+}
+
+// The same work cut evenly: one workgroup a place on the card, each with as
+// many steps as the others of the sequences' steps laid end to end, whatever
+// their lengths (64 sequences of up to 8192: 149 us by tiles, 131 so).  At
+// most 64 sequences, one a lane, so that every workgroup can lay them out by
+// itself.
+template <class E, int DP>
+__global__ __launch_bounds__(kThreads, DP <= 6 ? 2 : 1) void attend_even_kernel(CacheView c, int64_t layer, RaggedRows r,
+                                                                              AttendArgs a) {
+    constexpr int QT = 1, RT = 16 * QT, BYTES = RT * (32 * DP + 4) * 4;
+    const int lane = threadIdx.x & 63, j = min(lane, r.n - 1);
+    const int o0 = clamp_row(r.offsets[j], r.tokens), o1 = clamp_row(r.offsets[j + 1], r.tokens);
+    const int seq = r.seqs ? r.seqs[j] : j;
+    const bool good = (unsigned)seq < (unsigned)c.seqs;
+    const int length = good ? c.clamp_length(c.lengths[seq]) : 0;
+    // a tile's steps of 64 kWaves keys (1 for one that sees nothing: its rows are zeros)
+    int tiles = 0, steps = 1, c_lo = 0;
+    if (lane < r.n && o1 > o0) {
+        if (!good && blockIdx.x == 0 && threadIdx.x < 64) cache_report(c, kCacheBadSeq, seq, 0);
+        tiles = (int)(((int64_t)(o1 - o0) * a.group + RT - 1) / RT);
+        c_lo = key_begin(a, length - (o1 - o0)) >> 6;
+        steps = max(1, (((length + 63) >> 6) - c_lo + kWaves - 1) / kWaves);
+    }
+    int64_t below = (int64_t)tiles * steps;
+    int tiles_below = tiles, most = steps;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+        const int64_t y = __shfl_up((long long)below, x);
+        const int z = __shfl_up(tiles_below, x);
+        if (lane >= x) {
+            below += y;
+            tiles_below += z;
+        }
+        most = max(most, __shfl_xor(most, x));
+    }
+    // (kept in LDS: the registers are for the keys)
+    __shared__ int64_t s_below[64];
+    __shared__ int s_from[64], s_count[64], s_seq[64], s_length[64], s_lo[64], s_steps[64], s_tiles[64];
+    __shared__ int64_t s_total;
+    __shared__ int s_all, s_most;
+    if (threadIdx.x < 64) {
+        s_below[lane] = tiles > 0 ? below - (int64_t)tiles * steps : INT64_MAX;
+        s_from[lane] = o0;
+        s_count[lane] = o1 - o0;
+        s_seq[lane] = good ? seq : 0;
+        s_length[lane] = length;
+        s_lo[lane] = c_lo;
+        s_steps[lane] = steps;
+        s_tiles[lane] = tiles_below - tiles;
+        if (lane == 63) {
+            s_total = below;  // of a kv head
+            s_all = tiles_below;
+            s_most = most;
+        }
+    }
+    __syncthreads();
+    auto uniform = [](int64_t x) {
+        const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 | lo);
+    };
+    const int64_t total = uniform(s_total), all = total * c.kv_heads;
+    // each workgroup's steps: no tile in more parts than can be joined
+    const int64_t quota = uniform(max((all + gridDim.x - 1) / gridDim.x, (int64_t)(s_most / (kMaxSplits - 2) + 1)));
+    int64_t at = blockIdx.x * quota;
+    const int64_t end = min(at + quota, all);
+    while (at < end) {
+        const int kv = __builtin_amdgcn_readfirstlane((int)(at / total));
+        const int64_t rest = at - kv * total;
+        const int i = 63 - __clzll(__ballot(s_below[lane] <= rest) | 1ull);
+        const int n = __builtin_amdgcn_readfirstlane(s_steps[i]);
+        const int64_t in = rest - uniform(s_below[i]);
+        const int ordinal = __builtin_amdgcn_readfirstlane((int)(in / n));
+        const int s0 = (int)(in - (int64_t)ordinal * n);
+        const int s1 = (int)min((int64_t)n, s0 + (end - at));
+        const int64_t from = at - s0;  // the tile's first step
+        Tile t{};
+        t.row0 = __builtin_amdgcn_readfirstlane(s_from[i]);
+        t.count = __builtin_amdgcn_readfirstlane(s_count[i]);
+        t.seq = __builtin_amdgcn_readfirstlane(s_seq[i]);
+        t.length = __builtin_amdgcn_readfirstlane(s_length[i]);
+        t.r0 = ordinal * RT;
+        t.rows = (int)min((int64_t)RT, (int64_t)t.count * a.group - t.r0);
+        t.end = key_end(a, t.length, t.length - t.count + (t.r0 + t.rows - 1) / a.group);
+        t.begin = key_begin(a, t.length - t.count + t.r0 / a.group);
+        Share sh;
+        sh.kv = kv;
+        const int lo = __builtin_amdgcn_readfirstlane(s_lo[i]);
+        sh.c0 = lo + kWaves * s0;
+        sh.c1 = min(lo + kWaves * s1, t.end > t.begin ? (t.end + 63) >> 6 : 0);
+        sh.first = 0;
+        sh.step = kWaves;
+        const int64_t w0 = uniform(from / quota), w1 = uniform((from + n - 1) / quota);
+        sh.part = (int)(blockIdx.x - w0);
+        sh.parts = (int)(w1 - w0 + 1);
+        sh.ticket = a.tickets + ((int64_t)kv * s_all + __builtin_amdgcn_readfirstlane(s_tiles[i]) + ordinal);
+        // a workgroup leaves at most two parts: that of the tile it begins with,
+        // and that of the one it begins
+        sh.at0 = (int)(2 * w0 + (from > w0 * quota ? 1 : 0)) * BYTES;
+        sh.at1 = (int)(2 * (w0 + 1)) * BYTES;
+        sh.pitch = 2 * BYTES;
+        attend_share<E, DP, QT>(c, layer, a, t, sh);
+        at += s1 - s0;
+        __syncthreads();  // (this tile's results have left LDS)
+    }
 }
 
 template <class E, int DP, int QT>
@@ -297,7 +430,7 @@ hipError_t launch_few(const CacheView& c, int64_t layer, const RaggedRows& r, At
     // one).  One sequence: as many as that, all with the same work (262145
     // keys of 8 heads of 128: 104 us, with twice as many 113).  Several, of
     // lengths that the host does not know: twice as many, so that what the
-    // longest leave is small (64 of up to 8192: 155 us against 167).
+    // longest leave is small.
     constexpr int RESIDENT = DP * QT <= 6 ? 2 : 1;
     int64_t splits = ((r.n == 1 ? 1 : 2) * RESIDENT * a.cus + live - 1) / live;
     if (splits > (chunks + kWaves - 1) / kWaves) splits = (chunks + kWaves - 1) / kWaves;
@@ -309,6 +442,18 @@ hipError_t launch_few(const CacheView& c, int64_t layer, const RaggedRows& r, At
     if (splits > kMaxSplits) splits = kMaxSplits;
     if (splits < 1 || tiles > a.ntickets) splits = 1;
     a.splits = (int)splits;
+    // Several sequences, of lengths that may differ, and enough steps for every
+    // place on the card (6 of heads of 128, 12 of 64, as their bytes go): cut
+    // evenly.  64 sequences of up to 8192, 8 heads of 128: 131 us against 149;
+    // 12: 41 against 44, and 8 (4 steps) 35.1 against 34.5; 20 of 16 heads of
+    // 64 (13 steps): 54 against 58, and 32 of up to 4000 (11) 45.8 against 44.3.
+    constexpr int PLACES = DP <= 2 ? 3 : RESIDENT;
+    const int64_t places = (int64_t)PLACES * a.cus;
+    if (QT == 1 && r.n > 1 && r.n <= 64 && tiles <= a.ntickets &&
+        live * ((chunks + kWaves - 1) / kWaves) * DP >= 24 * places && 2 * places * RT * OP * 4 <= a.partial_bytes) {
+        attend_even_kernel<E, DP><<<(unsigned)places, kThreads, 0, s>>>(c, layer, r, a);
+        return hipGetLastError();
+    }
     const int64_t rounds = (chunks + kWaves * splits - 1) / (kWaves * splits);
     // wide heads have more to join (16 sequences of up to 8000, 2 heads of 256:
     // 58 us with steps of 1, 50 of 2, 45 of 3)

@@ -370,7 +370,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     constexpr bool OVER = D >= 96;
     __shared__ float join_lds[OVER ? 1 : 4 * kThreads + kMaxSplits * RT];
     float* so = OVER ? (float*)k_lds : join_lds;
-    join_parts<T, RT, D, kThreads, kMaxSplits>(a, t, kv, d, mem, base_at, parts, so, so + 4 * kThreads);
+    join_parts<T, RT, D, kThreads, kMaxSplits>(
+        a, t, kv, d, mem, [&](int s) { return base_at + s * (RT * OP * 4); }, parts, so, so + 4 * kThreads);
 }
 
 template <class E, int DP>
