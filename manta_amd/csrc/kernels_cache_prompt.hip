@@ -2,7 +2,9 @@
 // many rows of a sequence at a time: prompts, and passages after a cached
 // prefix.
 //
-// Bound by the matrix cores and by the softmax between the two products.  A
+// Bound by the instructions of the softmax and of staging beside the products:
+// 4 sequences of up to 4096 rows, 32 heads of 128 over 8, bf16: 643 us, 892
+// TFLOP/s (a large product reaches 1174).  A
 // workgroup takes 256 rows (128 of heads wider than 128; the query heads of a
 // kv head, and tokens) and goes over the keys 64 at a time: the codes become
 // f16 (bf16 for k of bf16 queries) once per workgroup, in LDS, and its waves
