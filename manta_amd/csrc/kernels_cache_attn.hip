@@ -317,10 +317,10 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_few_ker
 // their lengths (64 sequences of up to 8192: 149 us by tiles, 131 so).  At
 // most 64 sequences, one a lane, so that every workgroup can lay them out by
 // itself.
-template <class E, int DP>
-__global__ __launch_bounds__(kThreads, DP <= 6 ? 2 : 1) void attend_even_kernel(CacheView c, int64_t layer, RaggedRows r,
-                                                                              AttendArgs a) {
-    constexpr int QT = 1, RT = 16 * QT, BYTES = RT * (32 * DP + 4) * 4;
+template <class E, int DP, int QT>
+__global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_even_kernel(CacheView c, int64_t layer,
+                                                                                   RaggedRows r, AttendArgs a) {
+    constexpr int RT = 16 * QT, BYTES = RT * (32 * DP + 4) * 4;
     const int lane = threadIdx.x & 63, j = min(lane, r.n - 1);
     const int o0 = clamp_row(r.offsets[j], r.tokens), o1 = clamp_row(r.offsets[j + 1], r.tokens);
     const int seq = r.seqs ? r.seqs[j] : j;
@@ -448,11 +448,11 @@ hipError_t launch_few(const CacheView& c, int64_t layer, const RaggedRows& r, At
     // evenly.  64 sequences of up to 8192, 8 heads of 128: 131 us against 149;
     // 12: 41 against 44, and 8 (4 steps) 35.1 against 34.5; 20 of 16 heads of
     // 64 (13 steps): 54 against 58, and 32 of up to 4000 (11) 45.8 against 44.3.
-    constexpr int PLACES = DP <= 2 ? 3 : RESIDENT;
+    constexpr int PLACES = DP <= 2 && QT == 1 ? 3 : RESIDENT;
     const int64_t places = (int64_t)PLACES * a.cus;
-    if (QT == 1 && r.n > 1 && r.n <= 64 && tiles <= a.ntickets &&
-        live * ((chunks + kWaves - 1) / kWaves) * DP >= 24 * places && 2 * places * RT * OP * 4 <= a.partial_bytes) {
-        attend_even_kernel<E, DP><<<(unsigned)places, kThreads, 0, s>>>(c, layer, r, a);
+    if (r.n > 1 && r.n <= 64 && tiles <= a.ntickets &&
+        live * ((chunks + kWaves - 1) / kWaves) * DP >= 22 * places && 2 * places * RT * OP * 4 <= a.partial_bytes) {
+        attend_even_kernel<E, DP, QT><<<(unsigned)places, kThreads, 0, s>>>(c, layer, r, a);
         return hipGetLastError();
     }
     const int64_t rounds = (chunks + kWaves * splits - 1) / (kWaves * splits);

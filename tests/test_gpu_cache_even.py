@@ -38,6 +38,18 @@ def test_counts_windows_and_rows_that_see_nothing(rt, counts, window, causal):
     _check(rt, m, rng, "f16", 14, counts, window=window, causal=causal, longest=MANY, extra_rows=2)
 
 
+@pytest.mark.parametrize("page,kv,group,d,counts", [
+    (16, 2, 4, 64, [5, 8, 1, 7, 6, 5]), (32, 1, 6, 96, [5] * 9), (64, 2, 4, 128, [8, 0, 16, 1]), (16, 1, 1, 32, [32, 20, 31]),
+    (128, 1, 8, 256, [3, 4]), (64, 1, 25, 160, [1, 1, 1]),
+])
+def test_tiles_of_32_rows(rt, page, kv, group, d, counts):
+    print("even 32 rows", page, kv, group, d, counts, flush=True)
+    rng = np.random.default_rng(24)
+    m = filled(rng, [c + int(x) for c, x in zip(counts, rng.integers(0, 900, len(counts)))], page, kv, d)
+    for window in (0, 150):
+        _check(rt, m, rng, "bf16", kv * group, counts, window=window, longest=MANY)
+
+
 def test_one_long_sequence_among_short_ones(rt):
     """A tile in many parts, and workgroups that end several tiles."""
     print("even long", flush=True)
