@@ -4,11 +4,10 @@
 //
 // Bound by the instructions of the softmax and of staging beside the products:
 // 4 sequences of up to 4096 rows, 32 heads of 128 over 8, bf16: 643 us, 892
-// TFLOP/s (a large product reaches 1174).  A
-// workgroup takes 256 rows (128 of heads wider than 128; the query heads of a
-// kv head, and tokens) and goes over the keys 64 at a time: the codes become
-// f16 (bf16 for k of bf16 queries) once per workgroup, in LDS, and its waves
-// multiply them with 32 rows each.
+// TFLOP/s (a large product reaches 1174).  A workgroup takes 256 or 128 rows
+// (the query heads of a kv head, and tokens) and goes over the keys 64 at a
+// time: the codes become f16 (bf16 for k of bf16 queries) once per workgroup,
+// in LDS, and its waves multiply them with 32 rows each.
 #include "cache_attend.hpp"
 
 namespace manta {
@@ -376,9 +375,9 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
         a, t, kv, d, mem, [&](int s) { return base_at + s * (RT * OP * 4); }, parts, so, so + 4 * kThreads);
 }
 
-template <class E, int DP>
+template <class E, int DP, int WAVES>
 hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, AttendArgs a, hipStream_t s) {
-    constexpr int WAVES = DP <= 4 ? 8 : 4, OCC = DP <= 4 ? 2 : 1;
+    constexpr int OCC = DP <= 4 ? 2 : 1;  // waves a SIMD: wider heads need its registers
     constexpr int kThreads = 64 * WAVES, RT = WAVES * 32, OP = 32 * DP + 4;
     const int64_t slots = tile_slots(r.tokens, r.n, a.group, RT), tiles = slots * c.kv_heads;
     // about: keys that a tile sees in steps of 64, tiles that hold rows
@@ -387,7 +386,9 @@ hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, A
     const int64_t chunks = (keys + 63) / 64;
     int64_t live = r.n * ((each * a.group + RT - 1) / RT) * c.kv_heads;
     if (live > tiles) live = tiles;
-    int64_t splits = a.cus / live;  // (one workgroup fits a compute unit)
+    // Joining parts of 128 rows and more is dear (a prompt of 2048: 74 us whole,
+    // 100 in two parts): only for tiles that leave compute units empty.
+    int64_t splits = OCC * 4 / WAVES * a.cus / live;
     if (splits > chunks / 8) splits = chunks / 8;
     const int64_t fit = a.partial_bytes / (tiles * RT * OP * 4);
     if (splits > fit) splits = fit;
@@ -402,17 +403,29 @@ hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, A
     return hipGetLastError();
 }
 
+// Tiles of 256 rows stage the keys half as often; of 128, two of which fit a
+// compute unit, they fill the card with fewer rows.  4 sequences of up to 4096,
+// 32 heads over 8 (1400 tiles of 256): 641 us and 668; 8 of up to 512 (512):
+// 74 and 72; one of 2048 (256): 74 and 64; 4 of 30 tokens, 8 heads over 1 (16): 141 and 113.
+template <class E, int DP>
+hipError_t launch_rows(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a, hipStream_t s) {
+    const int64_t rows = ((int64_t)r.tokens + r.n - 1) / r.n * a.group;  // a sequence's, about
+    if (DP <= 4 && r.n * ((rows + 255) / 256) * c.kv_heads > 2 * a.cus)
+        return launch_many<E, DP, DP <= 4 ? 8 : 4>(c, layer, r, a, s);
+    return launch_many<E, DP, 4>(c, layer, r, a, s);
+}
+
 template <class E>
 hipError_t launch_width(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a, hipStream_t s) {
     switch (c.pitch / 32) {
-        case 1: return launch_many<E, 1>(c, layer, r, a, s);
-        case 2: return launch_many<E, 2>(c, layer, r, a, s);
-        case 3: return launch_many<E, 3>(c, layer, r, a, s);
-        case 4: return launch_many<E, 4>(c, layer, r, a, s);
-        case 5: return launch_many<E, 5>(c, layer, r, a, s);
-        case 6: return launch_many<E, 6>(c, layer, r, a, s);
-        case 7: return launch_many<E, 7>(c, layer, r, a, s);
-        default: return launch_many<E, 8>(c, layer, r, a, s);
+        case 1: return launch_rows<E, 1>(c, layer, r, a, s);
+        case 2: return launch_rows<E, 2>(c, layer, r, a, s);
+        case 3: return launch_rows<E, 3>(c, layer, r, a, s);
+        case 4: return launch_rows<E, 4>(c, layer, r, a, s);
+        case 5: return launch_rows<E, 5>(c, layer, r, a, s);
+        case 6: return launch_rows<E, 6>(c, layer, r, a, s);
+        case 7: return launch_rows<E, 7>(c, layer, r, a, s);
+        default: return launch_rows<E, 8>(c, layer, r, a, s);
     }
 }
 

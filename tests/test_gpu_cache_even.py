@@ -76,3 +76,16 @@ def test_listed_sequences_in_place_and_again(rt):
     with pytest.raises(_lib.MantaRocmError, match="page %d out of range" % (m.pages + 1)):
         rt.synchronize()
     c.close()
+
+
+@pytest.mark.parametrize("page,kv,group,d,n,count", [
+    (64, 40, 16, 64, 3, 130), (16, 130, 2, 32, 4, 40), (64, 130, 1, 128, 4, 60), (32, 130, 1, 96, 4, 70),
+    (16, 130, 1, 128, 4, 60),
+])
+def test_prompts_in_tiles_of_256_rows(rt, page, kv, group, d, n, count):
+    """More tiles than the card has places."""
+    print("prompts", page, kv, group, d, n, count, flush=True)
+    rng = np.random.default_rng(25)
+    counts = [count] + [int(x) for x in rng.integers(3 * count // 4, count, n - 1)]
+    m = filled(rng, [c + int(x) for c, x in zip(counts, rng.integers(0, 80, n))], page, kv, d)
+    _check(rt, m, rng, "f16", kv * group, counts, window=40 if page == 32 else 0)
