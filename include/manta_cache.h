@@ -11,7 +11,8 @@
  * see (an index in a device array) is checked by the kernels: such an entry
  * is skipped, nothing out of range is read or written, and the next
  * synchronizing call (manta_rocm_synchronize / manta_rocm_download) reports
- * it.  The reference has no counterpart: its row-wise `rope` kernel
+ * it.  A call takes at most 2^25 tokens and 2^21 sequences, attention 2^28
+ * rows (tokens * heads).  The reference has no counterpart: its row-wise `rope` kernel
  * (compiler/compiler.go:746-802) rotates f32 rows at positions 0, 1, 2, ...
  */
 #ifndef MANTA_CACHE_H
@@ -123,7 +124,8 @@ typedef struct MantaRocmCacheBuffers {
     int64_t book_count;
 } MantaRocmCacheBuffers;
 
-/* An empty cache: every page free, every sequence of length 0. */
+/* An empty cache: every page free, every sequence of length 0.  Beside the
+ * buffers it holds 96 MiB for attention's partial results. */
 int manta_rocm_cache_create(MantaRocm* rt, const MantaRocmCacheShape* shape, MantaRocmCache** out, char** err);
 /* Frees the handle and, unless the runtime went first, its device memory. */
 void manta_rocm_cache_destroy(MantaRocmCache* cache);
