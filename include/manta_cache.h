@@ -163,7 +163,9 @@ int manta_rocm_cache_copy_pages(MantaRocm* rt, MantaRocmCache* cache, const int3
  * NULL) owns rows offsets_dev[i] .. offsets_dev[i+1] (int32 [n+1], ascending,
  * within [0, tokens]) of the activation tensors, and they are its last
  * tokens: with c rows and length l, row j is at position l - c + j.  Rows of
- * negative position are skipped. */
+ * negative position are skipped.  Offsets that descend leave rows to nobody or
+ * to several sequences (still nothing out of range is read or written);
+ * attention may skip such a batch as a whole and report it. */
 
 /* Quantise k and v [tokens, kv_heads, head_dim] of one layer into the pages
  * (extended before).  Per page and head, max is the largest magnitude of its

@@ -56,6 +56,7 @@ enum CacheError {
     kCacheFull = 3,      // a: pages needed, b: pages free (unsigned)
     kCacheInUse = 4,     // a: the sequence
     kCacheBadCount = 5,  // a: the sequence, b: the count
+    kCacheBadOffsets = 6,  // a: the entry of the batch
 };
 MANTA_HD unsigned long long cache_error(int kind, int64_t a, int64_t b) {
     return ((unsigned long long)kind << 60) | (((unsigned long long)a & 0x3FFFFFFFull) << 30) |
@@ -71,6 +72,7 @@ inline void describe_cache_error(unsigned long long w, char* out, size_t size) {
     else if (kind == kCacheBadPage) snprintf(out, size, "cache page %lld out of range", as);
     else if (kind == kCacheFull) snprintf(out, size, "cache is out of pages: %lld needed, %lld free", a, b);
     else if (kind == kCacheInUse) snprintf(out, size, "cache sequence %lld is not empty", as);
+    else if (kind == kCacheBadOffsets) snprintf(out, size, "cache offsets descend at entry %lld of the batch", as);
     else snprintf(out, size, "cache sequence %lld: count %lld out of range", as, bs);
 }
 
@@ -110,6 +112,12 @@ MANTA_HD bool ragged_piece(int a, int b, int length, int64_t local, int shift, P
 // group / rows) tiles fit the slots [tile_base(a, i), tile_base(b, i + 1)).
 MANTA_HD int64_t tile_slots(int64_t tokens, int64_t n, int64_t group, int rows) { return tokens * group / rows + n; }
 MANTA_HD int64_t tile_base(int offset, int64_t i, int64_t group, int rows) { return offset * group / rows + i; }
+// A sequence's tiles: over a batch of ascending offsets at most tile_slots.
+MANTA_HD int tile_count(int from, int to, int64_t group, int rows) {
+    return to > from ? (int)(((int64_t)(to - from) * group + rows - 1) / rows) : 0;
+}
+// Whether each tile of a kv head, `tiles` of them, has a ticket of its own.
+MANTA_HD bool tiles_fit(int64_t tiles, int64_t kv_heads, int64_t tickets) { return tiles * kv_heads <= tickets; }
 
 // ---- checks (nullptr: nothing wrong) ----
 

@@ -323,6 +323,11 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_even_ke
     constexpr int RT = 16 * QT, BYTES = RT * (32 * DP + 4) * 4;
     const int lane = threadIdx.x & 63, j = min(lane, r.n - 1);
     const int o0 = clamp_row(r.offsets[j], r.tokens), o1 = clamp_row(r.offsets[j + 1], r.tokens);
+    // (tickets are counted for offsets that ascend)
+    if (__any(o1 < o0)) {
+        if (o1 < o0 && lane < r.n && blockIdx.x == 0 && threadIdx.x < 64) cache_report(c, kCacheBadOffsets, j, 0);
+        return;
+    }
     const int seq = r.seqs ? r.seqs[j] : j;
     const bool good = (unsigned)seq < (unsigned)c.seqs;
     const int length = good ? c.clamp_length(c.lengths[seq]) : 0;
@@ -330,7 +335,7 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_even_ke
     int tiles = 0, steps = 1, c_lo = 0;
     if (lane < r.n && o1 > o0) {
         if (!good && blockIdx.x == 0 && threadIdx.x < 64) cache_report(c, kCacheBadSeq, seq, 0);
-        tiles = (int)(((int64_t)(o1 - o0) * a.group + RT - 1) / RT);
+        tiles = tile_count(o0, o1, a.group, RT);
         c_lo = key_begin(a, length - (o1 - o0)) >> 6;
         steps = max(1, (((length + 63) >> 6) - c_lo + kWaves - 1) / kWaves);
     }
@@ -371,6 +376,7 @@ __global__ __launch_bounds__(kThreads, DP * QT <= 6 ? 2 : 1) void attend_even_ke
         const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
         return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 | lo);
     };
+    if (!tiles_fit(s_all, c.kv_heads, a.ntickets)) return;
     const int64_t total = uniform(s_total), all = total * c.kv_heads;
     // each workgroup's steps: no tile in more parts than can be joined
     const int64_t quota = uniform(max((all + gridDim.x - 1) / gridDim.x, (int64_t)(s_most / (kMaxSplits - 2) + 1)));
