@@ -132,13 +132,17 @@ void manta_rocm_cache_destroy(MantaRocmCache* cache);
 int manta_rocm_cache_shape(const MantaRocmCache* cache, MantaRocmCacheShape* out);
 int manta_rocm_cache_buffers(const MantaRocmCache* cache, MantaRocmCacheBuffers* out);
 
-/* -- pages.  The sequence lists are int32 device arrays of n distinct slots;
- * a call changes all of its entries or, on "out of pages", none. */
+/* -- pages.  The sequence lists are int32 device arrays of n distinct slots.
+ * fork and release skip an entry that is wrong and do the others; extend does
+ * all of its entries or, where one is wrong or pages are too few, none. */
 
 /* Grow sequences by counts_dev[i] >= 0 tokens: each takes the lowest free
  * pages, in the order of the list; one whose last page is partly filled and
  * shared when the call begins first gets a copy of it (every layer).  The
- * new tokens' contents are undefined until they are appended. */
+ * new tokens' contents are undefined until they are appended.  A refused call
+ * leaves its sequences as they are until it is reported: appends skip them and
+ * extends that name one are refused too, so that the steps that were already
+ * on their way (or in a graph) cost nothing that the cache holds. */
 int manta_rocm_cache_extend(MantaRocm* rt, MantaRocmCache* cache, const int32_t* seqs_dev, const int32_t* counts_dev,
                             int64_t n, char** err);
 /* children_dev[i] (empty, and no parent of this call) takes the first

@@ -37,12 +37,15 @@ struct MantaRocmCache : manta_rt::Attached {
     MantaRocmCacheShape shape{};
     CacheView view{};
     void* memory = nullptr;  // codes and largest values
-    void* book = nullptr;    // refs, lengths, tables; then the scratch
+    void* book = nullptr;    // refs, lengths, tables; then the scratch and the refused sequences' marks
     int64_t code_bytes = 0, max_count = 0, book_count = 0;
     manta::PageScratch scratch{};
     int32_t* free_list = nullptr;
     float* partial = nullptr;
     uint32_t* tickets = nullptr;
+    int reported(void* stream) override {
+        return (int)hipMemsetAsync(view.refused, 0, (size_t)view.seqs * 4, (hipStream_t)stream);
+    }
     void release() override {
         if (memory) (void)hipFree(memory);
         if (book) (void)hipFree(book);
@@ -250,12 +253,14 @@ int manta_rocm_cache_create(MantaRocm* rt, const MantaRocmCacheShape* shape, Man
     const size_t scratch = (size_t)(4 * v.pages + 64) * 4;
     hipError_t e = hipMalloc(&c->memory, 2 * ((size_t)c->code_bytes + max_bytes));
     if (e == hipSuccess) e = hipMemset(c->memory, 0, 2 * ((size_t)c->code_bytes + max_bytes));
-    if (e == hipSuccess) e = hipMalloc(&c->book, book_bytes + scratch);
+    const size_t marks = (size_t)v.seqs * 4;
+    if (e == hipSuccess) e = hipMalloc(&c->book, book_bytes + scratch + marks);
     // refs and lengths 0, tables -1
     if (e == hipSuccess) e = hipMemset(c->book, 0, (size_t)(v.pages + v.seqs) * 4);
     if (e == hipSuccess)
         e = hipMemset((char*)c->book + (size_t)(v.pages + v.seqs) * 4, 0xFF,
                       book_bytes - (size_t)(v.pages + v.seqs) * 4);
+    if (e == hipSuccess) e = hipMemset((char*)c->book + book_bytes + scratch, 0, marks);
     if (e == hipSuccess) e = hipMalloc((void**)&c->partial, kPartialBytes + kAttendTickets * 4);
     if (e == hipSuccess) e = hipMemset((char*)c->partial + kPartialBytes, 0, kAttendTickets * 4);
     if (e == hipSuccess) e = hipDeviceSynchronize();
@@ -275,6 +280,7 @@ int manta_rocm_cache_create(MantaRocm* rt, const MantaRocmCacheShape* shape, Man
     int32_t* w = (int32_t*)((char*)c->book + book_bytes);
     c->scratch = {w, w + 64, w + 64 + v.pages, w + 64 + 2 * v.pages};
     c->free_list = w + 64 + 3 * v.pages;
+    v.refused = (int32_t*)((char*)c->book + book_bytes + scratch);
     c->tickets = (uint32_t*)((char*)c->partial + kPartialBytes);
     c->rt = rt;
     if (!manta_rt::attach(rt, c)) {

@@ -33,6 +33,7 @@ struct CacheView {
     int32_t* refs;     // [pages]
     int32_t* lengths;  // [seqs]
     int32_t* tables;   // [seqs][table_pages]
+    int32_t* refused;  // [seqs]: 1 from a refused extend until it is reported
     unsigned long long* err;
     int64_t layers, pages;
     int page_tokens, page_shift;

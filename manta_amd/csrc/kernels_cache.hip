@@ -35,6 +35,15 @@ __device__ __forceinline__ bool piece_page(const CacheView& c, const Piece& p, i
     return false;
 }
 
+// Whether append leaves the piece alone.  A sequence whose extend was refused
+// has not grown: its last tokens are not the rows' place.  It is asked for with
+// the page and looked at before the first store, so that nothing waits for it.
+struct Keep {
+    int refused;
+    __device__ __forceinline__ Keep(const CacheView& c, int seq, int page) : refused(c.refused[seq]) {}
+    __device__ __forceinline__ bool operator()(const CacheView& c, int page) const { return refused; }
+};
+
 __device__ __forceinline__ int quantise(float x, float max) {
     const float r = __builtin_rintf(__fdiv_rn(x * 127.0f, max));
     return (int)fminf(127.0f, fmaxf(-127.0f, r));
@@ -50,6 +59,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(CacheView c, int64_t l
     Piece p;
     int seq, page;
     if (!my_piece(c, r, &p, &seq) || !piece_page(c, p, seq, &page)) return;
+    const Keep keep(c, seq, page);
     const int head = blockIdx.y, is_v = blockIdx.z;
     const int tid = threadIdx.x, d = c.head_dim;
     const T* src = is_v ? (const T*)x.v + head * x.v_head : (const T*)x.k + head * x.k_head;
@@ -75,6 +85,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(CacheView c, int64_t l
     const bool zero = bad || big < 0x1p-126f;  // every code 0
     const bool raise = big > old;
     if (zero) big = bad ? __builtin_nanf("") : 0.0f;
+    if (keep(c, page)) return;
     __syncthreads();  // every thread has read *slot
     if (tid == 0) *slot = big;
 
@@ -166,6 +177,7 @@ __global__ __launch_bounds__(kThreads) void append_wide_kernel(CacheView c, int6
         }
     }
     if (!piece_page(c, p, seq, &page)) return;
+    const Keep keep(c, seq, page);
     float* slot = (is_v ? c.v_max : c.k_max) + c.slab(layer, page) * c.kv_heads + head;
     const float old = p.from ? *slot : 0.0f;
 
@@ -207,6 +219,7 @@ __global__ __launch_bounds__(kThreads) void append_wide_kernel(CacheView c, int6
     const bool raise = big > old;
     const bool exact = big > 0x1p125f;
     if (zero) big = bad ? __builtin_nanf("") : 0.0f;
+    if (keep(c, page)) return;
     if (tid == 0) *slot = big;
     const float inv = 1.0f / big;
 
@@ -382,6 +395,7 @@ __device__ Growth growth(const CacheView& c, const int32_t* seqs, const int32_t*
         if (report) cache_report(c, kCacheBadSeq, g.seq, 0);
         return g;
     }
+    const int refused = c.refused[g.seq];  // (looked at last: nothing waits for it)
     g.length = c.clamp_length(c.lengths[g.seq]);
     if (add < 0 || (int64_t)g.length + add > (int64_t)c.table_pages << c.page_shift) {
         if (report) cache_report(c, kCacheBadCount, g.seq, add);
@@ -399,7 +413,7 @@ __device__ Growth growth(const CacheView& c, const int32_t* seqs, const int32_t*
         if (c.refs[last] > 1) g.last = last;
     }
     g.grown = g.length + add;
-    g.ok = true;
+    g.ok = !refused;
     return g;
 }
 
@@ -442,6 +456,8 @@ __global__ __launch_bounds__(kBook) void extend_kernel(CacheView c, PageScratch 
             if (!skip) cache_report(c, kCacheFull, need64, found);
             *w.count = 0;
         }
+        for (int i = tid; i < n; i += kBook)
+            if ((unsigned)seqs[i] < (unsigned)c.seqs) c.refused[seqs[i]] = 1;
         return;
     }
     __syncthreads();  // free_list is written

@@ -300,6 +300,7 @@ int check_cache_error(MantaRocm* rt, char** err) {
     const unsigned long long zero = 0;
     HIP_TRY(hipMemcpyAsync(rt->err_word + 1, &zero, sizeof(zero), hipMemcpyHostToDevice, rt->stream),
             "hipMemcpy(error word)");
+    for (manta_rt::Attached* a : rt->attached) HIP_TRY((hipError_t)a->reported(rt->stream), "hipMemset(reported)");
     HIP_TRY(hipStreamSynchronize(rt->stream), "hipStreamSynchronize");
     char text[160];
     manta::describe_cache_error(w, text, sizeof(text));

@@ -56,6 +56,11 @@ void launch_end(MantaRocm* rt, const char* what, void* start);
 struct Attached {
     virtual ~Attached() {}
     virtual void release() = 0;
+    // What the handle's kernels found wrong has been reported (a hipError_t).
+    virtual int reported(void* stream) {
+        (void)stream;
+        return 0;
+    }
 };
 bool attach(MantaRocm* rt, Attached* a);  // false: out of memory
 void detach(MantaRocm* rt, Attached* a);
