@@ -172,7 +172,8 @@ int manta_rocm_cache_copy_pages(MantaRocm* rt, MantaRocmCache* cache, const int3
  * attention may skip such a batch as a whole and report it. */
 
 /* Quantise k and v [tokens, kv_heads, head_dim] of one layer into the pages
- * (extended before).  Per page and head, max is the largest magnitude of its
+ * (extended before; the sequences are distinct, and a page that another table
+ * names too is skipped and reported).  Per page and head, max is the largest magnitude of its
  * tokens and code = round_half_even(x * 127 / max), in f32.  Tokens that the
  * page held before keep their codes; when the new tokens raise max, they
  * become round_half_even(code * old / max).  A max below 2^-126 counts as 0

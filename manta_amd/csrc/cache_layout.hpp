@@ -58,6 +58,7 @@ enum CacheError {
     kCacheInUse = 4,     // a: the sequence
     kCacheBadCount = 5,  // a: the sequence, b: the count
     kCacheBadOffsets = 6,  // a: the entry of the batch
+    kCacheShared = 7,      // a: the page
 };
 MANTA_HD unsigned long long cache_error(int kind, int64_t a, int64_t b) {
     return ((unsigned long long)kind << 60) | (((unsigned long long)a & 0x3FFFFFFFull) << 30) |
@@ -74,6 +75,7 @@ inline void describe_cache_error(unsigned long long w, char* out, size_t size) {
     else if (kind == kCacheFull) snprintf(out, size, "cache is out of pages: %lld needed, %lld free", a, b);
     else if (kind == kCacheInUse) snprintf(out, size, "cache sequence %lld is not empty", as);
     else if (kind == kCacheBadOffsets) snprintf(out, size, "cache offsets descend at entry %lld of the batch", as);
+    else if (kind == kCacheShared) snprintf(out, size, "cache page %lld is shared: extend copies it before an append", as);
     else snprintf(out, size, "cache sequence %lld: count %lld out of range", as, bs);
 }
 

@@ -36,12 +36,19 @@ __device__ __forceinline__ bool piece_page(const CacheView& c, const Piece& p, i
 }
 
 // Whether append leaves the piece alone.  A sequence whose extend was refused
-// has not grown: its last tokens are not the rows' place.  It is asked for with
-// the page and looked at before the first store, so that nothing waits for it.
+// has not grown: its last tokens are not the rows' place.  A page that several
+// tables name is not written (extend gives a sequence that goes on in one its
+// own copy).  Both are asked for with the page and looked at before the first
+// store, so that nothing waits for them.
 struct Keep {
-    int refused;
-    __device__ __forceinline__ Keep(const CacheView& c, int seq, int page) : refused(c.refused[seq]) {}
-    __device__ __forceinline__ bool operator()(const CacheView& c, int page) const { return refused; }
+    int refused, refs;
+    __device__ __forceinline__ Keep(const CacheView& c, int seq, int page) : refused(c.refused[seq]), refs(c.refs[page]) {}
+    __device__ __forceinline__ bool operator()(const CacheView& c, int page) const {
+        if (refused) return true;
+        if (refs <= 1) return false;
+        if (threadIdx.x == 0) cache_report(c, kCacheShared, page, 0);
+        return true;
+    }
 };
 
 __device__ __forceinline__ int quantise(float x, float max) {

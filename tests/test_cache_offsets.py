@@ -62,10 +62,12 @@ def test_tiles_of_descending_offsets_do_not(lib):
     assert lib.count(1024, 0, 1, 16) == 0 and lib.count(5, 5, 1, 16) == 0
 
 
-def test_error_word(lib):
+def test_error_words(lib):
     buf = C.create_string_buffer(160)
     lib.describe(6, 17, 0, buf)
     assert buf.value.decode() == "cache offsets descend at entry 17 of the batch"
+    lib.describe(7, 40000, 0, buf)
+    assert buf.value.decode() == "cache page 40000 is shared: extend copies it before an append"
 
 
 @pytest.mark.gpu

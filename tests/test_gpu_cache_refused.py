@@ -1,5 +1,5 @@
-"""What a refused extend leaves of the cache: all of it, bit for bit, until the
-refusal has been reported."""
+"""What a refused extend, or an append to a shared page, leaves of the cache:
+all of it, bit for bit, until the refusal has been reported."""
 import ctypes as C
 
 import numpy as np
@@ -79,6 +79,33 @@ def test_appends_after_a_refused_extend(rt, new, why):
     rt.synchronize()
     m.check_book(c)
     m.check_pages(c)
+    c.close()
+
+
+@pytest.mark.parametrize("tokens", [1, 30])
+def test_append_leaves_shared_pages(rt, tokens):
+    """Last tokens that a branch shares are not written over; the same rows of a
+    sequence whose pages are its own are."""
+    print("shared", tokens, flush=True)
+    rng = np.random.default_rng(tokens)
+    m = filled(rng, [40, 40, 0], 16, 2, 64, dirty=False)
+    m.fork([0], [2])
+    c = m.upload(rt)
+    before = _contents(c)
+    x = to_bits(rng.standard_normal((2 * tokens, 2, 64)) * 9, "bf16")
+    xd = rt.to_device(x)
+    for s in (0, 2):
+        c.append(0, xd, xd, _dev(rt, [0, tokens]), _dev(rt, [s]), dtype="bf16")
+        with pytest.raises(_lib.MantaRocmError, match="is shared"):
+            rt.synchronize()
+        _same(_contents(c), before)
+    c.append(0, xd, xd, _dev(rt, [0, tokens, 2 * tokens]), _dev(rt, [0, 1]), dtype="bf16")
+    with pytest.raises(_lib.MantaRocmError, match="is shared"):
+        rt.synchronize()
+    y = from_bits(x, "bf16")[tokens:]
+    m.append(0, y, y, [0, tokens], [1])
+    m.check_pages(c)
+    m.check_book(c)
     c.close()
 
 
