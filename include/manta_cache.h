@@ -174,7 +174,8 @@ int manta_rocm_cache_copy_pages(MantaRocm* rt, MantaRocmCache* cache, const int3
 /* Quantise k and v [tokens, kv_heads, head_dim] of one layer into the pages
  * (extended before; the sequences are distinct, and a page that another table
  * names too is skipped and reported).  Per page and head, max is the largest magnitude of its
- * tokens and code = round_half_even(x * 127 / max), in f32.  Tokens that the
+ * tokens and code = round_half_even(x * 127 / max), in f32 (where x * 127 is
+ * past the largest number, magnitudes above 2.67e36, +-127).  Tokens that the
  * page held before keep their codes; when the new tokens raise max, they
  * become round_half_even(code * old / max).  A max below 2^-126 counts as 0
  * (all codes 0); a new value that is not finite makes max NaN, and with it

@@ -128,7 +128,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(CacheView c, int64_t l
 // cannot matter: t * (1 / max) is within 127 * 3 * 2^-24 < 2^-15 of it (three
 // roundings), so only what lies closer than that to a half is divided.  Adding
 // 1.5 * 2^23 rounds, and leaves the code in the low byte.  |t| <= 127 max, but
-// for t beyond the largest number; `exact`: 1 / max is not a normal number.
+// for t beyond the largest number; `exact`: there may be such a t (max >= 2^121;
+// its code is 127 or -127), or 1 / max is not a normal number.
 __device__ __forceinline__ uint32_t ratio_codes(const float* t, float max, float inv, bool exact) {
     constexpr float kRound = 12582912.0f;
     uint32_t b[4];
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void append_wide_kernel(CacheView c, int6
     float big = fmaxf(__uint_as_float(top), old);
     const bool zero = bad || big < 0x1p-126f;  // every code 0
     const bool raise = big > old;
-    const bool exact = big > 0x1p125f;
+    const bool exact = big >= 0x1p121f;
     if (zero) big = bad ? __builtin_nanf("") : 0.0f;
     if (keep(c, page)) return;
     if (tid == 0) *slot = big;
