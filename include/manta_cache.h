@@ -177,7 +177,7 @@ int manta_rocm_cache_copy_pages(MantaRocm* rt, MantaRocmCache* cache, const int3
  * tokens and code = round_half_even(x * 127 / max), in f32 (where x * 127 is
  * past the largest number, magnitudes above 2.67e36, +-127).  Tokens that the
  * page held before keep their codes; when the new tokens raise max, they
- * become round_half_even(code * old / max).  A max below 2^-126 counts as 0
+ * become round_half_even(code * old / max), at any magnitude.  A max below 2^-126 counts as 0
  * (all codes 0); a new value that is not finite makes max NaN, and with it
  * every result that attends to the page's head. */
 int manta_rocm_cache_append(MantaRocm* rt, MantaRocmCache* cache, int64_t layer, int dtype, const void* k_dev,

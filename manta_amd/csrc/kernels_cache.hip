@@ -55,8 +55,13 @@ __device__ __forceinline__ int quantise(float x, float max) {
     const float r = __builtin_rintf(__fdiv_rn(x * 127.0f, max));
     return (int)fminf(127.0f, fmaxf(-127.0f, r));
 }
+// Where 127 * max would leave f32, old codes' products are taken of numbers
+// 2^-8 as large: code * old / max is the same, rounding for rounding.
+__device__ __forceinline__ float headroom(float max) { return max >= 0x1p121f ? 0x1p-8f : 1.0f; }
 __device__ __forceinline__ int requantise(int code, float old, float max) {
-    return (int)__builtin_rintf(__fdiv_rn((float)code * old, max));
+    const float h = headroom(max);
+    const float r = __builtin_rintf(__fdiv_rn((float)code * (old * h), max * h));
+    return (int)fminf(127.0f, fmaxf(-127.0f, r));
 }
 
 // One page's head of k (blockIdx.z 0) or v (1).
@@ -233,10 +238,11 @@ __global__ __launch_bounds__(kThreads) void append_wide_kernel(CacheView c, int6
 
     if (p.from && (raise || zero)) {
         auto renew = [&](uint32_t word, uint32_t* at, int bytes) {
+            const float h = headroom(big);
             float t[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) t[j] = (float)(int8_t)(word >> (8 * j)) * old;
-            word = zero ? 0 : ratio_codes(t, big, inv, exact);
+            for (int j = 0; j < 4; j++) t[j] = (float)(int8_t)(word >> (8 * j)) * (old * h);
+            word = zero ? 0 : ratio_codes(t, big * h, inv, exact);
             if (bytes == 4) *at = word;
             else
                 for (int j = 0; j < bytes; j++) ((uint8_t*)at)[j] = (uint8_t)(word >> (8 * j));

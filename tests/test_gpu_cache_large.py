@@ -42,3 +42,42 @@ def test_new_values(rt, dtype, tokens):
     assert (np.abs(m.k).max((3, 4)) == 127).all()  # the largest element has the largest code
     m.check_pages(c)
     c.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [1, 14])
+def test_values_that_were_there(rt, dtype, tokens):
+    """A page of two tokens goes on with larger ones: round_half_even(code * old
+    / max), each of its f32 steps on numbers 2^-8 as large, which changes no
+    rounding."""
+    print("append raises", dtype, tokens, flush=True)
+    rng = np.random.default_rng(tokens + 50)
+    pairs = [(1e35, 2e35), (2e36, 2.6e36), (3e36, 3.5e36), (1e37, 2e37), (1e37, 3e38), (4e37, 5e37), (3e38, 3.3e38),
+             (1.0, 3e38), (1e-38, 1e38)]
+    n, d = len(pairs), 64
+    m = Model(1, n, 16, 2, d, n, 1)
+    assert m.extend(range(n), [2 + tokens] * n)
+    rows = m.tables[:, 0]
+    old, new = (np.array(x, np.float32) for x in zip(*pairs))
+    m.k[0, rows, :, :2] = rng.integers(-127, 128, (n, 2, 2, d))
+    m.v[0, rows, :, :, :2] = rng.integers(-127, 128, (n, 2, d, 2))
+    m.k[0, rows, :, 0, :2] = 127, -127
+    m.km[0, rows], m.vm[0, rows] = old[:, None], old[:, None]
+    c = m.upload(rt)
+    x = rng.uniform(-0.5, 0.5, (n, tokens, 2, d)) * new[:, None, None, None]
+    x[:, -1, :, 3] = new[:, None]
+    x = to_bits(x.reshape(n * tokens, 2, d), dtype)
+    xd = rt.to_device(x)
+    c.append(0, xd, xd, _dev(rt, _offsets([tokens] * n)), dtype=dtype)
+    big = np.abs(from_bits(x, dtype)).reshape(n, -1).max(1)
+    h = np.float32(2.0 ** -8)
+
+    def again(codes):  # [n, ...]
+        codes = codes.astype(np.float32)
+        at = (slice(None),) + (None,) * (codes.ndim - 1)
+        return np.rint(codes * (old * h)[at] / (big * h)[at])
+
+    np.testing.assert_array_equal(c.k_max.download()[0, rows], np.stack([big, big], 1))
+    np.testing.assert_array_equal(c.k_codes.download()[0, rows, :, :2], again(m.k[0, rows, :, :2]))
+    np.testing.assert_array_equal(c.v_codes.download()[0, rows, :, :, :2], again(m.v[0, rows, :, :, :2]))
+    c.close()
