@@ -55,14 +55,22 @@ __device__ __forceinline__ int quantise(float x, float max) {
     const float r = __builtin_rintf(__fdiv_rn(x * 127.0f, max));
     return (int)fminf(127.0f, fmaxf(-127.0f, r));
 }
-// Where 127 * max would leave f32, old codes' products are taken of numbers
-// 2^-8 as large: code * old / max is the same, rounding for rounding.
+// Where 127 * max would leave f32, products with codes are taken of numbers
+// 2^-8 as large: code * old / max and code * max / 127 are the same, rounding
+// for rounding.
 __device__ __forceinline__ float headroom(float max) { return max >= 0x1p121f ? 0x1p-8f : 1.0f; }
 __device__ __forceinline__ int requantise(int code, float old, float max) {
     const float h = headroom(max);
     const float r = __builtin_rintf(__fdiv_rn((float)code * (old * h), max * h));
     return (int)fminf(127.0f, fmaxf(-127.0f, r));
 }
+
+// A page's values.
+struct Values {
+    float big, up;
+    __device__ __forceinline__ explicit Values(float max) : big(max * headroom(max)), up(max >= 0x1p121f ? 0x1p8f : 1.0f) {}
+    __device__ __forceinline__ float operator()(int code) const { return __fdiv_rn((float)code * big, 127.0f) * up; }
+};
 
 // One page's head of k (blockIdx.z 0) or v (1).
 template <class E>
@@ -312,13 +320,13 @@ __global__ __launch_bounds__(kThreads) void read_kernel(CacheView c, int64_t lay
     const int head = blockIdx.y, is_v = blockIdx.z, d = c.head_dim;
     T* dst = is_v ? (T*)x.v + head * x.v_head : (T*)x.k + head * x.k_head;
     const int64_t stride = is_v ? x.v_token : x.k_token;
-    const float big = ((is_v ? c.v_max : c.k_max) + c.slab(layer, page) * c.kv_heads)[head];
+    const Values value(((is_v ? c.v_max : c.k_max) + c.slab(layer, page) * c.kv_heads)[head]);
     const int8_t* codes = (is_v ? c.v_codes : c.k_codes) + c.slab(layer, page) * c.page_codes() +
                           (int64_t)head * c.page_tokens * c.pitch;
     for (int e = threadIdx.x; e < (p.to - p.from) * d; e += kThreads) {
         const int t = e / d, col = e % d;
         const int code = is_v ? codes[col * c.page_tokens + p.from + t] : codes[(p.from + t) * c.pitch + col];
-        dst[(p.row + t) * stride + col] = E::store(__fdiv_rn((float)code * big, 127.0f));
+        dst[(p.row + t) * stride + col] = E::store(value(code));
     }
 }
 
@@ -336,12 +344,10 @@ __global__ __launch_bounds__(kThreads) void read_wide_kernel(CacheView c, int64_
     const int head = blockIdx.y, is_v = blockIdx.z, d = c.head_dim, per = d / 8, count = p.to - p.from;
     T* dst = is_v ? (T*)x.v + head * x.v_head : (T*)x.k + head * x.k_head;
     const int64_t stride = is_v ? x.v_token : x.k_token;
-    const float big = ((is_v ? c.v_max : c.k_max) + c.slab(layer, page) * c.kv_heads)[head];
+    const Values page_value(((is_v ? c.v_max : c.k_max) + c.slab(layer, page) * c.kv_heads)[head]);
     const int8_t* codes = (is_v ? c.v_codes : c.k_codes) + c.slab(layer, page) * c.page_codes() +
                           (int64_t)head * c.page_tokens * c.pitch;
-    auto value = [&](uint32_t word, int j) {
-        return E::store(__fdiv_rn((float)(int8_t)(word >> (8 * j)) * big, 127.0f));
-    };
+    auto value = [&](uint32_t word, int j) { return E::store(page_value((int8_t)(word >> (8 * j)))); };
     if (!is_v) {
         for (int e = threadIdx.x; e < count * per; e += kThreads) {
             const int t = e / per, col = 8 * (e % per);

@@ -81,3 +81,33 @@ def test_values_that_were_there(rt, dtype, tokens):
     np.testing.assert_array_equal(c.k_codes.download()[0, rows, :, :2], again(m.k[0, rows, :, :2]))
     np.testing.assert_array_equal(c.v_codes.download()[0, rows, :, :, :2], again(m.v[0, rows, :, :, :2]))
     c.close()
+
+
+@pytest.mark.parametrize("d", [64, 33])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_values_read_back(rt, dtype, d):
+    """code * max / 127 with maxima up to the largest number: two roundings, and
+    the result's; the plain kernel (33 columns) and that of 16-byte pieces."""
+    print("read large", dtype, d, flush=True)
+    rng = np.random.default_rng(d)
+    maxima = np.array(MAXIMA + [1.0, np.finfo(np.float32).max], np.float32)
+    n = len(maxima)
+    m = Model(1, n, 16, 1, d, n, 1)
+    assert m.extend(range(n), [16] * n)
+    rows = m.tables[:, 0]
+    m.k[0, rows, :, :, :d] = rng.integers(-127, 128, (n, 1, 16, d))
+    m.v[0, rows, :, :d] = rng.integers(-127, 128, (n, 1, d, 16))
+    m.k[0, rows, :, 3, :2], m.v[0, rows, :, 2, :2] = (127, -127), (127, -127)
+    m.km[0, rows], m.vm[0, rows] = maxima[:, None], maxima[::-1, None]
+    c = m.upload(rt)
+    outs = [rt.empty((16 * n, 1, d), np.float32 if dtype == "f32" else np.uint16) for _ in range(2)]
+    c.read(0, _dev(rt, _offsets([16] * n)), outs[0], outs[1], dtype=dtype)
+    for j, o in enumerate(outs):
+        got = from_bits(o.download(), dtype).astype(np.float64)
+        want = np.concatenate([m.values(0, i)[j] for i in range(n)])
+        top = np.float64(3.3895313892515355e38)  # bf16's largest; beyond its half step a result is infinite
+        seen = np.abs(want) <= (top if dtype == "bf16" else np.inf)
+        assert np.isfinite(got[seen]).all()
+        tol = np.abs(want) * (2.0 ** -23 + (2.0 ** -8 if dtype == "bf16" else 0)) * 1.01
+        assert (np.abs(got - want)[seen] <= tol[seen]).all()
+    c.close()
