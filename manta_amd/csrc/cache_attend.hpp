@@ -217,13 +217,16 @@ __device__ __forceinline__ void join_parts(const AttendArgs& a, const Tile& t, i
 #pragma unroll
         for (int u = 0; u < EACH; u++) {
             if (j + u * PER < parts) {
-                const float w = e[u][1] * __builtin_amdgcn_exp2f(e[u][0] - base);
-                weight[(j + u * PER) * RT + row] = w;
-                sum += w;
+                e[u][1] *= __builtin_amdgcn_exp2f(e[u][0] - base);
+                sum += e[u][1];
             }
         }
 #pragma unroll
         for (int x = 1; x < PER; x <<= 1) sum += __shfl_xor(sum, x);
+        // (at most 1: values near the largest number stay finite)
+#pragma unroll
+        for (int u = 0; u < EACH; u++)
+            if (j + u * PER < parts) weight[(j + u * PER) * RT + row] = e[u][1] / sum;
         if (j == 0) {
             top_m[row] = big;
             top_l[row] = sum;
@@ -250,7 +253,7 @@ __device__ __forceinline__ void join_parts(const AttendArgs& a, const Tile& t, i
                     if (s0 + u < s1) y += e[u] * weight[(s0 + u) * RT + row];
             }
         }
-        if (groups == 1) store_out<T>(a, t, kv, d, row, k, y / top_l[row], top_m[row], top_l[row]);
+        if (groups == 1) store_out<T>(a, t, kv, d, row, k, y, top_m[row], top_l[row]);
         else if (group < groups) *(f32x4*)&so[4 * threadIdx.x] = y;
     }
     if (groups == 1) return;
@@ -259,7 +262,7 @@ __device__ __forceinline__ void join_parts(const AttendArgs& a, const Tile& t, i
         const int row = threadIdx.x / (D / 4), k = 4 * (threadIdx.x % (D / 4));
         f32x4 y = {0, 0, 0, 0};
         for (int h = 0; h < groups; h++) y += *(const f32x4*)&so[4 * (h * items + threadIdx.x)];
-        store_out<T>(a, t, kv, d, row, k, y / top_l[row], top_m[row], top_l[row]);
+        store_out<T>(a, t, kv, d, row, k, y, top_m[row], top_l[row]);
     }
 }
 
