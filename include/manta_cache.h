@@ -196,6 +196,9 @@ int manta_rocm_cache_read(MantaRocm* rt, const MantaRocmCache* cache, int64_t la
  * window > 0 only p - window + 1 .. p; otherwise (window must be 0) all.  A
  * row that sees nothing gets zeros.  lse_dev, when given, f32
  * [tokens, heads]: log of the sum of exp(scale q k), -inf for such a row.
+ * Scores and sums are f32; the operand of the second product, weight times the
+ * page's v_max against the largest of those that the row sees, is rounded to
+ * f16 (2^-11, and to zero below 2^-32 of that largest one).
  * longest: about the longest sequence of the batch (it sets how the work is
  * split, not the result's meaning). */
 int manta_rocm_cache_attention(MantaRocm* rt, const MantaRocmCache* cache, int64_t layer, int dtype,

@@ -92,7 +92,50 @@ __device__ __forceinline__ float sum_quarters(float x) {
     return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-__device__ __forceinline__ float finite_or_zero(float x) { return x < INFINITY ? x : 0.0f; }
+// Weights of the second product.  A page's v is code * v_max / 127, so what a
+// key adds to a row is weight * v_max: its operand is taken against the largest
+// of those that the row sees.  With m the running maximum of the scores and D
+// that of score - m + log2 v_max (both of the keys that the row sees),
+//
+//   p = exp2(score - m + x),  x = log2 v_max - D + lift,
+//
+// is at most 2^lift (as often as the maxima are kept), and is rounded to f16
+// (half a step, 2^-11, as the operand of an f32 sum; codes are exact): zero
+// where it is 2^(-25 - lift) of the largest, whatever the scales of the row's
+// pages and of those it does not see.  The sum of the weights takes a block's p
+// times exp2(-x).  A block's log2 v_max is never taken to be below D - kFar, so
+// that this factor stays in f32's range: its p are zero in f16 either way.
+constexpr float kFar = 60.0f;
+// A product that is rounded before a sum takes it.
+__device__ __forceinline__ float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+// log2 v_max.  (0 and what is not finite: their p are replaced.)
+__device__ __forceinline__ float lead_of(float v_max) {
+    return __builtin_amdgcn_logf(fminf(fmaxf(v_max, 0x1p-126f), 0x1.fffffep127f));
+}
+enum BlockKind {
+    kBlockUsual = 0,
+    kBlockNone = 1,    // no such page: none of its keys is seen
+    kBlockPoison = 2,  // v_max is not finite: NaN to the rows that see it
+    kBlockEmpty = 3,   // v_max is 0: nothing to add
+};
+__device__ __forceinline__ BlockKind block_kind(bool bad, float v_max) {
+    return bad ? kBlockNone : !(v_max < INFINITY) ? kBlockPoison : v_max < 0x1p-126f ? kBlockEmpty : kBlockUsual;
+}
+__device__ __forceinline__ float or_zero(float top) { return top == -INFINITY ? 0.0f : top; }
+// What sums of p * code are of the row's values, over the sum of the weights: a
+// product of two factors, each in f32's range.
+struct Unit {
+    float a, b;
+    // D: less the lift
+    __device__ __forceinline__ Unit(float D, float sum) {
+        b = __builtin_amdgcn_exp2f(0.5f * D);
+        a = b / (127.0f * sum);
+    }
+    __device__ __forceinline__ f32x4 operator()(f32x4 y) const { return y * a * b; }
+};
 
 // The rows of a tile (the same for every thread of the workgroup).
 struct Tile {

@@ -42,12 +42,13 @@ struct Share {  // a workgroup's part of a tile's keys
 // scores and weights share one scale each.
 //
 //   score = q.code * (k_max / 127 * scale * log2 e), weight = exp2(score - m),
-//   out = R / 127 * sum(weight * (v_max / R) * code) / sum(weight)
+//   out = sum(weight * v_max / 127 * code) / sum(weight)
 //
-// with m the running maximum and R at least the largest v_max so far: weight *
-// (v_max / R) is at most 1 and is rounded to f16 (half a step, 2^-11, as the
-// operand of an f32 sum; codes are exact).  The pages' own scales would leave
-// f16's range, and the codes times them would be rounded once more.
+// by way of p (cache_attend.hpp), m and D each wave's own, kept at every step.
+constexpr float kLift = 15.0f;  // p is at most 2^15
+// Scores past this, whose steps are 2^-8 and more, are rounded before m is
+// taken from them: p must not pass 2^15 by such steps.
+constexpr float kLarge = 65536.0f;
 template <class E, int DP, int QT>
 __device__ __forceinline__ void attend_share(const CacheView& c, int64_t layer, const AttendArgs& a, const Tile& t,
                                              const Share& sh) {
@@ -135,11 +136,11 @@ __device__ __forceinline__ void attend_share(const CacheView& c, int64_t layer, 
         for (int i = 0; i < DT; i++) v16[i] = stream<QT == 1>((const u32x4*)(p + 16 * i * c.page_tokens));
     };
 
-    float m[QT], l[QT], R = 0.0f;
+    float m[QT], D_max[QT], l[QT];
     f32x4 o[QT][DT];
 #pragma unroll
     for (int n = 0; n < QT; n++) {
-        m[n] = -INFINITY;
+        m[n] = D_max[n] = -INFINITY;
         l[n] = 0.0f;
 #pragma unroll
         for (int i = 0; i < DT; i++) o[n][i] = f32x4{0, 0, 0, 0};
@@ -172,12 +173,10 @@ __device__ __forceinline__ void attend_share(const CacheView& c, int64_t layer, 
         if (more) load_k(x + step);
 
         const float kscale = ks * fabsf(a.scale);
-        const bool any_bad = __any(bad);
-        const bool whole = 64 * x >= lo_all && 64 * x + 63 < hi_all && !any_bad;
-        const float R2 = fmaxf(R, max_quarters(finite_or_zero(bad ? 0.0f : vs)));
-        const float w = R2 > 0.0f ? vs / R2 : vs;
-        const float shrink = R2 > R ? R / R2 : 1.0f;
-        R = R2;
+        const BlockKind kind = block_kind(bad, vs);
+        const bool odd = __any(kind != kBlockUsual);
+        const bool whole = 64 * x >= lo_all && 64 * x + 63 < hi_all && !odd;
+        const float lead = lead_of(vs);
         half8 p[QT][2];
 #pragma unroll
         for (int n = 0; n < QT; n++) {
@@ -193,29 +192,40 @@ __device__ __forceinline__ void attend_share(const CacheView& c, int64_t layer, 
             }
 #pragma unroll
             for (int k = 0; k < 16; k++) top = fmaxf(top, e[k]);
-            top *= factor;
+            top = rounded(top * factor);
             const float m2 = fmaxf(m[n], max_quarters(top));
-            const float base = m2 == -INFINITY ? 0.0f : m2;
+            float base = or_zero(m2);
             const float keep = __builtin_amdgcn_exp2f(m[n] - base);
-            if (__any(m2 > m[n] || shrink != 1.0f)) {
+            const float was = D_max[n] + (m[n] - base);
+            const float D2 = fmaxf(was, max_quarters(top - base + lead));
+            if (__any(D2 > was)) {
+                const float shrink = __builtin_amdgcn_exp2f(was - or_zero(D2));
 #pragma unroll
-                for (int i = 0; i < DT; i++) o[n][i] *= keep * shrink;
+                for (int i = 0; i < DT; i++) o[n][i] *= shrink;
             }
             m[n] = m2;
+            D_max[n] = D2;
+            if (__any(fabsf(base) > kLarge)) {
+#pragma unroll
+                for (int k = 0; k < 16; k++) e[k] = rounded(e[k] * factor) - base;
+                factor = 1.0f;
+                base = 0.0f;
+            }
+            const float scale = fmaxf(lead, D2 - kFar) - or_zero(D2) + kLift, shift = scale - base;
             float sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                e[k] = __builtin_amdgcn_exp2f(e[k] * factor - base);
+                e[k] = __builtin_amdgcn_exp2f(e[k] * factor + shift);
                 sum += e[k];
-                p[n][k >> 3][k & 7] = (_Float16)(e[k] * w);
+                p[n][k >> 3][k & 7] = (_Float16)e[k];
             }
-            if (!whole) {
-                // nothing of a page that the row does not see, not even its NaN
+            if (odd && (kind == kBlockPoison || kind == kBlockEmpty)) {
+                const _Float16 all = kind == kBlockPoison ? (_Float16)NAN : (_Float16)0.0f;
 #pragma unroll
                 for (int k = 0; k < 16; k++)
-                    p[n][k >> 3][k & 7] = k >= from && k < to ? p[n][k >> 3][k & 7] : (_Float16)0.0f;
+                    if (k >= from && k < to) p[n][k >> 3][k & 7] = all;
             }
-            l[n] = l[n] * keep + sum;
+            l[n] = l[n] * keep + sum * __builtin_amdgcn_exp2f(-scale);
         }
 #pragma unroll
         for (int i = 0; i < DT; i++) {
@@ -238,46 +248,45 @@ __device__ __forceinline__ void attend_share(const CacheView& c, int64_t layer, 
 
     // the waves' results joined
     __shared__ float so[kWaves * RT * OP];
-    __shared__ float sm[kWaves][RT], sl[kWaves][RT], sR[kWaves];
+    __shared__ float sm[kWaves][RT], sD[kWaves][RT], sl[kWaves][RT];
 #pragma unroll
     for (int n = 0; n < QT; n++) {
         l[n] = sum_quarters(l[n]);
         if (g == 0) {
             sm[wave][16 * n + col] = m[n];
+            sD[wave][16 * n + col] = D_max[n];
             sl[wave][16 * n + col] = l[n];
         }
 #pragma unroll
         for (int i = 0; i < DT; i++) *(f32x4*)&so[(wave * RT + 16 * n + col) * OP + 16 * i + 4 * g] = o[n][i];
     }
-    if (lane == 0) sR[wave] = R;
     __syncthreads();
-    R = sR[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; w++) R = fmaxf(R, sR[w]);
 
     // 4 columns a thread: of the output, or of this part
     const Parts parts_mem(a);
     for (int i = threadIdx.x; i < t.rows * (D / 4); i += kThreads) {
         const int row = i / (D / 4), k = 4 * (i % (D / 4));
-        float big = sm[0][row];
+        float big = sm[0][row], lead = -INFINITY;
 #pragma unroll
         for (int w = 1; w < kWaves; w++) big = fmaxf(big, sm[w][row]);
-        const float base = big == -INFINITY ? 0.0f : big;
+        const float base = or_zero(big);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) lead = fmaxf(lead, sD[w][row] + (sm[w][row] - base));
         float sum = 0.0f;
         f32x4 y = {0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
-            const float f = __builtin_amdgcn_exp2f(sm[w][row] - base);
-            sum += f * sl[w][row];
-            y += *(const f32x4*)&so[(w * RT + row) * OP + k] * (R > 0.0f ? f * (sR[w] / R) : f);
+            sum += __builtin_amdgcn_exp2f(sm[w][row] - base) * sl[w][row];
+            y += *(const f32x4*)&so[(w * RT + row) * OP + k] *
+                 __builtin_amdgcn_exp2f(sD[w][row] + (sm[w][row] - base) - or_zero(lead));
         }
-        const float unit = R / 127.0f;
+        const Unit unit(or_zero(lead) - kLift, sum);
         if (parts > 1) {
             const int at = sh.at(sh.part) + row * (OP * 4);
-            parts_mem.store(at + 4 * k, sum == 0.0f ? f32x4{0, 0, 0, 0} : y / sum * unit);
+            parts_mem.store(at + 4 * k, sum == 0.0f ? f32x4{0, 0, 0, 0} : unit(y));
             if (k == 0) parts_mem.store(at + 4 * D, f32x2{big, sum});
         } else {
-            store_out<T>(a, t, kv, d, row, k, y / sum * unit, big, sum);
+            store_out<T>(a, t, kv, d, row, k, unit(y), big, sum);
         }
     }
     if (parts == 1) return;

@@ -3,7 +3,7 @@
 // prefix.
 //
 // Bound by the instructions of the softmax and of staging beside the products:
-// 4 sequences of up to 4096 rows, 32 heads of 128 over 8, bf16: 643 us, 892
+// 4 sequences of up to 4096 rows, 32 heads of 128 over 8, bf16: 657 us, 872
 // TFLOP/s (a large product reaches 1174).  A workgroup takes 256 or 128 rows
 // (the query heads of a kv head, and tokens) and goes over the keys 64 at a
 // time: the codes become f16 (bf16 for k of bf16 queries) once per workgroup,
@@ -24,13 +24,14 @@ constexpr int kKeys = 64;  // of a step
 // page, with one scale), and the product v^T p takes its p from the registers
 // that hold them.
 //
-// A weight carries v_max / R, R the largest v_max of the keys, in its exponent
-// (the sum of the weights is freed of it block by block), and is rounded to
-// f16 (half a step, 2^-11, as the operand of an f32 sum): whatever the pages'
-// scales, codes stay exact.  (Codes scaled as they are staged would be rounded
-// with their scale: 1.8 times the rounding error of an f16 result, not 1.4.)  The running maximum that weights are taken against moves when a
-// score exceeds it by 8 or more (a weight is at most 256, in f16), so most
-// steps leave the sums alone.
+// A weight carries its page's v_max in its exponent (p of cache_attend.hpp), and
+// codes stay exact.  (Codes scaled as they are staged would be rounded with
+// their scale: 1.8 times the rounding error of an f16 result, not 1.4.)  A row's
+// m and D move when they are exceeded by 8 or more (p is at most 2^15), so most
+// steps leave the sums alone.  (Weights against the largest v_max of all the
+// tile's keys instead: 633 us for the 657 above, and rows that see only pages of
+// small v lose their weights to a page that they do not see.)
+constexpr float kSlack = 8.0f, kLift = 7.0f;
 template <class E, int DP, int WAVES, int OCC, bool ONE_PAGE>
 __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView c, int64_t layer, RaggedRows r,
                                                                   AttendArgs a) {
@@ -43,10 +44,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     constexpr int CHUNKS = kKeys * D / 16, EACH = (CHUNKS + kThreads - 1) / kThreads;
     __shared__ T k_lds[2][kKeys * KPITCH];
     __shared__ _Float16 v_lds[2][D * VPITCH];
-    // of each block of 16 keys: the factor of its scores; log2 of its weights'
-    // v_max / R, and the inverse of that; 1: no such page, 2: a largest v that is not finite
+    // of each block of 16 keys: the factor of its scores, log2 of its v_max, its kind
     __shared__ f32x4 block_lds[2][4];
-    __shared__ float wave_max[WAVES];
 
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -74,23 +73,6 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     const int8_t* vbase = c.v_codes + slab0 * page_codes + head_codes;
     const float* kmax = c.k_max + slab0 * c.kv_heads + kv;
     const float* vmax = c.v_max + slab0 * c.kv_heads + kv;
-
-    // R
-    float R = 0.0f;
-    if (c1 > c0) {
-        const int to = min((64 * (c1 - 1) + 63) >> c.page_shift, last_page);
-        for (int p = ((64 * c0) >> c.page_shift) + tid; p <= to; p += kThreads) {
-            const int page = table[p];
-            if ((unsigned)page < (unsigned)c.pages) R = fmaxf(R, finite_or_zero(vmax[(int64_t)page * c.kv_heads]));
-        }
-        R = max_quarters(R);
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) R = fmaxf(R, __shfl_xor(R, x));
-        if (lane == 0) wave_max[wave] = R;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) R = fmaxf(R, wave_max[w]);
-    }
 
     // the wave's rows, clamped (the doubles are not stored), as operands
     const int d = c.head_dim, wave_row = wave * 32;
@@ -128,10 +110,9 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     }
 
     // codes on their way to LDS
-    const float inv_R = R > 0.0f ? 1.0f / R : 0.0f;
     u32x4 kc[EACH], vc[EACH];
     float v_big = 0.0f, k_big = 0.0f;  // block tid % 4: largest v, largest k
-    int flag = 0;
+    bool bad = false;
     auto page_of = [&](int x, int block) { return table[min((64 * x + 16 * block) >> c.page_shift, last_page)]; };
     // Vector loads, though their addresses are the same for all: a scalar load
     // on its way would make every wait for LDS a wait for memory.
@@ -153,9 +134,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     };
     auto fetch = [&](int x) {
         x = min(x, c1 - 1);
-        bool bad = (unsigned)page_v >= (unsigned)c.pages;
+        bad = (unsigned)page_v >= (unsigned)c.pages;
         if (bad && tid < 4) cache_report(c, kCacheBadPage, page_v, 0);
-        flag = bad;
         const unsigned page = bad ? 0 : page_v;
         k_big = kmax[(int64_t)page * c.kv_heads];
         v_big = vmax[(int64_t)page * c.kv_heads];
@@ -208,17 +188,12 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             }
         }
         if (tid < 4) {
-            // (a largest v below 2^-40 R, or 0: as if it were 2^-40 R, whose
-            // weights are zero in f16 too.  One that is not finite: the same,
-            // and its weights become NaN where they are seen.)
-            const bool poison = !(v_big < INFINITY);
-            const float log_w = poison ? 0.0f : __builtin_amdgcn_logf(fmaxf(v_big * inv_R, 0x1p-40f));
-            block_lds[buf][tid] = f32x4{k_big * fabsf(a.scale), log_w, __builtin_amdgcn_exp2f(-log_w),
-                                        flag ? 1.0f : poison ? 2.0f : 0.0f};
+            block_lds[buf][tid] = f32x4{k_big * fabsf(a.scale), lead_of(v_big), (float)block_kind(bad, v_big), 0.0f};
         }
     };
 
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, D_max = -INFINITY, l = 0.0f;
+    float D0 = -kLift;  // D as p takes it: less the lift, and a margin
     f32x16 o[DP];
 #pragma unroll
     for (int i = 0; i < DP; i++) o[i] = f32x16{};
@@ -260,7 +235,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
         read_v(0);
         const f32x4 block0 = block_lds[buf][h], block1 = block_lds[buf][2 + h];
         const float ks0 = block0[0], ks1 = block1[0];
-        const bool odd = __any(block0[3] != 0.0f || block1[3] != 0.0f);
+        const bool odd = __any(block0[2] != kBlockUsual || block1[2] != kBlockUsual);
         const bool whole = 64 * x >= all_lo && 64 * x + 63 < all_hi && !odd;
         half8 p[2][2];
         float factor0 = ks0, factor1 = ks1;
@@ -269,8 +244,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             // (the scale first: it may be zero or NaN, which a key that is not seen must not meet)
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                s[0][k] = k >= from && k < to && block0[3] != 1.0f ? s[0][k] * ks0 : -INFINITY;
-                s[1][k] = k + 32 >= from && k + 32 < to && block1[3] != 1.0f ? s[1][k] * ks1 : -INFINITY;
+                s[0][k] = k >= from && k < to && block0[2] != kBlockNone ? s[0][k] * ks0 : -INFINITY;
+                s[1][k] = k + 32 >= from && k + 32 < to && block1[2] != kBlockNone ? s[1][k] * ks1 : -INFINITY;
             }
             factor0 = factor1 = 1.0f;
         }
@@ -280,20 +255,33 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
             top0 = fmaxf(top0, s[0][k]);
             top1 = fmaxf(top1, s[1][k]);
         }
-        const float top = max_halves(fmaxf(top0 * factor0, top1 * factor1));
-        if (__any(top > m + 8.0f)) {
-            const float m2 = fmaxf(m, top);
-            const float keep = __builtin_amdgcn_exp2f(m - (m2 == -INFINITY ? 0.0f : m2));
+        top0 = rounded(top0 * factor0);
+        top1 = rounded(top1 * factor1);
+        float base = or_zero(m);
+        const float top = max_halves(fmaxf(top0, top1));
+        const float most = max_halves(fmaxf(top0 - base + block0[1], top1 - base + block1[1]));
+        const bool move = top > m + kSlack || most > D_max + kSlack;
+        if (__any(move)) {
+            // (each row by itself: its result does not depend on the others)
+            const float m2 = move ? fmaxf(m, top) : m, base2 = or_zero(m2), up = base2 - base;
+            const float D2 = move ? fmaxf(D_max, most) - up : D_max;
+            // (Large scores: p may pass what D says by the steps of the score and of
+            // the shift below, 2^-23 of them together.  Up to 2^28 there is room.)
+            const float margin = fminf(0x1p-22f * fabsf(base2), 30.0f), D3 = or_zero(D2) - kLift + margin;
+            const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(D0 - up - D3);
 #pragma unroll
-            for (int i = 0; i < DP; i++) o[i] *= keep;
-            l *= keep;
+            for (int i = 0; i < DP; i++) o[i] *= shrink;
+            l *= __builtin_amdgcn_exp2f(m - base2);
             m = m2;
+            D_max = D2;
+            D0 = D3;
+            base = base2;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float scale[2] = {fmaxf(block0[1], D0 - kFar) - D0, fmaxf(block1[1], D0 - kFar) - D0};
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const float factor = b ? factor1 : factor0, shift = (b ? block1[1] : block0[1]) - base;
+            const float factor = b ? factor1 : factor0, shift = scale[b] - base;
 #pragma unroll
             for (int k = 0; k < 16; k++) {
                 const float e = __builtin_amdgcn_exp2f(s[b][k] * factor + shift);
@@ -301,14 +289,17 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
                 p[b][k >> 3][k & 7] = (_Float16)e;
             }
         }
-        l += sum[0] * block0[2] + sum[1] * block1[2];
+        l += sum[0] * __builtin_amdgcn_exp2f(-scale[0]) + sum[1] * __builtin_amdgcn_exp2f(-scale[1]);
         if (odd) {
             int from2 = from, to2 = to;
             asm("" : "+v"(from2), "+v"(to2));  // (compared anew: nothing of this is kept for the usual step)
+            const bool change0 = block0[2] >= kBlockPoison, change1 = block1[2] >= kBlockPoison;
+            const _Float16 all0 = block0[2] == kBlockPoison ? (_Float16)NAN : (_Float16)0.0f;
+            const _Float16 all1 = block1[2] == kBlockPoison ? (_Float16)NAN : (_Float16)0.0f;
 #pragma unroll
             for (int k = 0; k < 16; k++) {
-                if (k >= from2 && k < to2 && block0[3] == 2.0f) p[0][k >> 3][k & 7] = (_Float16)NAN;
-                if (k + 32 >= from2 && k + 32 < to2 && block1[3] == 2.0f) p[1][k >> 3][k & 7] = (_Float16)NAN;
+                if (k >= from2 && k < to2 && change0) p[0][k >> 3][k & 7] = all0;
+                if (k + 32 >= from2 && k + 32 < to2 && change1) p[1][k >> 3][k & 7] = all1;
             }
         }
 #pragma unroll
@@ -346,19 +337,19 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void attend_many_kernel(CacheView 
     const Parts mem(a);
     const int64_t tile = slot * c.kv_heads + kv;
     const int base_at = parts > 1 ? (int)(tile * a.splits) * (RT * OP * 4) : 0;
-    const float unit = R / 127.0f;
     l = sum_halves(l);
     const int row = wave_row + col;
     if (row < t.rows) {
         // (a part that saw no key joins as zeros)
-        const float inv = parts > 1 && l == 0.0f ? 0.0f : unit / l;
+        Unit unit(D0, l);
+        if (parts > 1 && l == 0.0f) unit.a = 0.0f;
         const int at = base_at + (split * RT + row) * (OP * 4);
 #pragma unroll
         for (int i = 0; i < DP; i++) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const int k = 32 * i + 8 * u + 4 * h;
-                const f32x4 y = f32x4{o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]} * inv;
+                const f32x4 y = unit(f32x4{o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]});
                 if (parts > 1) mem.store(at + 4 * k, y);
                 else store_out<T>(a, t, kv, d, row, k, y, m, l);
             }
