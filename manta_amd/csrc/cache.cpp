@@ -244,7 +244,11 @@ int manta_rocm_cache_create(MantaRocm* rt, const MantaRocmCacheShape* shape, Man
     v.pitch = (v.head_dim + 31) / 32 * 32;
     v.seqs = (int)shape->seqs;
     v.table_pages = (int)shape->table_pages;
-    v.err = manta_rt::cache_error_word(rt);
+    rc = manta_rt::cache_error_words(rt, &v.err, &v.err_flag, err);
+    if (rc) {
+        delete c;
+        return rc;
+    }
     c->max_count = v.layers * v.pages * v.kv_heads;
     c->code_bytes = v.layers * v.pages * v.page_codes();
     c->book_count = v.pages + v.seqs + (int64_t)v.seqs * v.table_pages;
@@ -288,7 +292,6 @@ int manta_rocm_cache_create(MantaRocm* rt, const MantaRocmCacheShape* shape, Man
         delete c;
         return fail(err, MANTA_ROCM_ERROR, "cache_create: out of memory");
     }
-    manta_rt::cache_errors_possible(rt);
     *out = c;
     return MANTA_ROCM_OK;
 }

@@ -171,6 +171,8 @@ __device__ __forceinline__ Owner find_owner(const CacheView& c, const RaggedRows
 
 __device__ __forceinline__ void cache_report(const CacheView& c, int kind, int64_t a, int64_t b) {
     atomicMax(c.err, cache_error(kind, a, b));
+    // (a plain store: atomics on host memory need what the link may not have)
+    __hip_atomic_store(c.err_flag, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 #endif
 

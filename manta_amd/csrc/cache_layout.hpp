@@ -35,6 +35,7 @@ struct CacheView {
     int32_t* tables;   // [seqs][table_pages]
     int32_t* refused;  // [seqs]: 1 from a refused extend until it is reported
     unsigned long long* err;
+    uint32_t* err_flag;  // host memory: 1 where *err may hold something
     int64_t layers, pages;
     int page_tokens, page_shift;
     int kv_heads, head_dim, pitch;

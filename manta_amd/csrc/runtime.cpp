@@ -72,8 +72,9 @@ struct MantaRocm {
     std::set<MantaRocmCandidates*> bound;
     // rotary tables and caches, likewise
     std::set<manta_rt::Attached*> attached;
-    // a cache was made: err_word[1] may hold what its kernels found wrong
-    bool cache_errors = false;
+    // pinned host memory, once a cache was made: not 0 where err_word[1] may
+    // hold what its kernels found wrong
+    volatile uint32_t* cache_flag = nullptr;
 };
 
 struct MantaRocmCandidates {
@@ -288,10 +289,12 @@ int check_gather_error(MantaRocm* rt, char** err) {
 }
 
 // What a cache kernel found wrong (cache_layout.hpp), reported and cleared by
-// the next synchronizing call.  Looked at on every such call once a cache
-// exists: a graph's replays leave no other sign.
+// the next synchronizing call.  The kernels leave a flag in host memory, so
+// that a call that finds nothing costs a read (a copy of the word with every
+// call, since a graph's replays leave no other sign: 20 us for 0.9).
 int check_cache_error(MantaRocm* rt, char** err) {
-    if (!rt->cache_errors) return MANTA_ROCM_OK;
+    if (!rt->cache_flag || !*rt->cache_flag) return MANTA_ROCM_OK;
+    *rt->cache_flag = 0;
     unsigned long long w = 0;
     HIP_TRY(hipMemcpyAsync(&w, rt->err_word + 1, sizeof(w), hipMemcpyDeviceToHost, rt->stream),
             "hipMemcpy(error word)");
@@ -425,6 +428,7 @@ void manta_rocm_destroy(MantaRocm* rt) {
     if (rt->ws_ref) (void)hipFree(rt->ws_ref);
     if (rt->err_word) (void)hipFree(rt->err_word);
     if (rt->tickets) (void)hipFree(rt->tickets);
+    if (rt->cache_flag) (void)hipHostFree((void*)rt->cache_flag);
     // candidate sets still bound: their device memory goes with the runtime,
     // their handles stay valid for manta_rocm_unbind (which then frees only
     // the handle)
@@ -1478,9 +1482,17 @@ void manta_rt::detach(MantaRocm* rt, Attached* a) {
     rt->attached.erase(a);
 }
 
-unsigned long long* manta_rt::cache_error_word(const MantaRocm* rt) { return rt->err_word + 1; }
-
-void manta_rt::cache_errors_possible(MantaRocm* rt) { rt->cache_errors = true; }
+int manta_rt::cache_error_words(MantaRocm* rt, unsigned long long** word, uint32_t** flag, char** err) {
+    if (!rt->cache_flag) {
+        void* p = nullptr;
+        HIP_TRY(hipHostMalloc(&p, sizeof(uint32_t), hipHostMallocMapped | hipHostMallocCoherent), "hipHostMalloc(error flag)");
+        *(uint32_t*)p = 0;
+        rt->cache_flag = (uint32_t*)p;
+    }
+    HIP_TRY(hipHostGetDevicePointer((void**)flag, (void*)rt->cache_flag, 0), "hipHostGetDevicePointer(error flag)");
+    *word = rt->err_word + 1;
+    return MANTA_ROCM_OK;
+}
 
 int manta_rt::pack_candidates_into(MantaRocm* rt, const MantaRocmCandidates* c, const int32_t* top, int64_t nq,
                                    int64_t k, const int64_t* candidate_ids, int64_t* out_ids, void* out_rows,

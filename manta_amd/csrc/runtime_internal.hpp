@@ -65,10 +65,9 @@ struct Attached {
 bool attach(MantaRocm* rt, Attached* a);  // false: out of memory
 void detach(MantaRocm* rt, Attached* a);
 
-// The device word the cache kernels report into, and the flag that makes
-// synchronizing calls look at it.
-unsigned long long* cache_error_word(const MantaRocm* rt);
-void cache_errors_possible(MantaRocm* rt);
+// The device word the cache kernels report into, and the word in host memory
+// (as the device sees it) that makes synchronizing calls look at it.
+int cache_error_words(MantaRocm* rt, unsigned long long** word, uint32_t** flag, char** err);
 
 // The index a gather error word holds (report_gather_error's encoding).
 inline int gather_error_index(unsigned long long w) { return (int)(uint32_t)(~w & 0xFFFFFFFFull); }
