@@ -32,7 +32,8 @@ enum {
 };
 
 /* One activation tensor [tokens, heads, head_dim] and where its result goes.
- * Strides are in elements; head_dim is contiguous.  out_dev may be x_dev with
+ * Strides are in elements; head_dim is contiguous, and rows that are written
+ * may not run into each other.  out_dev may be x_dev with
  * the same strides; otherwise the two must not overlap. */
 typedef struct MantaRocmHeads {
     const void* x_dev;

@@ -189,7 +189,7 @@ int manta_rocm_rotary(MantaRocm* rt, const MantaRocmRotary* rot, int dtype, cons
         if (tokens && (!h.x_dev || !h.out_dev))
             return fail(err, MANTA_ROCM_ERROR, "rotary: tensor %lld: nil pointer", (long long)i);
         const char* bad = manta::check_strides(tokens, h.heads, head_dim, h.x_token, h.x_head);
-        if (!bad) bad = manta::check_strides(tokens, h.heads, head_dim, h.out_token, h.out_head);
+        if (!bad) bad = manta::check_out_strides(tokens, h.heads, head_dim, h.out_token, h.out_head);
         if (bad) return fail(err, MANTA_ROCM_ERROR, "rotary: tensor %lld: %s", (long long)i, bad);
         if (h.x_dev == h.out_dev && (h.x_token != h.out_token || h.x_head != h.out_head))
             return fail(err, MANTA_ROCM_ERROR, "rotary: tensor %lld: in place needs equal strides", (long long)i);
@@ -400,11 +400,12 @@ int check_rows(MantaRocm* rt, const MantaRocmCache* c, const char* what, int64_t
 }
 
 int kv_rows(const MantaRocmCache* c, const char* what, int dtype, void* k, int64_t k_token, int64_t k_head, void* v,
-            int64_t v_token, int64_t v_head, int64_t tokens, manta::KvRows* out, char** err) {
+            int64_t v_token, int64_t v_head, int64_t tokens, bool written, manta::KvRows* out, char** err) {
     if (!manta::element_type(dtype)) return fail(err, MANTA_ROCM_ERROR, "%s: unknown element type %d", what, dtype);
     if (tokens > 0 && (!k || !v)) return fail(err, MANTA_ROCM_ERROR, "%s: nil pointer", what);
-    const char* bad = manta::check_strides(tokens, c->shape.kv_heads, c->shape.head_dim, k_token, k_head);
-    if (!bad) bad = manta::check_strides(tokens, c->shape.kv_heads, c->shape.head_dim, v_token, v_head);
+    const auto check = written ? manta::check_out_strides : manta::check_strides;
+    const char* bad = check(tokens, c->shape.kv_heads, c->shape.head_dim, k_token, k_head);
+    if (!bad) bad = check(tokens, c->shape.kv_heads, c->shape.head_dim, v_token, v_head);
     if (bad) return fail(err, MANTA_ROCM_ERROR, "%s: %s", what, bad);
     const int size = element_size(dtype);
     *out = {k, v, k_token, k_head, v_token, v_head, dtype,
@@ -422,7 +423,7 @@ int manta_rocm_cache_append(MantaRocm* rt, MantaRocmCache* c, int64_t layer, int
     int rc = check_rows(rt, c, "cache_append", layer, offsets, seqs, n, tokens, err);
     if (rc) return rc;
     manta::KvRows x;
-    rc = kv_rows(c, "cache_append", dtype, (void*)k, k_token, k_head, (void*)v, v_token, v_head, tokens, &x, err);
+    rc = kv_rows(c, "cache_append", dtype, (void*)k, k_token, k_head, (void*)v, v_token, v_head, tokens, false, &x, err);
     if (rc || n == 0 || tokens == 0) return rc;
     const manta::RaggedRows r{offsets, seqs, (int)n, (int)tokens};
     return launch(rt, "cache_append", err,
@@ -435,7 +436,7 @@ int manta_rocm_cache_read(MantaRocm* rt, const MantaRocmCache* c, int64_t layer,
     int rc = check_rows(rt, c, "cache_read", layer, offsets, seqs, n, tokens, err);
     if (rc) return rc;
     manta::KvRows x;
-    rc = kv_rows(c, "cache_read", dtype, k, k_token, k_head, v, v_token, v_head, tokens, &x, err);
+    rc = kv_rows(c, "cache_read", dtype, k, k_token, k_head, v, v_token, v_head, tokens, true, &x, err);
     if (rc || n == 0 || tokens == 0) return rc;
     const manta::RaggedRows r{offsets, seqs, (int)n, (int)tokens};
     return launch(rt, "cache_read", err,
@@ -457,7 +458,7 @@ int manta_rocm_cache_attention(MantaRocm* rt, const MantaRocmCache* c, int64_t l
                     (long long)c->shape.kv_heads);
     if (tokens > 0 && (!q->x_dev || !q->out_dev)) return fail(err, MANTA_ROCM_ERROR, "cache_attention: nil pointer");
     const char* bad = manta::check_strides(tokens, q->heads, d, q->x_token, q->x_head);
-    if (!bad) bad = manta::check_strides(tokens, q->heads, d, q->out_token, q->out_head);
+    if (!bad) bad = manta::check_out_strides(tokens, q->heads, d, q->out_token, q->out_head);
     if (bad) return fail(err, MANTA_ROCM_ERROR, "cache_attention: %s", bad);
     if (q->x_dev == q->out_dev && (q->x_token != q->out_token || q->x_head != q->out_head))
         return fail(err, MANTA_ROCM_ERROR, "cache_attention: in place needs equal strides");

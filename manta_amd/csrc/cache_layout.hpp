@@ -142,12 +142,30 @@ inline const char* check_cache_shape(const MantaRocmCacheShape& s) {
     return nullptr;
 }
 
-// strides of [tokens, heads, head_dim] elements: rows may not run into each
-// other when written
+// strides of [tokens, heads, head_dim] elements
 inline const char* check_strides(int64_t tokens, int64_t heads, int64_t head_dim, int64_t token, int64_t head) {
     if (token < 0 || head < 0) return "strides must not be negative";
     if (heads > 1 && head < head_dim) return "head stride is below head_dim";
     if (tokens > 1 && token < head_dim) return "token stride is below head_dim";
+    return nullptr;
+}
+
+// ... that are written: rows may not run into each other
+inline const char* check_out_strides(int64_t tokens, int64_t heads, int64_t head_dim, int64_t token, int64_t head) {
+    if (const char* bad = check_strides(tokens, heads, head_dim, token, head)) return bad;
+    if (tokens <= 1 || heads <= 1) return nullptr;
+    typedef __int128 wide;
+    if ((wide)token >= (wide)head * (heads - 1) + head_dim) return nullptr;  // heads within a token
+    if ((wide)head >= (wide)token * (tokens - 1) + head_dim) return nullptr;  // tokens within a head
+    // rows a of the one axis and b of the other apart start near each other
+    const bool few_heads = heads <= tokens;
+    const int64_t n = few_heads ? heads : tokens, most = few_heads ? tokens : heads;
+    const wide step = few_heads ? head : token, other = few_heads ? token : head;
+    for (int64_t a = 1; a < n; a++) {
+        const wide at = step * a, b = at / other;
+        if (b >= 1 && b < most && at - b * other < head_dim) return "rows of the result run into each other";
+        if (b + 1 < most && (b + 1) * other - at < head_dim) return "rows of the result run into each other";
+    }
     return nullptr;
 }
 
