@@ -174,13 +174,18 @@ int manta_rocm_cache_copy_pages(MantaRocm* rt, MantaRocmCache* cache, const int3
 
 /* Quantise k and v [tokens, kv_heads, head_dim] of one layer into the pages
  * (extended before; the sequences are distinct, and a page that another table
- * names too is skipped and reported).  Per page and head, max is the largest magnitude of its
- * tokens and code = round_half_even(x * 127 / max), in f32 (where x * 127 is
- * past the largest number, magnitudes above 2.67e36, +-127).  Tokens that the
- * page held before keep their codes; when the new tokens raise max, they
- * become round_half_even(code * old / max), at any magnitude.  A max below 2^-126 counts as 0
- * (all codes 0); a new value that is not finite makes max NaN, and with it
- * every result that attends to the page's head. */
+ * names too is skipped and reported).  Per page and head, max is the largest
+ * magnitude of the tokens appended to it since its first, and code =
+ * round_half_even(x * 127 / max), in f32; +-127 where x * 127 is past the
+ * largest number (magnitudes above 2.67e36).  Tokens that the page held before
+ * keep their codes; when the new tokens raise max, they become
+ * round_half_even(code * old / max), at any magnitude.  A max below 2^-126
+ * counts as 0 (all codes 0); a new value that is not finite makes max NaN, and
+ * with it every result that attends to the page's head.
+ * A max only rises until the page's first token is appended again: after
+ * release, or fork to a part of a page, it may be that of a token that is gone,
+ * and what is appended then is coded by it.  (A NaN stays likewise: the tokens
+ * left have lost their codes to it.) */
 int manta_rocm_cache_append(MantaRocm* rt, MantaRocmCache* cache, int64_t layer, int dtype, const void* k_dev,
                             int64_t k_token, int64_t k_head, const void* v_dev, int64_t v_token, int64_t v_head,
                             const int32_t* offsets_dev, const int32_t* seqs_dev, int64_t n, int64_t tokens,

@@ -670,9 +670,9 @@ template <class E>
 static hipError_t append_of(const CacheView& c, int64_t layer, const RaggedRows& r, const KvRows& x, hipStream_t s) {
     const dim3 grid((unsigned)ragged_slots(r.tokens, r.n, c.page_shift), c.kv_heads, 2);
     // a few tokens a sequence are soon done and wait less in the plain kernel
-    // (64 sequences, 8 heads of 128, with the read back: 1 token each 12.0 us
-    // against 16.1, 8 20.3 against 22.1, 16 26.5 against 25.0; prompts of up to
-    // 2048: 212 us against 73)
+    // (64 sequences, 8 heads of 128, with the read back: 1 token each 12.7 us
+    // against 16.4, 8 20.6 against 22.3, 16 27.0 against 24.6; prompts of up to
+    // 2048: 184 us against 74)
     if (!x.wide || c.head_dim % E::kWide != 0 || r.tokens < (int64_t)12 * r.n) {
         append_kernel<E><<<grid, kThreads, 0, s>>>(c, layer, r, x);
         return hipGetLastError();

@@ -15,8 +15,10 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kMaxSplits = 128;
 
 
-// A load of what nobody reads again (262145 keys of 8 heads of 128: 104 us
-// without the hint, 97 with it; two tiles of rows may share keys).
+// A load of what one tile of rows reads once (262145 keys of 8 heads of 128:
+// 108 us without the hint, 97 with it; 64 ragged sequences of up to 8192: 145
+// and 132).  Pages that branches share are read once a branch, and lose by it:
+// 64 branches of 16000 tokens 195 us without, 257 with it; of 1000, 35 and 36.
 template <bool ONCE, class V>
 __device__ __forceinline__ V stream(const V* p) {
     return ONCE ? __builtin_nontemporal_load(p) : *p;
@@ -446,11 +448,13 @@ hipError_t launch_few(const CacheView& c, int64_t layer, const RaggedRows& r, At
     // one).  One sequence: as many as that, all with the same work (262145
     // keys of 8 heads of 128: 104 us, with twice as many 113).  Several, of
     // lengths that the host does not know: twice as many, so that what the
-    // longest leave is small.
+    // longest leave is small.  (That holds for windows too, where all steps are
+    // alike: 16 of 5 tokens of 6 heads of 96 a kv head, the last 4096 keys: 40.1
+    // us, with half as many 41.5.)
     constexpr int RESIDENT = DP * QT <= 6 ? 2 : 1;
     int64_t splits = ((r.n == 1 ? 1 : 2) * RESIDENT * a.cus + live - 1) / live;
     if (splits > (chunks + kWaves - 1) / kWaves) splits = (chunks + kWaves - 1) / kWaves;
-    // joining costs as much as two steps (300 keys: 8.5 us alone, 9.7 in two
+    // joining costs as much as two steps (300 keys: 8.6 us alone, 9.9 in two
     // parts; 1000: 9.8 in two, 8.8 in four)
     if (chunks <= 2 * kWaves) splits = 1;
     const int64_t fit = a.partial_bytes / (tiles * RT * OP * 4);
@@ -463,6 +467,9 @@ hipError_t launch_few(const CacheView& c, int64_t layer, const RaggedRows& r, At
     // evenly.  64 sequences of up to 8192, 8 heads of 128: 131 us against 149;
     // 12: 41 against 44, and 8 (4 steps) 35.1 against 34.5; 20 of 16 heads of
     // 64 (13 steps): 54 against 58, and 32 of up to 4000 (11) 45.8 against 44.3.
+    // Windows (64 sequences, 4096 keys: 104 against 115; 1024: 41 against 44, not
+    // taken) and tiles of 32 rows (32 of 8 tokens, up to 4000 keys: 75 against
+    // 100; 8 of 7, not taken: 37.4 against 36.2) lie on the same line within 7%.
     constexpr int PLACES = DP <= 2 && QT == 1 ? 3 : RESIDENT;
     const int64_t places = (int64_t)PLACES * a.cus;
     if (r.n > 1 && r.n <= 64 && tiles <= a.ntickets &&
@@ -471,8 +478,8 @@ hipError_t launch_few(const CacheView& c, int64_t layer, const RaggedRows& r, At
         return hipGetLastError();
     }
     const int64_t rounds = (chunks + kWaves * splits - 1) / (kWaves * splits);
-    // wide heads have more to join (16 sequences of up to 8000, 2 heads of 256:
-    // 58 us with steps of 1, 50 of 2, 45 of 3)
+    // wide heads have more to join (8 sequences of up to 8000, 2 heads of 256: 33
+    // us with steps of 1, 25 of 2, 28 of 3; one sequence: 20, 22, 25)
     constexpr int LEAST = DP <= 4 ? 1 : 3;
     a.rounds = rounds < LEAST ? LEAST : (int)rounds;
     attend_few_kernel<E, DP, QT><<<dim3((unsigned)slots, c.kv_heads, (unsigned)splits), kThreads, 0, s>>>(c, layer, r, a);
@@ -497,8 +504,8 @@ template <class E>
 hipError_t launch_rows(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a, hipStream_t s) {
     const int64_t rows = ((int64_t)r.tokens * a.group + r.n - 1) / r.n;  // a sequence's, about
     if (rows <= 16) return launch_width<E, 1>(c, layer, r, a, s);
-    // (8 sequences of up to 16000, 64 rows each: 133 us in two tiles here, 106
-    // staged once there; 32 of up to 8000, 40 rows each: 166 either way)
+    // (8 sequences of up to 16000, 64 rows each: 85 us in two tiles here, 89
+    // staged once there; 32 of up to 8000, 40 rows each: 124 either way)
     if (rows <= 32) return launch_width<E, 2>(c, layer, r, a, s);
     return launch_attend_many(c, layer, r, a, s);
 }

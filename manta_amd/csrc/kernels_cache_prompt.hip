@@ -377,8 +377,10 @@ hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, A
     const int64_t chunks = (keys + 63) / 64;
     int64_t live = r.n * ((each * a.group + RT - 1) / RT) * c.kv_heads;
     if (live > tiles) live = tiles;
-    // Joining parts of 128 rows and more is dear (a prompt of 2048: 74 us whole,
-    // 100 in two parts): only for tiles that leave compute units empty.
+    // Joining parts of 128 rows and more is dear (a prompt of 2048: 65 us whole,
+    // 100 in two parts): only for tiles that leave compute units empty (4 of 30
+    // tokens over 30000 keys: 381 us in two parts, 112 in 16).  A prompt of 1000
+    // is near that line, and split: 49 us, whole 36.
     int64_t splits = OCC * 4 / WAVES * a.cus / live;
     if (splits > chunks / 8) splits = chunks / 8;
     const int64_t fit = a.partial_bytes / (tiles * RT * OP * 4);
@@ -396,8 +398,9 @@ hipError_t launch_many(const CacheView& c, int64_t layer, const RaggedRows& r, A
 
 // Tiles of 256 rows stage the keys half as often; of 128, two of which fit a
 // compute unit, they fill the card with fewer rows.  4 sequences of up to 4096,
-// 32 heads over 8 (1400 tiles of 256): 641 us and 668; 8 of up to 512 (512):
-// 74 and 72; one of 2048 (256): 74 and 64; 4 of 30 tokens, 8 heads over 1 (16): 141 and 113.
+// 32 heads over 8 (1400 tiles of 256): 651 us and 675; 8 of up to 512 (512): 74
+// and 71; one of 2048 (256): 76 and 65; 4 of 30 tokens, 8 heads over 1 (16): 144
+// and 112.
 template <class E, int DP>
 hipError_t launch_rows(const CacheView& c, int64_t layer, const RaggedRows& r, const AttendArgs& a, hipStream_t s) {
     const int64_t rows = ((int64_t)r.tokens + r.n - 1) / r.n * a.group;  // a sequence's, about
