@@ -61,17 +61,19 @@ class PassageReader:
         positions = np.concatenate([self.lengths[s] + np.arange(n) for s, n in zip(seqs, counts)])
         off, pos, sq = self._ints(offsets), self._ints(positions), self._ints(seqs)
         self.cache.extend(sq, self._ints(counts))  # once, for every layer
+        lengths = list(self.lengths)
         for s, n in zip(seqs, counts):
-            self.lengths[s] += n
+            lengths[s] += n
         x = np.concatenate([np.asarray(r, np.float32) for r in rows])
         for i, w in enumerate(self.layers):
             q, k = self._heads(x, w.q, self.q_heads), self._heads(x, w.k, self.kv_heads)
             v = self._heads(x, w.v, self.kv_heads)
             self.rt.rotary(self.rot, pos, [(q, q), (k, k)])
             self.cache.append(i, k, v, off, sq)
-            out = self.cache.attention(i, q, off, sq, longest=max(self.lengths))
+            out = self.cache.attention(i, q, off, sq, longest=max(lengths))
             y = out.download().view(np.float16).astype(np.float32)
             x = x + y.reshape(len(x), -1) @ w.o
+        self.lengths = lengths  # (a refused extend, reported by the downloads, has left the sequences as they were)
         return [x[a:b] for a, b in zip(offsets[:-1], offsets[1:])]
 
     def read(self, question: np.ndarray, passages: Sequence[np.ndarray], steps: Sequence[np.ndarray] = ()) -> np.ndarray:
