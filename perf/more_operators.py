@@ -262,8 +262,7 @@ def _prepare_own(case, x):
         s["x"] = _put(rt, x["x"])
         s["norm"] = _put(rt, x["norm"]) if case["norm"] else None
         s["add"] = _put(rt, x["add"]) if case.get("add") else None
-        s["codes"] = rt.empty((case["rows"], w.pitch), np.int8)
-        s["scales"] = rt.empty((case["rows"],), np.float32)
+        s["quantized"] = rt.quantized(case["rows"], case["k"])
         s["y"], yv = _empty(rt, (case["rows"], case["n"]), dt)
         s["out"] = {"out": yv}
     elif op == "rotary":
@@ -328,8 +327,8 @@ def run(s):
 def _run_own(s):
     case, op, rt = s["case"], s["case"]["op"], s["rt"]
     if op in ("product", "gated"):
-        rt.quantize_rows(s["x"], s["codes"], s["scales"], norm=s["norm"], eps=_EPS, dtype=case["dtype"])
-        rt.matmul_q8(s["weight"], s["codes"], s["scales"], out=s["y"], add=s["add"], dtype=case["dtype"])
+        rt.quantize_rows(s["x"], s["quantized"], norm=s["norm"], eps=_EPS, dtype=case["dtype"])
+        rt.matmul_q8(s["weight"], s["quantized"], out=s["y"], add=s["add"], dtype=case["dtype"])
     elif op == "rotary":
         rt.rotary_normed(s["rot"], s["pos"], s["parts"], s["norms"], eps=_EPS, dtype=case["dtype"])
     elif op == "beams":
