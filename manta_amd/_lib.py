@@ -21,12 +21,13 @@ PROJ_F16, PROJ_Q8_COL, PROJ_F16_T, PROJ_Q8_COL_T = 0, 1, 2, 3
 DENSE_F32, DENSE_F16 = 32, 16
 F32, F16, BF16 = 32, 16, 17
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+GATES = {None: 0, "silu": 1, "gelu": 2}
 ROTARY_NONE, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BLEND = 0, 1, 2, 3
 
 OPS = {"dot": DOT, "cosine": COSINE, "l2_distance": L2_DISTANCE}
 
 # Every exported symbol of include/manta_rocm.h, include/manta_cache.h,
-# include/manta_mll.h and include/manta_module.h:
+# include/manta_decode.h, include/manta_mll.h and include/manta_module.h:
 # name -> (restype, argtypes).
 _p = C.c_void_p
 _i64 = C.c_int64
@@ -216,6 +217,20 @@ SIGNATURES = {
         C.c_int, [_p, _p, _i64, C.c_int, _p, _p, _p, _p, _i64, _i64, C.c_double, C.c_int, _i64, _i64,
                   _err]),
     "manta_rocm_copy": (C.c_int, [_p, _p, _p, C.c_size_t, _err]),
+    # include/manta_decode.h
+    "manta_rocm_weight_bind": (C.c_int, [_p, _p, _p, _i64, _i64, C.c_int, C.POINTER(_p), _err]),
+    "manta_rocm_weight_unbind": (None, [_p]),
+    "manta_rocm_quantized_bytes": (_i64, [_i64, _i64]),
+    "manta_rocm_quantize_rows": (C.c_int, [_p, C.c_int, _p, _i64, _i64, _i64, _p, C.c_double, _p, _p, _err]),
+    "manta_rocm_matmul_q8": (
+        C.c_int, [_p, _p, _p, _p, _i64, C.c_int, _p, _i64, _p, _i64, _err]),
+    "manta_rocm_rotary_normed": (
+        C.c_int, [_p, _p, C.c_int, _p, _i64, _i64, _p, _p, _i64, C.c_double, _err]),
+    "manta_rocm_beams_create": (C.c_int, [_p, _i64, _i64, _i64, C.POINTER(_p), _err]),
+    "manta_rocm_beams_destroy": (None, [_p]),
+    "manta_rocm_beam_select": (
+        C.c_int, [_p, _p, C.c_int, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _err]),
+    "manta_rocm_cache_reorder": (C.c_int, [_p, _p, _p, _p, _i64, _i64, _err]),
     "manta_rocm_embed_pooled": (
         C.c_int,
         [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, C.c_int, _p, _i64, _p, _err],

@@ -20,8 +20,8 @@ SYNTH = os.path.join(HERE, "libmanta_synth.so")
 
 HIP_SOURCES = ["kernels_score.hip", "kernels_ref.hip", "kernels_topk.hip", "kernels_mq.hip", "kernels_mq4.hip", "kernels_mq8.hip",
                "kernels_embed.hip", "kernels_encoder.hip", "kernels_enc16.hip", "kernels_exec.hip", "kernels_dense.hip", "kernels_rotary.hip",
-               "kernels_cache.hip", "kernels_cache_attn.hip", "kernels_cache_prompt.hip", "noalloc.hip", "runtime.cpp", "cache.cpp", "mll.cpp",
-               "module.cpp", "program.cpp"]
+               "kernels_cache.hip", "kernels_cache_attn.hip", "kernels_cache_prompt.hip", "kernels_product.hip", "kernels_beams.hip", "noalloc.hip", "runtime.cpp", "cache.cpp", "decode.cpp",
+               "mll.cpp", "module.cpp", "program.cpp"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

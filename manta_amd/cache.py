@@ -93,7 +93,8 @@ class Rotary:
             pass
 
 
-def rotary(rt, rot: Rotary, positions, parts, inverse: bool, dtype: Optional[str]) -> None:
+def _parts(rot, parts, dtype):
+    """(element type, tokens, head_dim, the packed tensors, their number)."""
     parts = list(parts)
     if not parts:
         raise ValueError("rotary needs at least one tensor")
@@ -112,8 +113,26 @@ def rotary(rt, rot: Rotary, positions, parts, inverse: bool, dtype: Optional[str
             tokens, dim = t, d
         elif (t, d) != (tokens, dim):
             raise ValueError("rotary tensors must agree on tokens and head_dim")
+    return kind, tokens, dim, packed, len(parts)
+
+
+def rotary(rt, rot: Rotary, positions, parts, inverse: bool, dtype: Optional[str]) -> None:
+    kind, tokens, dim, packed, n = _parts(rot, parts, dtype)
     call("manta_rocm_rotary", rt.handle, rot.handle, kind, _ints("positions", positions, tokens), tokens, dim, packed,
-         len(parts), 1 if inverse else 0)
+         n, 1 if inverse else 0)
+
+
+def rotary_normed(rt, rot: Rotary, positions, parts, norms, eps: float, dtype: Optional[str]) -> None:
+    kind, tokens, dim, packed, n = _parts(rot, parts, dtype)
+    if len(norms) != n:
+        raise ValueError("rotary_normed needs a norm (or None) for each tensor (%d for %d)" % (len(norms), n))
+    addrs = []
+    for w in norms:
+        if w is not None and (w.dtype != np.float32 or tuple(w.shape) != (dim,) or w.strides not in (None, (1,))):
+            raise ValueError("a norm must be f32 [%d] (got %s %s)" % (dim, w.dtype, w.shape))
+        addrs.append(0 if w is None else w.addr)
+    call("manta_rocm_rotary_normed", rt.handle, rot.handle, kind, _ints("positions", positions, tokens), tokens, dim,
+         packed, struct.pack("=%dQ" % n, *addrs), n, eps)
 
 
 class _Part:
@@ -199,6 +218,13 @@ class Cache:
         n = seqs.shape[0]
         call("manta_rocm_cache_release", self.rt.handle, self.handle, _ints("seqs", seqs),
              None if keep is None else _ints("keep", keep, n), n)
+
+    def reorder(self, seqs, parents, group: Optional[int] = None) -> None:
+        """Groups of `group` sequences (all of them): entry i takes over what
+        entry parents[i] of its group held; -1 empties it."""
+        n = seqs.shape[0]
+        call("manta_rocm_cache_reorder", self.rt.handle, self.handle, _ints("seqs", seqs), _ints("parents", parents, n),
+             n, max(n, 1) if group is None else group)
 
     def compact(self, live=None) -> None:
         """Move live pages down into free ones; live: int32 [1], their count."""

@@ -10,10 +10,15 @@
 
 #include "cache_kernels.hpp"
 #include "cache_layout.hpp"
+#include "decode_layout.hpp"
+#include "launch_common.hpp"
 #include "runtime_internal.hpp"
 
 using manta::CacheView;
+using manta_rt::aligned16;
+using manta_rt::element_size;
 using manta_rt::fail;
+using manta_rt::launch;
 
 // Partial results of attention whose keys are split over workgroups, and the
 // tickets of the last one to finish (zero between calls).
@@ -58,36 +63,12 @@ struct MantaRocmCache : manta_rt::Attached {
 
 namespace {
 
-#define TRY_HIP(call, what)                                                             \
-    do {                                                                                \
-        hipError_t e_ = (call);                                                         \
-        if (e_ != hipSuccess)                                                           \
-            return fail(err, MANTA_ROCM_ERROR, "%s: %s (%s)", what, hipGetErrorName(e_), hipGetErrorString(e_)); \
-    } while (0)
-
-// A launch, counted and timed as the runtime's other kernels are.
-template <class F>
-int launch(MantaRocm* rt, const char* what, char** err, F f) {
-    void* ev = manta_rt::launch_begin(rt);
-    const hipError_t e = f((hipStream_t)manta_rt::runtime_stream(rt));
-    manta_rt::launch_end(rt, what, ev);
-    if (e != hipSuccess)
-        return fail(err, MANTA_ROCM_ERROR, "%s: %s (%s)", what, hipGetErrorName(e), hipGetErrorString(e));
-    return MANTA_ROCM_OK;
-}
-
 int check_cache(MantaRocm* rt, const MantaRocmCache* c, const char* what, char** err) {
     if (!c) return fail(err, MANTA_ROCM_ERROR, "%s: nil cache", what);
     if (!c->rt) return fail(err, MANTA_ROCM_ERROR, "%s: the cache's runtime is destroyed", what);
     if (c->rt != rt) return fail(err, MANTA_ROCM_ERROR, "%s: the cache belongs to another runtime", what);
     return manta_rt::use(rt, err);
 }
-
-bool aligned16(const void* p, int64_t a, int64_t b, int size) {
-    return ((uintptr_t)p % 16) == 0 && (a * size) % 16 == 0 && (b * size) % 16 == 0;
-}
-
-int element_size(int dtype) { return dtype == MANTA_ROCM_F32 ? 4 : 2; }
 
 }  // namespace
 
@@ -169,14 +150,15 @@ void manta_rocm_rotary_unbind(MantaRocmRotary* r) {
     delete r;
 }
 
-int manta_rocm_rotary(MantaRocm* rt, const MantaRocmRotary* rot, int dtype, const int32_t* positions_dev,
-                      int64_t tokens, int64_t head_dim, const MantaRocmHeads* parts, int64_t nparts, int inverse,
-                      char** err) {
-    if (!manta::element_type(dtype)) return fail(err, MANTA_ROCM_ERROR, "rotary: unknown element type %d", dtype);
+// manta_rocm_rotary, and with norms manta_rocm_rotary_normed.
+static int rotary_call(const char* what, MantaRocm* rt, const MantaRocmRotary* rot, int dtype,
+                       const int32_t* positions_dev, int64_t tokens, int64_t head_dim, const MantaRocmHeads* parts,
+                       const float* const* norms, int64_t nparts, double eps, int inverse, char** err) {
+    if (!manta::element_type(dtype)) return fail(err, MANTA_ROCM_ERROR, "%s: unknown element type %d", what, dtype);
     if (tokens < 0 || tokens > manta::kMaxTokens)
-        return fail(err, MANTA_ROCM_ERROR, "rotary: bad token count %lld", (long long)tokens);
+        return fail(err, MANTA_ROCM_ERROR, "%s: bad token count %lld", what, (long long)tokens);
     if (nparts < 1 || nparts > manta::kRotaryParts || !parts)
-        return fail(err, MANTA_ROCM_ERROR, "rotary: 1 to %d tensors (got %lld)", manta::kRotaryParts,
+        return fail(err, MANTA_ROCM_ERROR, "%s: 1 to %d tensors (got %lld)", what, manta::kRotaryParts,
                     (long long)nparts);
     manta::RotaryArgs a{};
     const int size = element_size(dtype), wide = 16 / size;
@@ -184,27 +166,27 @@ int manta_rocm_rotary(MantaRocm* rt, const MantaRocmRotary* rot, int dtype, cons
     for (int64_t i = 0; i < nparts; i++) {
         const MantaRocmHeads& h = parts[i];
         if (h.heads <= 0 || h.heads > 65535)
-            return fail(err, MANTA_ROCM_ERROR, "rotary: tensor %lld: 1 to 65535 heads (got %lld)", (long long)i,
+            return fail(err, MANTA_ROCM_ERROR, "%s: tensor %lld: 1 to 65535 heads (got %lld)", what, (long long)i,
                         (long long)h.heads);
         if (tokens && (!h.x_dev || !h.out_dev))
-            return fail(err, MANTA_ROCM_ERROR, "rotary: tensor %lld: nil pointer", (long long)i);
+            return fail(err, MANTA_ROCM_ERROR, "%s: tensor %lld: nil pointer", what, (long long)i);
         const char* bad = manta::check_strides(tokens, h.heads, head_dim, h.x_token, h.x_head);
         if (!bad) bad = manta::check_out_strides(tokens, h.heads, head_dim, h.out_token, h.out_head);
-        if (bad) return fail(err, MANTA_ROCM_ERROR, "rotary: tensor %lld: %s", (long long)i, bad);
+        if (bad) return fail(err, MANTA_ROCM_ERROR, "%s: tensor %lld: %s", what, (long long)i, bad);
         if (h.x_dev == h.out_dev && (h.x_token != h.out_token || h.x_head != h.out_head))
-            return fail(err, MANTA_ROCM_ERROR, "rotary: tensor %lld: in place needs equal strides", (long long)i);
+            return fail(err, MANTA_ROCM_ERROR, "%s: tensor %lld: in place needs equal strides", what, (long long)i);
         a.part[i] = {h.x_dev, h.out_dev, (int)h.heads, h.x_token, h.x_head, h.out_token, h.out_head};
         a.heads += (int)h.heads;
         a.wide = a.wide && aligned16(h.x_dev, h.x_token, h.x_head, size) &&
                  aligned16(h.out_dev, h.out_token, h.out_head, size);
     }
-    if (!rot) return fail(err, MANTA_ROCM_ERROR, "rotary: nil frequencies");
+    if (!rot) return fail(err, MANTA_ROCM_ERROR, "%s: nil frequencies", what);
     if (head_dim < rot->rot || head_dim > manta::kMaxHeadDim)
-        return fail(err, MANTA_ROCM_ERROR, "rotary: head_dim %lld must be %d (the rotated columns) to %d",
+        return fail(err, MANTA_ROCM_ERROR, "%s: head_dim %lld must be %d (the rotated columns) to %d", what,
                     (long long)head_dim, rot->rot, manta::kMaxHeadDim);
-    if (tokens && !positions_dev) return fail(err, MANTA_ROCM_ERROR, "rotary: nil positions");
-    if (!rot->rt) return fail(err, MANTA_ROCM_ERROR, "rotary: the frequencies' runtime is destroyed");
-    if (rot->rt != rt) return fail(err, MANTA_ROCM_ERROR, "rotary: the frequencies belong to another runtime");
+    if (tokens && !positions_dev) return fail(err, MANTA_ROCM_ERROR, "%s: nil positions", what);
+    if (!rot->rt) return fail(err, MANTA_ROCM_ERROR, "%s: the frequencies' runtime is destroyed", what);
+    if (rot->rt != rt) return fail(err, MANTA_ROCM_ERROR, "%s: the frequencies belong to another runtime", what);
     int rc = manta_rt::use(rt, err);
     if (rc || tokens == 0) return rc;
     a.parts = (int)nparts;
@@ -219,7 +201,27 @@ int manta_rocm_rotary(MantaRocm* rt, const MantaRocmRotary* rot, int dtype, cons
     a.dtype = dtype;
     // whole pieces of `wide` pairs and of `wide` copied columns
     a.wide = a.wide && (a.rot / 2) % wide == 0 && (a.head_dim - a.rot) % wide == 0;
-    return launch(rt, "rotary", err, [&](hipStream_t s) { return manta::launch_rotary(a, s); });
+    if (!norms) return launch(rt, what, err, [&](hipStream_t s) { return manta::launch_rotary(a, s); });
+    manta::RotaryNorms n{};
+    for (int64_t i = 0; i < nparts; i++) n.weight[i] = norms[i];
+    n.eps = eps;
+    return launch(rt, what, err, [&](hipStream_t s) { return manta::launch_rotary_normed(a, n, s); });
+}
+
+int manta_rocm_rotary(MantaRocm* rt, const MantaRocmRotary* rot, int dtype, const int32_t* positions_dev,
+                      int64_t tokens, int64_t head_dim, const MantaRocmHeads* parts, int64_t nparts, int inverse,
+                      char** err) {
+    return rotary_call("rotary", rt, rot, dtype, positions_dev, tokens, head_dim, parts, nullptr, nparts, 0.0, inverse,
+                       err);
+}
+
+int manta_rocm_rotary_normed(MantaRocm* rt, const MantaRocmRotary* rot, int dtype, const int32_t* positions_dev,
+                             int64_t tokens, int64_t head_dim, const MantaRocmHeads* parts,
+                             const float* const* norms_dev, int64_t nparts, double eps, char** err) {
+    if (!norms_dev) return fail(err, MANTA_ROCM_ERROR, "rotary_normed: nil norms");
+    if (const char* bad = manta::check_eps(eps)) return fail(err, MANTA_ROCM_ERROR, "rotary_normed: %s", bad);
+    return rotary_call("rotary_normed", rt, rot, dtype, positions_dev, tokens, head_dim, parts, norms_dev, nparts, eps,
+                       0, err);
 }
 
 // ------------------------------------------------------------------- cache
@@ -355,6 +357,22 @@ int manta_rocm_cache_release(MantaRocm* rt, MantaRocmCache* c, const int32_t* se
     if (!seqs) return fail(err, MANTA_ROCM_ERROR, "cache_release: nil pointer");
     return launch(rt, "cache_pages", err,
                   [&](hipStream_t s) { return manta::launch_cache_release(c->view, seqs, keep, (int)n, s); });
+}
+
+int manta_rocm_cache_reorder(MantaRocm* rt, MantaRocmCache* c, const int32_t* seqs, const int32_t* parents, int64_t n,
+                             int64_t group, char** err) {
+    int rc = check_cache(rt, c, "cache_reorder", err);
+    if (rc) return rc;
+    if (n < 0 || n > c->shape.seqs || n > manta::kMaxReorder)
+        return fail(err, MANTA_ROCM_ERROR, "cache_reorder: bad sequence count %lld", (long long)n);
+    if (group < 1 || group > manta::kMaxReorderGroup || n % group != 0)
+        return fail(err, MANTA_ROCM_ERROR, "cache_reorder: %lld sequences in groups of %lld", (long long)n,
+                    (long long)group);
+    if (n == 0) return MANTA_ROCM_OK;
+    if (!seqs || !parents) return fail(err, MANTA_ROCM_ERROR, "cache_reorder: nil pointer");
+    return launch(rt, "cache_pages", err, [&](hipStream_t s) {
+        return manta::launch_cache_reorder(c->view, seqs, parents, (int)n, (int)group, s);
+    });
 }
 
 int manta_rocm_cache_compact(MantaRocm* rt, MantaRocmCache* c, int32_t* live, char** err) {

@@ -31,6 +31,11 @@ struct RotaryArgs {
     int wide;  // every row starts on 16 bytes and splits into 16-byte pieces
 };
 hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s);
+struct RotaryNorms {
+    const float* weight[kRotaryParts];  // [head_dim] each, or nullptr: not normed
+    double eps;
+};
+hipError_t launch_rotary_normed(const RotaryArgs& a, const RotaryNorms& n, hipStream_t s);
 
 // ---- cache ----
 struct RaggedRows {
@@ -61,6 +66,8 @@ hipError_t launch_cache_extend(const CacheView& c, const PageScratch& w, const i
 hipError_t launch_cache_fork(const CacheView& c, const int32_t* parents, const int32_t* children,
                              const int32_t* tokens, int n, hipStream_t s);
 hipError_t launch_cache_release(const CacheView& c, const int32_t* seqs, const int32_t* keep, int n, hipStream_t s);
+hipError_t launch_cache_reorder(const CacheView& c, const int32_t* seqs, const int32_t* parents, int n, int group,
+                                hipStream_t s);
 hipError_t launch_cache_compact(const CacheView& c, const PageScratch& w, int32_t* live, hipStream_t s);
 // copy pages from[i] -> to[i], i < *count (count in device memory) or n, and
 // with remap [pages] replace the pages that the tables name

@@ -60,6 +60,8 @@ enum CacheError {
     kCacheBadCount = 5,  // a: the sequence, b: the count
     kCacheBadOffsets = 6,  // a: the entry of the batch
     kCacheShared = 7,      // a: the page
+    kCacheBadParent = 8,   // a: the entry, b: its parent
+    kCacheTwice = 9,       // a: the sequence
 };
 MANTA_HD unsigned long long cache_error(int kind, int64_t a, int64_t b) {
     return ((unsigned long long)kind << 60) | (((unsigned long long)a & 0x3FFFFFFFull) << 30) |
@@ -77,6 +79,8 @@ inline void describe_cache_error(unsigned long long w, char* out, size_t size) {
     else if (kind == kCacheInUse) snprintf(out, size, "cache sequence %lld is not empty", as);
     else if (kind == kCacheBadOffsets) snprintf(out, size, "cache offsets descend at entry %lld of the batch", as);
     else if (kind == kCacheShared) snprintf(out, size, "cache page %lld is shared: extend copies it before an append", as);
+    else if (kind == kCacheBadParent) snprintf(out, size, "cache reorder entry %lld: parent %lld out of range", as, bs);
+    else if (kind == kCacheTwice) snprintf(out, size, "cache reorder names sequence %lld twice", as);
     else snprintf(out, size, "cache sequence %lld: count %lld out of range", as, bs);
 }
 

@@ -1,0 +1,75 @@
+// decode_layout.hpp -- where quantised rows, bound weights and the parts of
+// beams lie, and the checks of the decoding calls' arguments.  Plain C++ (no
+// HIP), shared by the kernels, the C ABI and the CPU tests.
+#pragma once
+
+#include <math.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "cache_layout.hpp"
+#include "manta_decode.h"
+
+namespace manta {
+
+// ---- products in 8 bits ----
+// Both operands lie in blocks of 16 rows (tokens or output columns) and 64 of
+// the summed columns, 1 KB: four runs of 16 columns, each of them row after
+// row.  Lane l of a wave that reads 16 bytes at 16 l has row l % 16, columns
+// 16 (l / 16) to + 15: an operand of v_mfma_i32_16x16x64_i8.
+constexpr int64_t kMaxWidth = 131072;  // 127 * 128 * 131072 < 2^31
+constexpr int64_t kMaxColumns = 1 << 24;
+constexpr double kMinEps = 0x1p-126;
+
+MANTA_HD int64_t product_pitch(int64_t width) { return (width + 127) / 128 * 128; }
+MANTA_HD int64_t product_rows(int64_t rows) { return (rows + 15) / 16 * 16; }
+MANTA_HD int64_t product_at(int64_t pitch, int64_t r, int64_t c) {
+    return ((r >> 4) * (pitch >> 6) + (c >> 6)) * 1024 + ((c & 63) >> 4) * 256 + (r & 15) * 16 + (c & 15);
+}
+// The row of a bound weight that holds output column c: a gated weight's G
+// (half 0) and U (half 1) take turns in blocks of 16, so that a wave has both
+// factors of a result.
+MANTA_HD int64_t weight_row(int64_t c, int half, bool gated) {
+    return gated ? (c >> 4) * 32 + half * 16 + (c & 15) : c;
+}
+MANTA_HD int64_t weight_rows(int64_t n, bool gated) { return product_rows(n) * (gated ? 2 : 1); }
+
+inline const char* check_weight(int64_t width, int64_t n, int gate) {
+    if (width < 1 || width > kMaxWidth) return "width must be 1 to 131072";
+    if (n < 1 || n > kMaxColumns) return "columns must be 1 to 16777216";
+    if (gate < MANTA_ROCM_GATE_NONE || gate > MANTA_ROCM_GATE_GELU) return "unknown gate";
+    return nullptr;
+}
+inline const char* check_eps(double eps) {
+    return eps >= kMinEps && isfinite((float)eps) ? nullptr : "eps must be at least 2^-126 and finite";
+}
+
+// ---- beams ----
+constexpr int kMaxBeams = 64, kMaxBest = 64;
+constexpr int64_t kMaxBeamRows = 1 << 20;
+constexpr int kBeamPiece = 8192;  // logits that a workgroup holds at a time
+constexpr int kBeamParts = 64;    // workgroups of a row, at most
+// 64-bit words of a part: its best keys, its largest logit, its sum
+MANTA_HD int64_t beam_part_words(int64_t best) { return best + 2; }
+MANTA_HD int beam_parts(int64_t vocab) {
+    const int64_t pieces = (vocab + kBeamPiece - 1) / kBeamPiece;
+    return (int)(pieces < kBeamParts ? pieces : kBeamParts);
+}
+
+inline const char* check_beams(int64_t groups, int64_t beams, int64_t best) {
+    if (groups < 0 || beams < 1 || beams > kMaxBeams) return "1 to 64 beams";
+    if (best < 1 || best > kMaxBest) return "1 to 64 results a group";
+    if (groups > kMaxBeamRows / beams) return "more than 1048576 beams in all";
+    return nullptr;
+}
+
+// ---- reorder ----
+constexpr int64_t kMaxReorder = 4096, kMaxReorderGroup = 1024;
+constexpr int kReorderInts = 8192;   // table entries that a workgroup holds
+// columns of the tables that a workgroup takes
+MANTA_HD int reorder_columns(int64_t group) {
+    const int64_t c = kReorderInts / group;
+    return c >= 256 ? 256 : c >= 128 ? 128 : c >= 64 ? 64 : c >= 32 ? 32 : c >= 16 ? 16 : 8;
+}
+
+}  // namespace manta

@@ -5,6 +5,7 @@
 // waits for the host.  The layout and the mapping of ragged batches are in
 // cache_layout.hpp.
 #include "cache_kernels.hpp"
+#include "decode_layout.hpp"
 
 #pragma clang fp contract(off)
 
@@ -581,6 +582,77 @@ __global__ __launch_bounds__(kThreads) void release_kernel(CacheView c, const in
     if (tid == 0) c.lengths[seq] = keep;
 }
 
+// Entry i of a group takes over what entry parents[i] of it held.  A workgroup
+// takes `columns` columns of a group's tables: it holds the parents' entries
+// in LDS before it writes the first, so nothing that is still to be read is
+// overwritten, and no two workgroups touch one entry.  Past a sequence's pages
+// its table holds -1, so whole rows move without anybody's length, which the
+// first workgroup of a group replaces.  References are added and dropped where
+// an entry changes (their order does not matter: sums).  Every workgroup
+// checks the whole list, so that all of them or none go on: marks of refused
+// sequences are only set where every workgroup stops anyway.
+constexpr int kSeen = 1 << 17;  // slots whose first naming a workgroup remembers at a time
+__global__ __launch_bounds__(kThreads) void reorder_kernel(CacheView c, const int32_t* seqs, const int32_t* parents,
+                                                           int n, int group, int columns) {
+    extern __shared__ int32_t held[];  // [group][columns]
+    __shared__ uint32_t seen[kSeen / 32];
+    __shared__ int32_t slot[kMaxReorderGroup], parent[kMaxReorderGroup], length[kMaxReorderGroup];
+    const int tid = threadIdx.x;
+    const bool first = blockIdx.x == 0 && blockIdx.y == 0;
+    int wrong = 0;
+    for (int64_t s0 = 0; s0 < c.seqs; s0 += kSeen) {
+        const int words = (int)((min((int64_t)kSeen, c.seqs - s0) + 31) / 32);
+        for (int k = tid; k < words; k += kThreads) seen[k] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+            const int seq = seqs[i], p = parents[i];
+            if ((unsigned)seq >= (unsigned)c.seqs) {
+                if (first && s0 == 0) cache_report(c, kCacheBadSeq, seq, 0);
+                wrong = 1;
+            } else if (seq >= s0 && seq - s0 < kSeen) {
+                const int at = (int)(seq - s0);
+                if (atomicOr(&seen[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u) {
+                    if (first) cache_report(c, kCacheTwice, seq, 0);
+                    wrong = 1;
+                }
+                if (c.refused[seq]) wrong = 1;
+            }
+            if (p < -1 || p >= group) {
+                if (first && s0 == 0) cache_report(c, kCacheBadParent, i, p);
+                wrong = 1;
+            }
+        }
+        __syncthreads();
+    }
+    if (__syncthreads_or(wrong)) {
+        for (int i = tid; i < n && first; i += kThreads)
+            if ((unsigned)seqs[i] < (unsigned)c.seqs) c.refused[seqs[i]] = 1;
+        return;
+    }
+    const int base = blockIdx.y * group;
+    for (int i = tid; i < group; i += kThreads) {
+        slot[i] = seqs[base + i];
+        parent[i] = parents[base + i];
+    }
+    __syncthreads();
+    const int c0 = blockIdx.x * columns, width = min(columns, c.table_pages - c0);
+    for (int e = tid; e < group * width; e += kThreads)
+        held[e] = c.tables[(int64_t)slot[e / width] * c.table_pages + c0 + e % width];
+    if (blockIdx.x == 0)
+        for (int i = tid; i < group; i += kThreads) length[i] = c.lengths[slot[i]];
+    __syncthreads();
+    for (int e = tid; e < group * width; e += kThreads) {
+        const int i = e / width, col = e % width, p = parent[i];
+        const int before = held[e], after = p < 0 ? -1 : held[p * width + col];
+        if (before == after) continue;
+        c.tables[(int64_t)slot[i] * c.table_pages + c0 + col] = after;
+        if ((unsigned)before < (unsigned)c.pages) atomicSub(&c.refs[before], 1);
+        if ((unsigned)after < (unsigned)c.pages) atomicAdd(&c.refs[after], 1);
+    }
+    if (blockIdx.x == 0)
+        for (int i = tid; i < group; i += kThreads) c.lengths[slot[i]] = parent[i] < 0 ? 0 : length[parent[i]];
+}
+
 // One workgroup: the r-th live page at or past the live count moves to the
 // r-th free page below it.
 __global__ __launch_bounds__(kBook) void compact_kernel(CacheView c, PageScratch w, int32_t* live_out) {
@@ -721,6 +793,14 @@ hipError_t launch_cache_fork(const CacheView& c, const int32_t* parents, const i
 
 hipError_t launch_cache_release(const CacheView& c, const int32_t* seqs, const int32_t* keep, int n, hipStream_t s) {
     release_kernel<<<n, kThreads, 0, s>>>(c, seqs, keep);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_reorder(const CacheView& c, const int32_t* seqs, const int32_t* parents, int n, int group,
+                                hipStream_t s) {
+    const int columns = reorder_columns(group);
+    const dim3 grid((c.table_pages + columns - 1) / columns, n / group);
+    reorder_kernel<<<grid, kThreads, (size_t)group * columns * 4, s>>>(c, seqs, parents, n, group, columns);
     return hipGetLastError();
 }
 
