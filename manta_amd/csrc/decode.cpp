@@ -198,6 +198,7 @@ int manta_rocm_matmul_q8(MantaRocm* rt, const MantaRocmWeight* w, const int8_t* 
     const int size = element_size(dtype);
     a.wide = aligned(out, rows > 1 ? out_row : 0, 0, size, 4 * size) &&
              (!add || aligned(add, rows > 1 ? add_row : 0, 0, size, 4 * size));
+    a.wide16 = aligned16(out, rows > 1 ? out_row : 0, 0, size) && (!add || aligned16(add, rows > 1 ? add_row : 0, 0, size));
     a.cus = manta_rt::runtime_cus(rt);
     return launch(rt, "matmul_q8", err, [&](hipStream_t s) { return manta::launch_product(a, s); });
 }

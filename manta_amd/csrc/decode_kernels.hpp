@@ -37,7 +37,8 @@ struct ProductArgs {
     int steps;        // blocks of 64 summed columns
     int w_blocks;     // blocks of 16 weight rows
     int dtype, gate;
-    int wide;  // four columns of out (and add) are one aligned access
+    int wide;    // four columns of out (and add) are one aligned access
+    int wide16;  // 16 bytes of out (and add) are
     int cus;
 };
 hipError_t launch_product(const ProductArgs& a, hipStream_t s);

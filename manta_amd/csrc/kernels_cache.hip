@@ -5,6 +5,7 @@
 // waits for the host.  The layout and the mapping of ragged batches are in
 // cache_layout.hpp.
 #include "cache_kernels.hpp"
+#include "code_common.hpp"
 #include "decode_layout.hpp"
 
 #pragma clang fp contract(off)
@@ -136,31 +137,6 @@ __global__ __launch_bounds__(kThreads) void append_kernel(CacheView c, int64_t l
         if (!zero && col < d) q = quantise(E::load(src[(p.row + t) * stride + col]), big);
         codes[col * c.page_tokens + p.from + t] = (int8_t)q;
     }
-}
-
-// Four codes, t[j] / max rounded half to even, the division left out where it
-// cannot matter: t * (1 / max) is within 127 * 3 * 2^-24 < 2^-15 of it (three
-// roundings), so only what lies closer than that to a half is divided.  Adding
-// 1.5 * 2^23 rounds, and leaves the code in the low byte.  |t| <= 127 max, but
-// for t beyond the largest number; `exact`: there may be such a t (max >= 2^121;
-// its code is 127 or -127), or 1 / max is not a normal number.
-__device__ __forceinline__ uint32_t ratio_codes(const float* t, float max, float inv, bool exact) {
-    constexpr float kRound = 12582912.0f;
-    uint32_t b[4];
-    float far = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const float q = t[j] * inv, n = q + kRound;
-        far = fmaxf(far, fabsf(q - (n - kRound)));
-        b[j] = __float_as_uint(n);
-    }
-    if (exact || far > 0.5f - 0x1p-15f) {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            b[j] = (uint32_t)(int)fminf(127.0f, fmaxf(-127.0f, __builtin_rintf(__fdiv_rn(t[j], max))));
-    }
-    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u);
-    return lo | hi << 16;
 }
 
 // Rows that start on 16 bytes and split into 16-byte pieces.  The same

@@ -1,8 +1,12 @@
 // kernels_product.hip -- products in 8 bits for gfx950: rows quantised with a
 // scale each, times a weight with a scale a column, summed in int32 on
 // v_mfma_i32_16x16x64_i8.
+#include <atomic>
+
 #include "cache_kernels.hpp"
+#include "code_common.hpp"
 #include "decode_kernels.hpp"
+#include "mq_common.hpp"
 
 #pragma clang fp contract(off)
 
@@ -10,7 +14,6 @@ namespace manta {
 
 namespace {
 
-typedef int v4i __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------- quantise
@@ -80,6 +83,142 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantizeArgs a) {
     }
 }
 
+// The same results for rows that start on 16 bytes, each read once: 16 columns
+// a piece, NP pieces a thread, held in registers from the load until they are
+// coded.  WAVES waves a row; the rows of a block of 16 are taken on one XCD
+// (workgroup i runs on XCD i % 8), whose L2 joins their 16-byte runs into whole
+// lines.
+template <class E, bool NORM, int WAVES, int NP>
+__global__ __launch_bounds__(kThreads) void quantize_wide_kernel(QuantizeArgs a) {
+    typedef typename E::T T;
+    constexpr int V = E::kWide, L = 16 / V, RPW = kThreads / 64 / WAVES;  // rows of a workgroup
+    struct alignas(16) Pack16 {
+        T v[V];
+    };
+    __shared__ uint32_t tops[kThreads / 64];
+    __shared__ double sums[kThreads / 64];
+    constexpr int PER = 128 / RPW;  // workgroups of 8 blocks of rows
+    const int wave = threadIdx.x >> 6, in = blockIdx.x % PER;
+    const int64_t block = (int64_t)(blockIdx.x / PER) * 8 + in % 8;
+    const int64_t row = block * 16 + in / 8 * RPW + wave / WAVES;
+    const bool live = row < a.rows;
+    const int tid = threadIdx.x % (64 * WAVES);
+    const T* x = (const T*)a.x + (live ? row : 0) * a.x_row;
+    Pack16 held[NP][L];
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        const int c0 = (tid + 64 * WAVES * p) * 16;
+#pragma unroll
+        for (int l = 0; l < L; l++) {
+            held[p][l] = Pack16{};
+            const int c = c0 + l * V;
+            if (!live || c >= a.width) continue;
+            if (c + V <= a.width) held[p][l] = *(const Pack16*)(x + c);
+            else {
+#pragma unroll
+                for (int j = 0; j < V; j++)
+                    if (c + j < a.width) held[p][l].v[j] = x[c + j];
+            }
+        }
+    }
+    // z of piece p, element e
+    float w[NP][NORM ? 16 : 1];
+    if (NORM) {
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int c = (tid + 64 * WAVES * p) * 16 + e;
+                if (c + 4 <= a.width) {
+                    struct alignas(4) F4 {
+                        float v[4];
+                    };
+                    const F4 f = *(const F4*)(a.norm + c);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[p][NORM ? e + j : 0] = f.v[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[p][NORM ? e + j : 0] = c + j < a.width ? a.norm[c + j] : 0.0f;
+                }
+            }
+    }
+    auto value = [&](int p, int e) { return E::load(held[p][e / V].v[e % V]); };
+    auto z = [&](int p, int e) { return NORM ? value(p, e) * w[p][NORM ? e : 0] : value(p, e); };
+    uint32_t top = 0;
+    double sum = 0.0;
+#pragma unroll
+    for (int p = 0; p < NP; p++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            if (NORM) {
+                const double v = (double)value(p, e);
+                sum = fma(v, v, sum);
+            }
+            top = max(top, __float_as_uint(z(p, e)) & 0x7FFFFFFFu);
+        }
+    for (int s = 32; s; s >>= 1) {
+        top = max(top, (uint32_t)__shfl_xor((int)top, s));
+        if (NORM) sum += __shfl_xor(sum, s);
+    }
+    if (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) {
+            tops[wave] = top;
+            sums[wave] = sum;
+        }
+        __syncthreads();
+        sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) {
+            top = max(top, tops[wave / WAVES * WAVES + k]);
+            sum += sums[wave / WAVES * WAVES + k];
+        }
+    }
+    if (!live) return;
+    const bool bad = top >= 0x7F800000u;
+    const float big = __uint_as_float(top);
+    const bool zero = bad || big < 0x1p-126f;
+    if (tid == 0) {
+        float scale = 0.0f;
+        if (bad) scale = __builtin_nanf("");
+        else if (!zero) scale = NORM ? (float)((double)big / 127.0 / sqrt(sum / a.width + a.eps)) : __fdiv_rn(big, 127.0f);
+        a.scales[row] = scale;
+    }
+    const float inv = 1.0f / big;
+    const bool exact = big >= 0x1p121f;
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        const int c0 = (tid + 64 * WAVES * p) * 16;
+        if (c0 >= a.pitch) continue;
+        uint32_t word[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float t[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) t[j] = z(p, 4 * k + j) * 127.0f;
+            word[k] = zero ? 0 : ratio_codes(t, big, inv, exact);
+        }
+        *(uint4*)(a.codes + product_at(a.pitch, row, c0)) = make_uint4(word[0], word[1], word[2], word[3]);
+    }
+}
+
+template <class E, bool NORM>
+hipError_t quantize_of(const QuantizeArgs& a, hipStream_t s) {
+    const int64_t blocks = (a.rows + 127) / 128;
+    // a wave a row up to 1024 columns, a workgroup a row up to 32768
+    if (a.wide && a.width <= 1024) {
+        quantize_wide_kernel<E, NORM, 1, 1><<<(unsigned)(blocks * 32), kThreads, 0, s>>>(a);
+    } else if (a.wide && a.width <= 32768 && blocks < (1 << 16)) {
+        const dim3 grid((unsigned)(blocks * 128));
+        if (a.width <= 4096) quantize_wide_kernel<E, NORM, 4, 1><<<grid, kThreads, 0, s>>>(a);
+        else if (a.width <= 8192) quantize_wide_kernel<E, NORM, 4, 2><<<grid, kThreads, 0, s>>>(a);
+        else if (a.width <= 16384) quantize_wide_kernel<E, NORM, 4, 4><<<grid, kThreads, 0, s>>>(a);
+        else quantize_wide_kernel<E, NORM, 4, 8><<<grid, kThreads, 0, s>>>(a);
+    } else {
+        quantize_kernel<E><<<(unsigned)(a.rows < (1 << 20) ? a.rows : 1 << 20), kThreads, 0, s>>>(a);
+    }
+    return hipGetLastError();
+}
+
 // ----------------------------------------------------------------- product
 
 __device__ __forceinline__ float activate(float v, int gate) {
@@ -111,43 +250,97 @@ __device__ __forceinline__ void store4(const ProductArgs& a, int64_t row, int c,
         if (c + j < a.n) out[j] = E::store(add ? y[j] + E::load(add[j]) : y[j]);
 }
 
-// A 16 x 16 tile of sums: lane l has weight rows 16 wb + 4 (l / 16) + 0 .. 3
-// of token l % 16.
-__device__ __forceinline__ void scaled(const ProductArgs& a, int wb, float row_scale, v4i sums, float* y) {
-    const float4 t = *(const float4*)(a.w_scales + wb * 16 + 4 * ((threadIdx.x & 63) >> 4));
-    const float f[4] = {t.x, t.y, t.z, t.w};
+// Scales of NT weight blocks from wb on: lane l has those of rows
+// 4 (l / 16) + 0 .. 3 of each, as it has their sums (16 x 16 tiles: weight rows
+// 4 (l / 16) + 0 .. 3 of token l % 16).
+template <int NT>
+struct BlockScales {
+    float4 v[NT];
+    __device__ __forceinline__ BlockScales(const ProductArgs& a, int wb) {
+        const int c0 = 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-    for (int j = 0; j < 4; j++) y[j] = (float)sums[j] * (row_scale * f[j]);
-}
+        for (int t = 0; t < NT; t++) v[t] = *(const float4*)(a.w_scales + min(wb + t, a.w_blocks - 1) * 16 + c0);
+    }
+    __device__ __forceinline__ void times(int t, float row_scale, v4i sums, float* y) const {
+        const float f[4] = {v[t].x, v[t].y, v[t].z, v[t].w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = (float)sums[j] * (row_scale * f[j]);
+    }
+};
 
-// The results of NT weight blocks from block wb on for the token of this
-// lane (row, in range).
+// The results of NT weight blocks from block wb on for this lane's token
+// (row; stored if it is one).  Where rows allow 16-byte accesses of 16-bit
+// elements, two blocks' halves change places between neighbouring rows of 16
+// lanes, so that a lane has 8 columns in a row and a row of lanes 32 bytes of
+// each token: half as many stores, of whole 64-byte pieces.
 template <class E, bool GATED, int NT>
-__device__ __forceinline__ void finish(const ProductArgs& a, int64_t row, int wb, const v4i* sums) {
-    const float scale = a.x_scales[row];
-    const int c0 = 4 * ((threadIdx.x & 63) >> 4);
+__device__ __forceinline__ void finish(const ProductArgs& a, int64_t row, float row_scale, int wb,
+                                       const BlockScales<NT>& scales, const v4i* sums) {
+    constexpr int G = GATED ? 2 : 1, NR = NT / G;  // result blocks
+    const int g = (threadIdx.x & 63) >> 4;
+    const int first = GATED ? wb / 2 : wb, end = GATED ? a.w_blocks / 2 : a.w_blocks;
+    float y[NR][4];
 #pragma unroll
-    for (int t = 0; t < NT; t += GATED ? 2 : 1) {
-        if (wb + t >= a.w_blocks) break;
-        float y[4];
-        scaled(a, wb + t, scale, sums[t], y);
+    for (int r = 0; r < NR; r++) {
+        scales.times(r * G, row_scale, sums[r * G], y[r]);
         if (GATED) {
             float u[4];
-            scaled(a, wb + t + 1, scale, sums[t + (GATED ? 1 : 0)], u);
+            scales.times(r * G + G - 1, row_scale, sums[r * G + G - 1], u);
 #pragma unroll
-            for (int j = 0; j < 4; j++) y[j] = activate(y[j], a.gate) * u[j];
+            for (int j = 0; j < 4; j++) y[r][j] = activate(y[r][j], a.gate) * u[j];
         }
-        store4<E>(a, row, (GATED ? (wb + t) / 2 : wb + t) * 16 + c0, y);
     }
+    if constexpr (E::kWide == 8 && NR % 2 == 0) {
+        if (a.wide16) {
+            typedef typename E::T T;
+            struct alignas(16) Eight {
+                T v[8];
+            };
+#pragma unroll
+            for (int r = 0; r < NR; r += 2) {
+                float z[8];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(y[r][j]), __float_as_uint(y[r + 1][j]),
+                                                                    false, false);
+                    z[j] = __uint_as_float(p[0]);
+                    z[4 + j] = __uint_as_float(p[1]);
+                }
+                const int c = (first + r + (g & 1)) * 16 + (g >> 1) * 8;
+                if (row >= a.rows || first + r + (g & 1) >= end) continue;
+                T* out = (T*)a.out + row * a.out_row + c;
+                const T* add = a.add ? (const T*)a.add + row * a.add_row + c : nullptr;
+                if (c + 8 <= a.n) {
+                    Eight o, q{};
+                    if (add) q = *(const Eight*)add;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) o.v[j] = E::store(add ? z[j] + E::load(q.v[j]) : z[j]);
+                    *(Eight*)out = o;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (c + j < a.n) out[j] = E::store(add ? z[j] + E::load(add[j]) : z[j]);
+                }
+            }
+            return;
+        }
+    }
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int r = 0; r < NR; r++)
+        if (first + r < end) store4<E>(a, row, (first + r) * 16 + 4 * g, y[r]);
 }
 
-// A wave takes 16 MT tokens and 16 NT weight rows and reads both operands
-// where they lie: each is 16 bytes a lane, a block's KB in all.
-template <class E, bool GATED, int MT, int NT>
-__global__ __launch_bounds__(kThreads) void product_kernel(ProductArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wb = (blockIdx.x * (kThreads / 64) + wave) * NT;
-    if (wb >= a.w_blocks) return;
+// Few rows: the weight's bytes are what is read.  A workgroup takes all the
+// rows (16 MT at most) and 16 NT weight rows; its waves take U steps of the
+// summed columns in turn, read both operands where they lie (16 bytes a lane,
+// a block's KB in all) a turn ahead of their use, and join their sums, whole
+// numbers, in LDS.
+template <class E, bool GATED, int WAVES, int MT, int NT, int U>
+__global__ __launch_bounds__(WAVES * 64) void product_few_kernel(ProductArgs a) {
+    __shared__ v4i joined[WAVES][MT * NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wb = blockIdx.x * NT;
     const int64_t blocks = (a.rows + 15) / 16, rb = (int64_t)blockIdx.y * MT;
     const int8_t* xp[MT];
     const int8_t* wp[NT];
@@ -160,40 +353,214 @@ __global__ __launch_bounds__(kThreads) void product_kernel(ProductArgs a) {
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int t = 0; t < NT; t++) sums[m][t] = v4i{0, 0, 0, 0};
-    for (int k = 0; k < a.steps; k++) {
-        v4i xv[MT], wv[NT];
+    v4i xv[2][U][MT], wv[2][U][NT];
+    auto fetch = [&](int k0, int into) {
 #pragma unroll
-        for (int m = 0; m < MT; m++) xv[m] = *(const v4i*)(xp[m] + (int64_t)k * 1024);
+        for (int u = 0; u < U; u++) {
+            const int64_t at = (int64_t)min(k0 + u, a.steps - 1) * 1024;
 #pragma unroll
-        for (int t = 0; t < NT; t++) wv[t] = *(const v4i*)(wp[t] + (int64_t)k * 1024);
+            for (int t = 0; t < NT; t++) wv[into][u][t] = __builtin_nontemporal_load((const v4i*)(wp[t] + at));
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+            for (int m = 0; m < MT; m++) xv[into][u][m] = *(const v4i*)(xp[m] + at);
+        }
+    };
+    auto multiply = [&](int k0, int from) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) sums[m][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[t], xv[m], sums[m][t], 0, 0, 0);
+        for (int u = 0; u < U; u++) {
+            if (k0 + u >= a.steps) break;
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                    sums[m][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[from][u][t], xv[from][u][m], sums[m][t], 0, 0, 0);
+        }
+    };
+    constexpr int TURN = WAVES * U;
+    fetch(wave * U, 0);
+    for (int k = wave * U; k < a.steps; k += 2 * TURN) {
+        fetch(k + TURN, 1);
+        multiply(k, 0);
+        fetch(k + 2 * TURN, 0);
+        multiply(k + TURN, 1);
     }
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) joined[wave][m * NT + t][lane] = sums[m][t];
+    __syncthreads();
+    constexpr int G = GATED ? 2 : 1;  // tiles that finish together
+    for (int i = wave; i < MT * NT / G; i += WAVES) {
+        const int m = i / (NT / G), t = i % (NT / G) * G;
+        v4i all[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            all[g] = joined[0][m * NT + t + g][lane];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) all[g] += joined[w][m * NT + t + g][lane];
+        }
         const int64_t row = (rb + m) * 16 + (lane & 15);
-        if (row < a.rows) finish<E, GATED, NT>(a, row, wb, sums[m]);
+        finish<E, GATED, G>(a, row, a.x_scales[min(row, a.rows - 1)], wb + t, BlockScales<G>(a, wb + t), all);
     }
 }
 
+// Many rows: a workgroup of WM x WN waves takes 16 WM MT tokens and 16 WN NT
+// weight rows, a wave MT x NT tiles of 16 x 16.  Blocks of both operands
+// stream through LDS, ST of the summed columns' steps ahead of the products,
+// by direct-to-LDS loads: a block is 1 KB in a row where it lies and where it
+// goes, and a wave reads it back 16 bytes a lane in order, so neither side
+// has a bank conflict.
+//
+// 8192 x 4096 x 4096 bf16: 121 us, 2.27 POP/s (torch's int8 product of that
+// size, without scales: 130).  What bounds it: a step's products alone take 54
+// of a 256 x 256 tile's 67 us when the whole card works on random codes (the
+// clock falls with the matrix cores' load: 43 us on 16 compute units), the
+// fill of 32 KB a step about 45 bytes a clock.
+template <class E, bool GATED, int WM, int WN, int MT, int NT, int ST>
+__global__ __launch_bounds__(WM* WN * 64) void product_tile_kernel(
+    ProductArgs a, int row_tiles, int w_tiles) {
+    constexpr int TM = WM * MT, TN = WN * NT, WAVES = WM * WN;
+    constexpr int LPW = (TM + TN) / WAVES;  // blocks that a wave loads a step
+    static_assert(LPW * WAVES == TM + TN, "a step's blocks split evenly over the waves");
+    constexpr int STAGE = (TM + TN) * 1024;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // Workgroup i runs on XCD i % 8: each XCD takes a run of tiles, in strips
+    // of 8 row tiles, so that its 32 workgroups share 8 + 4 tiles' operands in
+    // its L2.
+    int rt, wt;
+    {
+        const int total = row_tiles * w_tiles, xcd = blockIdx.x & 7;
+        const int t = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
+        const int strip = 8 * w_tiles, first = t / strip * 8, rows = min(8, row_tiles - first), in = t % strip;
+        rt = first + in % rows;
+        wt = in / rows;
+    }
+    const int64_t x_blocks = (a.rows + 15) / 16;
+    const int8_t* src[LPW];
+#pragma unroll
+    for (int i = 0; i < LPW; i++) {
+        const int b = wave * LPW + i;
+        // (blocks past the operand read its last one; nothing of theirs is stored)
+        const int8_t* p = b < TM ? a.x + min((int64_t)rt * TM + b, x_blocks - 1) * a.steps * 1024
+                                 : a.w + (int64_t)min(wt * TN + b - TM, a.w_blocks - 1) * a.steps * 1024;
+        src[i] = p + lane * 16;
+    }
+    const uint32_t base = lds_addr(smem) + wave * LPW * 1024;
+    auto issue = [&](int k) {
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(base + (k % ST) * STAGE);
+#pragma unroll
+        for (int i = 0; i < LPW; i++) {
+            lds_load16(src[i], dst + i * 1024);
+            src[i] += 1024;
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < ST; k++)
+        if (k < a.steps) issue(k);
+    v4i sums[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) sums[m][t] = v4i{0, 0, 0, 0};
+    const int m0 = wave % WM * MT, t0 = wave / WM * NT;  // this wave's blocks of the tile
+    v4i wv[2][NT], xv[2][MT];
+    auto read = [&](int k, int into) {
+        const uint8_t* stage = smem + (k % ST) * STAGE + lane * 16;
+#pragma unroll
+        for (int t = 0; t < NT; t++) wv[into][t] = *(const v4i*)(stage + (TM + t0 + t) * 1024);
+#pragma unroll
+        for (int m = 0; m < MT; m++) xv[into][m] = *(const v4i*)(stage + (m0 + m) * 1024);
+    };
+    auto multiply = [&](int from) {
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+                sums[m][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[from][t], xv[from][m], sums[m][t], 0, 0, 0);
+    };
+    // Step k's products run while step k + 1's operands come out of LDS.  At
+    // the barrier step k + 1 has arrived and every wave holds step k, whose
+    // place step k + ST takes.
+    auto step = [&](int k, int now) {
+        if (k + 1 < a.steps) {
+            mq_wait_barrier<LPW, ST - 2>(a.steps - 2 - k);
+            if (k + ST < a.steps) issue(k + ST);
+            read(k + 1, now ^ 1);
+        }
+        multiply(now);
+    };
+    mq_wait_barrier<LPW, ST - 1>(a.steps - 1);
+    read(0, 0);
+    for (int k = 0; k < a.steps; k += 2) {  // (steps is even)
+        step(k, 0);
+        step(k + 1, 1);
+    }
+    const int64_t row0 = ((int64_t)rt * TM + m0) * 16 + (lane & 15);
+    const BlockScales<NT> scales(a, wt * TN + t0);
+    float row_scales[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) row_scales[m] = a.x_scales[min(row0 + 16 * m, a.rows - 1)];
+#pragma unroll
+    for (int m = 0; m < MT; m++) finish<E, GATED, NT>(a, row0 + 16 * m, row_scales[m], wt * TN + t0, scales, sums[m]);
+}
+
+template <class E, bool GATED, int WM, int WN, int MT, int NT, int ST>
+hipError_t product_tiles(const ProductArgs& a, hipStream_t s) {
+    constexpr int TM = WM * MT, TN = WN * NT;
+    const size_t lds = (size_t)ST * (TM + TN) * 1024;
+    int device = 0;
+    if (const hipError_t e = hipGetDevice(&device)) return e;
+    static std::atomic<uint64_t> set{0};  // devices whose kernel may use that much LDS
+    if (!(set.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
+        const hipError_t e = hipFuncSetAttribute((const void*)product_tile_kernel<E, GATED, WM, WN, MT, NT, ST>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+        set.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
+    }
+    const int64_t row_tiles = (a.rows + 16 * TM - 1) / (16 * TM), w_tiles = (a.w_blocks + TN - 1) / TN;
+    product_tile_kernel<E, GATED, WM, WN, MT, NT, ST>
+        <<<(unsigned)(row_tiles * w_tiles), WM * WN * 64, lds, s>>>(a, (int)row_tiles, (int)w_tiles);
+    return hipGetLastError();
+}
+
+template <class E, bool GATED, int WAVES, int MT, int NT, int U>
+hipError_t product_few(const ProductArgs& a, hipStream_t s) {
+    const dim3 grid((a.w_blocks + NT - 1) / NT, (unsigned)((a.rows + 16 * MT - 1) / (16 * MT)));
+    product_few_kernel<E, GATED, WAVES, MT, NT, U><<<grid, WAVES * 64, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+// Which tile: figures are bf16, 4096 summed columns, us on 256 compute units.
 template <class E, bool GATED>
 hipError_t product_of(const ProductArgs& a, hipStream_t s) {
-    constexpr int MT = 4, NT = 4;
-    const int64_t row_tiles = ((a.rows + 15) / 16 + MT - 1) / MT;
-    for (int64_t r0 = 0; r0 < row_tiles; r0 += 32768) {  // (a grid's second axis is 16 bits)
-        ProductArgs p = a;
-        const int64_t first = r0 * MT * 16;
-        p.x += first * a.steps * 64;
-        p.x_scales += first;
-        p.rows = a.rows - first;
-        p.out = (typename E::T*)a.out + first * a.out_row;
-        if (a.add) p.add = (const typename E::T*)a.add + first * a.add_row;
-        const dim3 grid((a.w_blocks + 4 * NT - 1) / (4 * NT), (unsigned)(row_tiles - r0 < 32768 ? row_tiles - r0 : 32768));
-        product_kernel<E, GATED, MT, NT><<<grid, kThreads, 0, s>>>(p);
-    }
-    return hipGetLastError();
+    const int64_t rb = (a.rows + 15) / 16, wb = a.w_blocks;
+    auto few = [&](int mt, int nt) { return ((rb + mt - 1) / mt) * ((wb + nt - 1) / nt); };
+    // The smallest tile that still is a workgroup a compute unit or less: more
+    // of them share the reading of the weight, and its latency (32 rows x 4096
+    // columns: 16 x 32 tiles 5.9, 32 x 32 7.3; 64 x 4096: 64 x 32 9.1, tiles
+    // through LDS 14.9)
+    if constexpr (!GATED)
+        if (few(1, 1) <= a.cus) return product_few<E, GATED, 8, 1, 1, 4>(a, s);
+    if (few(1, 2) <= a.cus) return product_few<E, GATED, 8, 1, 2, 2>(a, s);
+    if (few(2, 2) <= a.cus) return product_few<E, GATED, 8, 2, 2, 2>(a, s);
+    if (few(4, 2) <= a.cus) return product_few<E, GATED, 4, 4, 2, 2>(a, s);
+    // Up to 32 rows of more columns, where the weight's bytes are all that
+    // counts (16 rows x 24576 columns: 16.6, tiles 18.2; 32 rows are even)
+    if (rb == 1) return product_few<E, GATED, 8, 1, 2, 2>(a, s);
+    if (rb == 2) return product_few<E, GATED, 8, 2, 2, 2>(a, s);
+    // Tiles of 64 x 64 while those are few: a larger tile of a unit's own takes
+    // as long as several of them (512 x 4096: 17.5, 128 x 128 26.9; 1024 x 4096
+    // 29.0, 30.8; 512 x 12288 40.2, 37.9)
+    const int64_t t64 = ((a.rows + 63) / 64) * ((wb + 3) / 4), t128 = ((a.rows + 127) / 128) * ((wb + 7) / 8);
+    if (t64 <= 4 * a.cus) return product_tiles<E, GATED, 2, 2, 2, 2, 4>(a, s);
+    // 256 x 256 needs half of the operands' reads of 128 x 128, but comes in
+    // whole rounds of a tile a unit, 57 each, against 17.5 for a 128 x 128 tile
+    // a unit and 10 (1024 x 12288: 60.1 and 66.0; 2048 x 4096: 57.7 and 43;
+    // 8192 x 4096: 121 and 158)
+    const int64_t t256 = ((a.rows + 255) / 256) * ((wb + 15) / 16);
+    if ((t256 + a.cus - 1) / a.cus * 13 <= t128 * 4 / a.cus + 2) return product_tiles<E, GATED, 2, 4, 8, 4, 2>(a, s);
+    return product_tiles<E, GATED, 2, 2, 4, 4, 2>(a, s);
 }
 
 template <class E>
@@ -204,11 +571,10 @@ hipError_t product_type(const ProductArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_quantize_rows(const QuantizeArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)(a.rows < (1 << 20) ? a.rows : 1 << 20));
-    if (a.dtype == MANTA_ROCM_F32) quantize_kernel<F32><<<grid, kThreads, 0, s>>>(a);
-    else if (a.dtype == MANTA_ROCM_F16) quantize_kernel<F16><<<grid, kThreads, 0, s>>>(a);
-    else quantize_kernel<Bf16><<<grid, kThreads, 0, s>>>(a);
-    return hipGetLastError();
+    const bool norm = a.norm != nullptr;
+    if (a.dtype == MANTA_ROCM_F32) return norm ? quantize_of<F32, true>(a, s) : quantize_of<F32, false>(a, s);
+    if (a.dtype == MANTA_ROCM_F16) return norm ? quantize_of<F16, true>(a, s) : quantize_of<F16, false>(a, s);
+    return norm ? quantize_of<Bf16, true>(a, s) : quantize_of<Bf16, false>(a, s);
 }
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t s) {
