@@ -274,9 +274,28 @@ struct BlockScales {
 // lanes, so that a lane has 8 columns in a row and a row of lanes 32 bytes of
 // each token: half as many stores, of whole 64-byte pieces.
 template <class E, bool GATED, int NT>
+struct Added {  // what such a lane adds, asked for ahead
+    static constexpr int NR = NT / (GATED ? 2 : 1);  // result blocks
+    static constexpr bool kPairs = E::kWide == 8 && NR % 2 == 0;
+    struct alignas(16) Eight {
+        typename E::T v[8];
+    };
+    Eight v[NR / 2 + 1];
+    __device__ __forceinline__ void fetch(const ProductArgs& a, int64_t row, int wb) {
+        if (GATED || !kPairs || !a.wide16 || !a.add || row >= a.rows) return;
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int r = 0; r + 1 < NR; r += 2) {
+            const int c = (wb + r + (g & 1)) * 16 + (g >> 1) * 8;
+            if (c + 8 <= a.n) v[r / 2] = *(const Eight*)((const typename E::T*)a.add + row * a.add_row + c);
+        }
+    }
+};
+template <class E, bool GATED, int NT>
 __device__ __forceinline__ void finish(const ProductArgs& a, int64_t row, float row_scale, int wb,
-                                       const BlockScales<NT>& scales, const v4i* sums) {
-    constexpr int G = GATED ? 2 : 1, NR = NT / G;  // result blocks
+                                       const BlockScales<NT>& scales, const v4i* sums,
+                                       const Added<E, GATED, NT>& added) {
+    constexpr int G = GATED ? 2 : 1, NR = NT / G;
     const int g = (threadIdx.x & 63) >> 4;
     const int first = GATED ? wb / 2 : wb, end = GATED ? a.w_blocks / 2 : a.w_blocks;
     float y[NR][4];
@@ -290,12 +309,10 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t row, float 
             for (int j = 0; j < 4; j++) y[r][j] = activate(y[r][j], a.gate) * u[j];
         }
     }
-    if constexpr (E::kWide == 8 && NR % 2 == 0) {
+    if constexpr (Added<E, GATED, NT>::kPairs) {
         if (a.wide16) {
             typedef typename E::T T;
-            struct alignas(16) Eight {
-                T v[8];
-            };
+            typedef typename Added<E, GATED, NT>::Eight Eight;
 #pragma unroll
             for (int r = 0; r < NR; r += 2) {
                 float z[8];
@@ -311,8 +328,8 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t row, float 
                 T* out = (T*)a.out + row * a.out_row + c;
                 const T* add = a.add ? (const T*)a.add + row * a.add_row + c : nullptr;
                 if (c + 8 <= a.n) {
-                    Eight o, q{};
-                    if (add) q = *(const Eight*)add;
+                    Eight o;
+                    const Eight& q = added.v[r / 2];
 #pragma unroll
                     for (int j = 0; j < 8; j++) o.v[j] = E::store(add ? z[j] + E::load(q.v[j]) : z[j]);
                     *(Eight*)out = o;
@@ -399,7 +416,9 @@ __global__ __launch_bounds__(WAVES * 64) void product_few_kernel(ProductArgs a) 
             for (int w = 1; w < WAVES; w++) all[g] += joined[w][m * NT + t + g][lane];
         }
         const int64_t row = (rb + m) * 16 + (lane & 15);
-        finish<E, GATED, G>(a, row, a.x_scales[min(row, a.rows - 1)], wb + t, BlockScales<G>(a, wb + t), all);
+        Added<E, GATED, G> added;
+        added.fetch(a, row, wb + t);
+        finish<E, GATED, G>(a, row, a.x_scales[min(row, a.rows - 1)], wb + t, BlockScales<G>(a, wb + t), all, added);
     }
 }
 
@@ -501,8 +520,13 @@ __global__ __launch_bounds__(WM* WN * 64) void product_tile_kernel(
     float row_scales[MT];
 #pragma unroll
     for (int m = 0; m < MT; m++) row_scales[m] = a.x_scales[min(row0 + 16 * m, a.rows - 1)];
+    Added<E, GATED, NT> added[2];
+    added[0].fetch(a, row0, wt * TN + t0);
 #pragma unroll
-    for (int m = 0; m < MT; m++) finish<E, GATED, NT>(a, row0 + 16 * m, row_scales[m], wt * TN + t0, scales, sums[m]);
+    for (int m = 0; m < MT; m++) {
+        if (m + 1 < MT) added[(m + 1) & 1].fetch(a, row0 + 16 * (m + 1), wt * TN + t0);
+        finish<E, GATED, NT>(a, row0 + 16 * m, row_scales[m], wt * TN + t0, scales, sums[m], added[m & 1]);
+    }
 }
 
 template <class E, bool GATED, int WM, int WN, int MT, int NT, int ST>
