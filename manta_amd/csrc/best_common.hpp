@@ -37,8 +37,8 @@ __device__ __forceinline__ int rank_in(const uint64_t* keys, int n, uint64_t min
 // time, the lanes' comparisons counted by ballots.  20 steps of about 4 N
 // instructions on one wave, where every thread ranking its own value among
 // 256 took 1,000 on each (64 rows of 200,000, k = 100: 49 -> 26 us).
-template <int N>
-__device__ __forceinline__ void find_floor(const uint32_t* tops, int k, BestShared& B) {
+template <int N, class Shared>
+__device__ __forceinline__ void find_floor(const uint32_t* tops, int k, Shared& B) {
     if (threadIdx.x >= 64) return;
     uint32_t t[N];
 #pragma unroll

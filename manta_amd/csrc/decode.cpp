@@ -269,7 +269,7 @@ int manta_rocm_beam_select(MantaRocm* rt, MantaRocmBeams* b, int dtype, const vo
     a.logits_row = logits_row;
     a.groups = (int)groups;
     a.beams = (int)beams;
-    a.parts = manta::beam_parts(vocab);
+    a.parts = manta::beam_parts(groups * beams, vocab);
     a.best = (int)best;
     a.vocab = vocab;
     a.scores = scores;

@@ -2,17 +2,24 @@
 //   scores[g, b] + logits[g, b, t] - log(sum over u of exp(logits[g, b, u]))
 // over a group's beams b and the vocabulary t.
 //
-// One launch, and every logit is read once.  A workgroup holds 8,192 of a
-// row's logits in registers: their largest, the sum of exp(x - largest) and
-// the row's `best` largest of them, which is all that the total's order within
-// a row can ask for.  The last workgroup of a group (a ticket) joins the parts
-// of each beam, and takes the best of the beams' candidates.
+// One launch, and every logit is read once.  A workgroup takes a part of a row,
+// 4,096 logits at a time, and a wave its quarter of them in registers (the next
+// ones on their way): it keeps the largest it has seen, the sum of exp(x -
+// largest), and the `best` largest logits, which is all that the total's order
+// within a row can ask for, a lane each in order.  After the first piece few
+// logits reach the last of those, so no wave waits for another before the part
+// is done.  The last workgroup of a group (a ticket) joins the parts of each
+// beam, and takes the best of the beams' candidates.
+//
+// 64 groups of 8 beams of 130001 logits: f32 96 us, 2.8 TB/s, bf16 93; what
+// bounds it are the exponentials, 22 of about 34 vector instructions a logit,
+// which fill two thirds of the SIMDs' cycles.
 //
 // Sums and totals are f64: totals of different beams lie a few 1e-2 apart
 // where `best` of them are taken from a vocabulary, so an error of f32 (1e-7
 // of a sum) would exchange two of them once in 10^5 choices, and this one
-// (1e-15) does not.  A vector instruction of f64 takes as long as one of f32
-// here.
+// (below 1e-11) does not.  A vector instruction of f64 takes as long as one of
+// f32 here.
 #include "best_common.hpp"
 #include "cache_kernels.hpp"
 #include "decode_kernels.hpp"
@@ -23,31 +30,42 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kHeld = kBeamPiece / kThreads;  // logits a thread holds
-constexpr int kFound = 1024;                  // candidates that the last workgroup ranks at once
+constexpr int kAhead = 4;                     // candidates that a thread of it holds
+constexpr int kFound = 512;                   // candidates that the last workgroup ranks at once
 
-// exp(d) for d <= 0 (0 below -708), within 2e-16 of it: d = k ln 2 + r, and the
-// series of exp(r) to r^13 / 13!, |r| <= ln(2) / 2.
-__device__ __forceinline__ double exp_neg(double d) {
-    if (d < -708.0) d = -HUGE_VAL;
-    const double k = rint(d * 1.4426950408889634);
-    double r = fma(k, -0x1.62e42fefa39efp-1, d);  // ln 2 in two parts
-    r = fma(k, -0x1.abc9e3b39803fp-56, r);
-    double p = 1.0 / 6227020800.0;
-    p = fma(p, r, 1.0 / 479001600.0);
-    p = fma(p, r, 1.0 / 39916800.0);
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return d < -708.0 ? 0.0 : ldexp(p, (int)k);
-}
+// exp(d) for -700 <= d <= 0 (NaN stays), within 1e-11 of it: d = k ln 2 + r, |r|
+// <= ln(2) / 2, and the series of exp(r) to r^9 / 9!.  Adding 1.5 * 2^52 rounds
+// to k and leaves it in the low word, and k goes into the exponent by an
+// addition.  The constants stay in scalar registers: as literals each would
+// cost two moves a use.
+struct Exp {
+    double magic = 6755399441055744.0, log2e = 1.4426950408889634, ln2 = -0x1.62e42fefa39efp-1;
+    double c9 = 1.0 / 362880.0, c8 = 1.0 / 40320.0, c7 = 1.0 / 5040.0, c6 = 1.0 / 720.0, c5 = 1.0 / 120.0,
+           c4 = 1.0 / 24.0, c3 = 1.0 / 6.0;
+    __device__ __forceinline__ Exp() {
+        asm("" : "+s"(magic), "+s"(log2e), "+s"(ln2), "+s"(c9), "+s"(c8));
+        asm("" : "+s"(c7), "+s"(c6), "+s"(c5), "+s"(c4), "+s"(c3));
+    }
+    __device__ __forceinline__ double operator()(double d) const {
+        const double t = fma(d, log2e, magic);
+        const double r = fma(t - magic, ln2, d);
+        double p = fma(c9, r, c8);
+        p = fma(p, r, c7);
+        p = fma(p, r, c6);
+        p = fma(p, r, c5);
+        p = fma(p, r, c4);
+        p = fma(p, r, c3);
+        p = fma(p, r, 0.5);
+        p = fma(p, r, 1.0);
+        p = fma(p, r, 1.0);
+        // (a NaN's low word has no bits that reach the exponent)
+        uint32_t hi = (uint32_t)__double2hiint(p);
+        const uint32_t k = (uint32_t)__double2loint(t);
+        asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(hi) : "v"(k));
+        return __hiloint2double((int)hi, __double2loint(p));
+    }
+};
+__device__ __forceinline__ double exp_neg(double d) { return d < -700.0 ? 0.0 : Exp()(d); }
 
 // Order-preserving map of f64 (not NaN, -0 made +0) to u64; 0 is below all.
 __device__ __forceinline__ uint64_t total_order(double t) {
@@ -57,9 +75,6 @@ __device__ __forceinline__ uint64_t total_order(double t) {
 __device__ __forceinline__ double order_total(uint64_t o) {
     return __longlong_as_double((long long)(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o));
 }
-
-// Order of a logit: never 0, every NaN above the numbers.
-__device__ __forceinline__ uint32_t logit_order(float x) { return x != x ? 0xFFC00000u : float_order(x); }
 
 struct Joined {  // of a row or a part: exp(largest) * sum
     double largest, sum;
@@ -86,41 +101,55 @@ __device__ __forceinline__ void store_part(uint64_t* p, uint64_t v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+struct Floor {
+    uint32_t floor;
+};
 struct MergeShared {
     double largest[kMaxBeams], log_sum[kMaxBeams], score[kMaxBeams];
     int ended[kMaxBeams];
     Candidate found[kFound];
     Candidate wave_best[kThreads / 64];
     uint32_t tops[kThreads];
-    uint32_t floor;
+    Floor floor;
     int count;
 };
 
 // The last workgroup of group g: the best totals over its beams' parts.
-__device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShared& M, BestShared& B) {
+__device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShared& M) {
     const int tid = threadIdx.x;
     const int words = (int)beam_part_words(a.best);
     const uint64_t* work = a.work + (int64_t)g * a.beams * a.parts * words;
-    for (int b = tid; b < a.beams; b += kThreads) {
-        const int row = g * a.beams + b;
-        M.score[b] = (double)a.scores[row];
-        M.ended[b] = a.ended && a.ended[row] != 0;
-        if (!M.ended[b]) {
-            Joined j{0.0, 0.0};
-            for (int p = 0; p < a.parts; p++) {
-                const uint64_t* part = work + ((int64_t)b * a.parts + p) * words + a.best;
-                j = join(j, {__longlong_as_double((long long)load_part(part)),
-                             __longlong_as_double((long long)load_part(part + 1))});
-            }
-            M.largest[b] = j.largest;
-            M.log_sum[b] = log(j.sum);
+    const int per = a.parts * a.best;  // candidates of a beam
+    const int n = a.beams * per;
+    // (keys of ended beams are whatever an earlier call left: not looked at)
+    auto key_at = [&](int i) { return load_part(work + (int64_t)(i / a.best) * words + i % a.best); };
+    uint64_t keys[kAhead];  // this thread's first ones, on their way
+#pragma unroll
+    for (int r = 0; r < kAhead; r++) keys[r] = tid + kThreads * r < n ? key_at(tid + kThreads * r) : 0ull;
+    // A wave a beam and a lane a part.
+    for (int b = tid >> 6; b < a.beams; b += kThreads / 64) {
+        const int row = g * a.beams + b, lane = tid & 63;
+        const bool over = a.ended && a.ended[row] != 0;
+        double largest = 0.0, sum = 0.0;
+        if (!over && lane < a.parts) {
+            const uint64_t* part = work + ((int64_t)b * a.parts + lane) * words + a.best;
+            largest = __longlong_as_double((long long)load_part(part));
+            sum = __longlong_as_double((long long)load_part(part + 1));
+        }
+        double most = sum == 0.0 ? -HUGE_VAL : largest;
+        for (int s = 32; s; s >>= 1) most = fmax(most, __shfl_xor(most, s));
+        sum = sum == 0.0 ? 0.0 : sum * exp_neg(largest - most);
+        for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
+        if (lane == 0) {
+            M.score[b] = (double)a.scores[row];
+            M.ended[b] = over;
+            M.largest[b] = most;
+            M.log_sum[b] = log(sum);
         }
     }
     if (tid == 0) M.count = 0;
     __syncthreads();
-    const int per = a.parts * a.best;  // candidates of a beam
-    const int n = a.beams * per;
-    auto candidate = [&](int i) {
+    auto candidate = [&](int i, uint64_t key) {
         const int b = i / per, k = i - b * per;
         Candidate c{0, 0};
         double t;
@@ -129,7 +158,6 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
             t = M.score[b];
             c.place = ((uint64_t)b << 32) | (uint32_t)a.end_token;
         } else {
-            const uint64_t key = load_part(work + ((int64_t)b * a.parts + k / a.best) * words + k % a.best);
             if (!key) return c;
             // (apart: the largest may be a number that swallows the logarithm)
             t = M.score[b] + (((double)key_score(key, 0) - M.largest[b]) - M.log_sum[b]);
@@ -142,19 +170,24 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
     // (compared as f32: narrowing keeps the order) are few and hold the result.
     auto coarse = [](const Candidate& c) { return c.total ? float_order((float)order_total(c.total)) : 0u; };
     uint32_t top = 0;
-    for (int i = tid; i < n; i += kThreads) top = max(top, coarse(candidate(i)));
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < kAhead; r++)
+            if (tid + kThreads * r < n) f(candidate(tid + kThreads * r, keys[r]));
+        for (int i = tid + kThreads * kAhead; i < n; i += kThreads) f(candidate(i, key_at(i)));
+    };
+    each([&](const Candidate& c) { top = max(top, coarse(c)); });
     M.tops[tid] = top;
     __syncthreads();
-    find_floor<4>(M.tops, a.best, B);
+    find_floor<4>(M.tops, a.best, M.floor);
     __syncthreads();
-    const uint32_t floor = B.floor;
-    for (int i = tid; i < n; i += kThreads) {
-        const Candidate c = candidate(i);
+    const uint32_t floor = M.floor.floor;
+    each([&](const Candidate& c) {
         if (c.total && coarse(c) >= floor) {
             const int at = atomicAdd(&M.count, 1);
             if (at < kFound) M.found[at] = c;
         }
-    }
+    });
     __syncthreads();
     const int found = M.count;
     auto put = [&](int k, const Candidate& c) {
@@ -177,10 +210,9 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
     Candidate last{~0ull, 0};
     for (int k = 0; k < a.best; k++) {
         Candidate mine{0, ~0ull};
-        for (int i = tid; i < n; i += kThreads) {
-            const Candidate c = candidate(i);
+        each([&](const Candidate& c) {
             if (c.total && better(last, c) && better(c, mine)) mine = c;
-        }
+        });
         for (int s = 32; s; s >>= 1) {
             const Candidate o{(uint64_t)__shfl_xor((long long)mine.total, s), (uint64_t)__shfl_xor((long long)mine.place, s)};
             if (better(o, mine)) mine = o;
@@ -195,10 +227,126 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
     }
 }
 
+// The largest of a wave's 64 numbers, in every lane (all of them active).
+__device__ __forceinline__ float wave_max(float x) {
+    auto step = [&](float y) { x = fmaxf(x, y); };
+    const int low = (int)0xFF800000u;  // -inf where a shift has no source
+#define MANTA_DPP(ctrl, rows) \
+    step(__uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(low, (int)__float_as_uint(x), ctrl, rows, 0xf, false)))
+    MANTA_DPP(0x111, 0xf);  // row_shr 1, 2, 4, 8: lane 15 of a row has its row's
+    MANTA_DPP(0x112, 0xf);
+    MANTA_DPP(0x114, 0xf);
+    MANTA_DPP(0x118, 0xf);
+    MANTA_DPP(0x142, 0xa);  // row_bcast 15, 31: lane 63 has the wave's
+    MANTA_DPP(0x143, 0xc);
+#undef MANTA_DPP
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
+}
+
+// What a wave has seen: the largest, and a lane's sum of exp(x - largest).
+struct Seen {
+    float top = -__builtin_inff();
+    double sum = 0.0;
+    // Returns the wave's largest of these.
+    template <int N>
+    __device__ __forceinline__ float add(const float (&x)[N], const Exp& exp) {
+        float now = x[0];
+#pragma unroll
+        for (int j = 1; j < N; j++) now = fmaxf(now, x[j]);  // (a NaN shows in the sum)
+        now = wave_max(now);
+        if (now > top) {
+            sum *= exp_neg((double)top - (double)now);
+            top = now;
+        }
+        // (all masked: 0 stands in for -inf, and the sum does not count)
+        const float from = top == -__builtin_inff() ? 0.0f : top, least = from - 600.0f;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const double d = (double)x[j] - (double)from;
+            sum += exp(x[j] < least ? -600.0 : d);  // (1e-261 of the largest for less)
+            // four at a time: sixteen at once do not fit the registers
+            if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        return now;
+    }
+};
+
+// A wave's `best` largest logits: lane i has the key of the i-th (0: none).
+struct Kept {
+    uint64_t key = 0;
+    float tau = -__builtin_inff();  // the last one's logit and token, once there are so many:
+    int tau_token = -1;             // what is to come in lies above it
+
+    // Begin with the lanes' own largest of the first piece, sorted by counting
+    // (and taken out of x): few others are left to come in one by one.
+    template <int N, class Token>
+    __device__ __forceinline__ void start(float (&x)[N], Token token, int best) {
+        const uint32_t lane = threadIdx.x & 63;
+        float high = x[0];
+        int at = 0;
+#pragma unroll
+        for (int j = 1; j < N; j++)
+            if (x[j] > high || !(high == high)) {
+                high = x[j];
+                at = j;
+            }
+        // (lanes without one come last, and apart from each other)
+        const bool none = !(high > -__builtin_inff());
+        int t = 0;
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (j == at) t = token(j);
+        const uint64_t mine = none ? (uint64_t)(63 - lane) : make_key(high, (uint32_t)t, 0);
+        int rank = 0;
+#pragma unroll 8
+        for (int i = 0; i < 64; i++) {
+            const uint64_t one = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(mine >> 32), i) << 32) |
+                                 (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, i);
+            rank += one > mine ? 1 : 0;
+        }
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(uint32_t)mine);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(uint32_t)(mine >> 32));
+        key = hi && (int)lane < best ? ((uint64_t)hi << 32) | lo : 0ull;
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (j == at && !none) x[j] = -__builtin_inff();
+        look(best);
+    }
+    __device__ __forceinline__ void look(int best) {
+        const uint64_t end = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(key >> 32), best - 1) << 32) |
+                             (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, best - 1);
+        if (end) {
+            tau = key_score(end, 0);
+            tau_token = (int)key_index(end);
+        }
+    }
+    template <class Token>
+    __device__ __forceinline__ void offer(float x, Token token, int best) {
+        unsigned long long m = __ballot(x >= tau);
+        if (!m) return;
+        const int t = token();
+        m &= __ballot(x > tau || t < tau_token);
+        while (m) {
+            const int from = __ffsll(m) - 1;
+            m &= m - 1;
+            const uint64_t one =
+                make_key(__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), from)),
+                         (uint32_t)__builtin_amdgcn_readlane(t, from), 0);
+            const int place = __popcll(__ballot(key > one)), lane = threadIdx.x & 63;
+            if (place >= best) continue;
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)key, 0x138, 0xf, 0xf, false);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(key >> 32), 0x138, 0xf, 0xf, false);
+            const uint64_t before = ((uint64_t)hi << 32) | lo;  // the lane before's
+            if (lane >= place) key = lane == place ? one : before;
+        }
+        look(best);
+    }
+};
+
 template <class E>
-__global__ __launch_bounds__(kThreads) void beam_kernel(BeamArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
     typedef typename E::T T;
-    constexpr int V = E::kWide;
+    constexpr int V = E::kWide, LOADS = kHeld / V;
     // Which thread and workgroup takes a logit depends on its place in the row
     // alone, so that rows of equal logits have equal sums to the last bit and
     // their totals tie; rows start anywhere, and the loads are 16 bytes all the
@@ -206,13 +354,14 @@ __global__ __launch_bounds__(kThreads) void beam_kernel(BeamArgs a) {
     struct alignas(sizeof(T)) Pack16 {
         T v[V];
     };
-    __shared__ BestShared B;
-    __shared__ MergeShared M;
-    __shared__ uint64_t kept_keys[kMaxBest];
-    __shared__ uint32_t wave_top[kThreads / 64];
-    __shared__ double wave_sum[kThreads / 64];
+    __shared__ union Shared {
+        BestShared best;
+        MergeShared merge;
+        __device__ Shared() {}
+    } S;
+    __shared__ double wave_largest[kThreads / 64], wave_sum[kThreads / 64];
     __shared__ int last;
-    const int tid = threadIdx.x, part = blockIdx.x, row = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x, row = blockIdx.y;
     const int g = row / a.beams;
     const bool over = a.ended && a.ended[row] != 0;
     uint64_t* dst = a.work + ((int64_t)row * a.parts + part) * beam_part_words(a.best);
@@ -220,70 +369,62 @@ __global__ __launch_bounds__(kThreads) void beam_kernel(BeamArgs a) {
         const T* src = (const T*)a.logits + (int64_t)row * a.logits_row;
         const int64_t end = a.vocab, pieces = (end + kBeamPiece - 1) / kBeamPiece;
         const int64_t p0 = pieces * part / a.parts, p1 = pieces * (part + 1) / a.parts;
-        Joined all{0.0, 0.0};
-        int kept = 0;
-        for (int64_t p = p0; p < p1; p++) {
-            const int64_t v0 = p * kBeamPiece;
-            auto at = [&](int j) { return v0 + ((j / V) * kThreads + tid) * V + j % V; };
-            uint32_t o[kHeld];  // order of a logit; 0 where there is none
+        const int64_t mine = wave * (kBeamPiece / 4);
+        Pack16 held[LOADS];
+        auto fetch = [&](int64_t p) {
 #pragma unroll
-            for (int j = 0; j < kHeld; j += V) {
-                const int64_t v = at(j);
+            for (int l = 0; l < LOADS; l++) {
+                const int64_t v = p * kBeamPiece + mine + (l * 64 + lane) * V;
                 if (v + V <= end) {
-                    const Pack16 x = *(const Pack16*)(src + v);
-#pragma unroll
-                    for (int k = 0; k < V; k++) o[j + k] = logit_order(E::load(x.v[k]));
+                    held[l] = *(const Pack16*)(src + v);
                 } else {
 #pragma unroll
                     for (int k = 0; k < V; k++)
-                        o[j + k] = v + k < end ? logit_order(E::load(src[v + k])) : 0u;
+                        if (v + k < end) held[l].v[k] = src[v + k];
                 }
             }
-            uint32_t top = 0;
+        };
+        const Exp exp;
+        Seen seen;
+        Kept kept;
+        if (p0 < p1) fetch(p0);
+        for (int64_t p = p0; p < p1; p++) {
+            const int first = (int)(p * kBeamPiece + mine) + lane * V;
+            auto at = [&](int j) { return first + (j / V) * 64 * V + j % V; };
+            float x[kHeld];  // (-inf where there is none)
 #pragma unroll
-            for (int j = 0; j < kHeld; j++) top = max(top, o[j]);
-            for (int s = 32; s; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
-            if ((tid & 63) == 0) wave_top[tid >> 6] = top;
-            __syncthreads();
-            for (int w = 0; w < kThreads / 64; w++) top = max(top, wave_top[w]);
-            const double largest = (double)order_float(top);
-            // (all masked: 0 stands in for -inf, and the sum is 0)
-            const double from = largest == -HUGE_VAL ? 0.0 : largest;
-            double sum = 0.0;
+            for (int j = 0; j < kHeld; j++) x[j] = E::load(held[j / V].v[j % V]);
+            if ((p + 1) * kBeamPiece > end) {
 #pragma unroll
-            for (int j = 0; j < kHeld; j++)
-                if (o[j]) sum += exp_neg((double)order_float(o[j]) - from);
-            for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
-            if ((tid & 63) == 0) wave_sum[tid >> 6] = sum;
-            __syncthreads();
-            sum = 0.0;
-            for (int w = 0; w < kThreads / 64; w++) sum += wave_sum[w];
-            all = join(all, {from, sum});
-            // the piece's best, and with those of the pieces before
-            auto token = [&](int j) { return o[j] ? (int)at(j) : -1; };
-            int now = block_best<kHeld>([&](int j) { return o[j]; }, token, kHeld, a.best, B);
-            if (now < 0)
-                now = best_streamed(
-                    [&](int64_t i) {
-                        const int64_t v = v0 + i;
-                        return v < end ? make_key(E::load(src[v]), (uint32_t)v, 0) : 0ull;
-                    },
-                    kBeamPiece, 1ull, a.best, B);
-            if (p > p0) {
-                __syncthreads();
-                for (int i = tid; i < kept; i += kThreads) B.keys[now + i] = kept_keys[i];
-                __syncthreads();
-                now = best_of(now + kept, a.best, B);
+                for (int j = 0; j < kHeld; j++)
+                    if (at(j) >= end) x[j] = -__builtin_inff();
             }
-            kept = now;
-            __syncthreads();
-            if (p + 1 < p1) {
-                for (int i = tid; i < kept; i += kThreads) kept_keys[i] = B.keys[i];
-                __syncthreads();
+            if (p + 1 < p1) fetch(p + 1);
+            const float top = seen.add(x, exp);
+            if (p == p0) kept.start(x, at, a.best);
+            if (top >= kept.tau && top > -__builtin_inff()) {
+#pragma unroll
+                for (int j = 0; j < kHeld; j++)
+                    kept.offer(x[j], [&] { return at(j); }, a.best);
             }
         }
-        for (int i = tid; i < a.best; i += kThreads) store_part(dst + i, i < kept ? B.keys[i] : 0ull);
+        for (int s = 32; s; s >>= 1) seen.sum += __shfl_xor(seen.sum, s);
+        if (lane == 0) {
+            const bool none = seen.top == -__builtin_inff();
+            wave_largest[wave] = none ? 0.0 : (double)seen.top;
+            wave_sum[wave] = none && seen.sum == seen.sum ? 0.0 : seen.sum;
+        }
+        // the waves' lists by rank
+        S.best.keys[tid] = lane < a.best ? kept.key : 0ull;
+        __syncthreads();
+        const uint64_t key = S.best.keys[tid];
+        const int rank = key ? rank_in(S.best.keys, kThreads, key) : a.best;
+        if (rank < a.best) store_part(dst + rank, key);
+        const int live = __syncthreads_count(key != 0);
+        for (int i = live + tid; i < a.best; i += kThreads) store_part(dst + i, 0ull);
         if (tid == 0) {
+            Joined all{0.0, 0.0};
+            for (int w = 0; w < kThreads / 64; w++) all = join(all, {wave_largest[w], wave_sum[w]});
             store_part(dst + a.best, (uint64_t)__double_as_longlong(all.largest));
             store_part(dst + a.best + 1, (uint64_t)__double_as_longlong(all.sum));
         }
@@ -297,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void beam_kernel(BeamArgs a) {
         if (last) __hip_atomic_store(&a.tickets[g], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (last) merge_group(a, g, M, B);
+    if (last) merge_group(a, g, S.merge);
 }
 
 template <class E>
