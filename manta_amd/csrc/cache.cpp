@@ -205,6 +205,7 @@ static int rotary_call(const char* what, MantaRocm* rt, const MantaRocmRotary* r
     manta::RotaryNorms n{};
     for (int64_t i = 0; i < nparts; i++) n.weight[i] = norms[i];
     n.eps = eps;
+    n.inv_dim = 1.0 / (double)head_dim;
     return launch(rt, what, err, [&](hipStream_t s) { return manta::launch_rotary_normed(a, n, s); });
 }
 

@@ -100,64 +100,94 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 // sqrt(mean(x^2) + eps).  `lanes` (a power of two) lanes hold a head, NP
 // pieces each, from its load to its store, so a head is read once and its sum
 // of squares is one exchange among them.  Sums of squares are f64: no number
-// of f32 leaves its range.
+// of f32 leaves its range.  The weights are fetched into LDS once for a
+// workgroup's `tokens`, whose heads it takes as one run, the first ones' data
+// on their way while the angles are worked out.  Bytes bound: 8192 tokens of 40
+// heads of 128, bf16 31 us, 5.4 TB/s (rotary alone 26).
+constexpr int kNormTokens = 8;
 template <class E, int V, bool INTERLEAVED, int NP>
-__global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, RotaryNorms n, int lanes) {
+__global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, RotaryNorms n, int lanes, int tokens) {
     typedef typename E::T T;
-    __shared__ float cs[kMaxHeadDim / 2], sn[kMaxHeadDim / 2];
+    __shared__ alignas(16) float cs[kNormTokens][kMaxHeadDim / 2], sn[kNormTokens][kMaxHeadDim / 2];
+    __shared__ alignas(16) float weight[kRotaryParts][kMaxHeadDim];
     const int half = a.rot >> 1;
     const int turned = half / V;                // pieces of V pairs
     const int rest = (a.head_dim - a.rot) / V;  // pieces of V columns past them
     const int pieces = turned + rest;
     const int per = (a.heads + gridDim.y - 1) / gridDim.y;
-    const int h0 = blockIdx.y * per, h1 = min(a.heads, h0 + per);
+    const int h0 = blockIdx.y * per, heads = min(a.heads, h0 + per) - h0;
+    const int64_t t0 = (int64_t)blockIdx.x * tokens;
+    const int count = (int)min((int64_t)tokens, a.tokens - t0), all = count * heads;
     const int gl = threadIdx.x & (lanes - 1), g0 = threadIdx.x / lanes, step = kThreads / lanes;
-    for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
-        __syncthreads();  // an earlier token's angles have been used
-        const double pos = (double)a.positions[token];
-        for (int p = threadIdx.x; p < half; p += kThreads) {
-            const double t = pos * a.turns[p];
-            const float r = (float)(t - rint(t));
-            float s, c;
-            sincospif(2.0f * r, &s, &c);
-            cs[p] = a.magnitude * c;
-            sn[p] = a.magnitude * s;
+
+    // a head's elements as this lane has them
+    Pack<E, V> lo[NP], hi[NP];
+    T* out = nullptr;
+    int token = 0, part = 0;
+    auto fetch = [&](int i) {
+        token = i / heads;
+        int h = h0 + i - token * heads;
+        // (the parts' fields are picked with constant indices: they stay in
+        // scalar registers, where a lane's own index would read them from memory)
+        part = 0;
+        const T* src = (const T*)a.part[0].x + (t0 + token) * a.part[0].x_token + h * a.part[0].x_head;
+        out = (T*)a.part[0].out + (t0 + token) * a.part[0].out_token + h * a.part[0].out_head;
+#pragma unroll
+        for (int k = 1; k < kRotaryParts; k++) {
+            if (k >= a.parts || h < a.part[k - 1].heads) break;
+            h -= a.part[k - 1].heads;
+            part = k;
+            src = (const T*)a.part[k].x + (t0 + token) * a.part[k].x_token + h * a.part[k].x_head;
+            out = (T*)a.part[k].out + (t0 + token) * a.part[k].out_token + h * a.part[k].out_head;
         }
-        __syncthreads();
-        for (int hb = h0; hb < h1; hb += step) {  // (all lanes stay for the exchange)
-            int h = hb + g0;
-            const bool live = h < h1;
-            int k = 0;
-            if (live)
-                while (h >= a.part[k].heads) h -= a.part[k++].heads;
-            const RotaryPart& q = a.part[k];
-            const float* w = n.weight[k];
-            const T* x = (const T*)q.x + token * q.x_token + h * q.x_head;
-            T* y = (T*)q.out + token * q.out_token + h * q.out_head;
-            Pack<E, V> lo[NP], hi[NP];
-            double sum = 0.0;
 #pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const int piece = gl + lanes * i;
-                lo[i] = Pack<E, V>{};
-                hi[i] = Pack<E, V>{};
-                if (live && piece < turned) {
-                    const int p = piece * V;
-                    lo[i] = *(const Pack<E, V>*)(x + (INTERLEAVED ? 2 * p : p));
-                    hi[i] = *(const Pack<E, V>*)(x + (INTERLEAVED ? 2 * p + V : half + p));
-                } else if (live && piece < pieces) {
-                    lo[i] = *(const Pack<E, V>*)(x + a.rot + (piece - turned) * V);
-                }
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const double u = E::load(lo[i].v[j]), v = E::load(hi[i].v[j]);
-                    sum = fma(u, u, sum);
-                    sum = fma(v, v, sum);
-                }
+        for (int p = 0; p < NP; p++) {
+            const int piece = gl + lanes * p, at = piece * V;
+            if (piece < turned) {
+                lo[p] = *(const Pack<E, V>*)(src + (INTERLEAVED ? 2 * at : at));
+                hi[p] = *(const Pack<E, V>*)(src + (INTERLEAVED ? 2 * at + V : half + at));
+            } else if (piece < pieces) {
+                lo[p] = *(const Pack<E, V>*)(src + a.rot + (piece - turned) * V);
             }
-            for (int s = lanes >> 1; s; s >>= 1) sum += __shfl_xor(sum, s);
-            if (!live) continue;
-            const float r = w ? (float)(1.0 / sqrt(sum / a.head_dim + n.eps)) : 1.0f;
+        }
+    };
+#pragma unroll
+    for (int p = 0; p < NP; p++) lo[p] = hi[p] = Pack<E, V>{};  // (what is not fetched counts as 0)
+    if (g0 < all) fetch(g0);
+    for (int k = 0; k < a.parts; k++)
+        if (n.weight[k])
+            for (int c = threadIdx.x; c < a.head_dim; c += kThreads) weight[k][c] = n.weight[k][c];
+    for (int e = threadIdx.x; e < count * half; e += kThreads) {
+        const int token = e / half, p = e - token * half;
+        const double t = (double)a.positions[t0 + token] * a.turns[p];
+        const float r = (float)(t - rint(t));
+        float s, c;
+        sincospif(2.0f * r, &s, &c);
+        cs[token][p] = a.magnitude * c;
+        sn[token][p] = a.magnitude * s;
+    }
+    __syncthreads();
+    for (int base = 0; base < all; base += step) {  // (all lanes stay for the exchange)
+        const bool live = base + g0 < all;
+        double sum = 0.0;
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const double u = E::load(lo[p].v[j]), v = E::load(hi[p].v[j]);
+                sum = fma(u, u, sum);
+                sum = fma(v, v, sum);
+            }
+        for (int s = lanes >> 1; s; s >>= 1) sum += __shfl_xor(sum, s);
+        bool norm = n.weight[0] != nullptr;
+#pragma unroll
+        for (int k = 1; k < kRotaryParts; k++)
+            if (part == k) norm = n.weight[k] != nullptr;
+        // the hardware's 2^-23 and a step of Newton's, of the error squared
+        const double mean = fma(sum, n.inv_dim, n.eps), r0 = __builtin_amdgcn_rsq(mean);
+        const float r = norm ? (float)fma(0.5 * r0, fma(-mean * r0, r0, 1.0), r0) : 1.0f;
+        const float* w = weight[part];
+        if (live) {
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 const int piece = gl + lanes * i;
@@ -167,8 +197,8 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                     Pack<E, V> o;
 #pragma unroll
                     for (int j = 0; j < V; j++)
-                        o.v[j] = w ? E::store(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
-                    *(Pack<E, V>*)(y + at) = o;
+                        o.v[j] = norm ? E::store(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
+                    *(Pack<E, V>*)(out + at) = o;
                     continue;
                 }
                 const int p = piece * V;
@@ -179,7 +209,7 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                 for (int j = 0; j < V; j++) {
                     u[j] = E::load(lo[i].v[j]);
                     u[V + j] = E::load(hi[i].v[j]);
-                    if (w) {
+                    if (norm) {
                         u[j] = u[j] * r * w[at0 + j];
                         u[V + j] = u[V + j] * r * w[at1 + j];
                     }
@@ -189,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                 for (int j = 0; j < V; j++) {
                     // pair p + j: elements 2j and 2j + 1 of the run, or j of each half
                     const int e1 = INTERLEAVED ? 2 * j : j, e2 = INTERLEAVED ? 2 * j + 1 : V + j;
-                    const float c = cs[p + j], s = sn[p + j];
+                    const float c = cs[token][p + j], s = sn[token][p + j];
                     o[e1] = E::store(u[e1] * c - u[e2] * s);
                     o[e2] = E::store(u[e2] * c + u[e1] * s);
                 }
@@ -199,28 +229,37 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                     ylo.v[j] = o[j];
                     yhi.v[j] = o[V + j];
                 }
-                *(Pack<E, V>*)(y + at0) = ylo;
-                *(Pack<E, V>*)(y + at1) = yhi;
+                *(Pack<E, V>*)(out + at0) = ylo;
+                *(Pack<E, V>*)(out + at1) = yhi;
             }
         }
+        if (base + step + g0 < all) fetch(base + step + g0);
     }
 }
 
 template <class E>
 hipError_t launch_normed(const RotaryArgs& a, const RotaryNorms& n, hipStream_t s) {
-    int split = 1;
-    while (split < 8 && split * 2 <= a.heads && a.tokens * split < 512) split *= 2;
-    const dim3 grid((unsigned)(a.tokens < (1 << 20) ? a.tokens : 1 << 20), split);
     const int v = a.wide ? E::kWide : 1;
     const int pieces = (a.rot / 2 + a.head_dim - a.rot) / v;
     int lanes = 1;
     while (lanes < pieces && lanes < 64) lanes *= 2;  // pieces <= 255, <= 64 when wide
+    // few tokens: a token's heads over several workgroups, so that the card is
+    // full; many: as many a workgroup as give it about five rounds of its
+    // lanes, while there are 1,024 workgroups (8192 x 40 heads of 128: bf16 1
+    // token 39.3 us, 2 33.7, 4 31.3; f32 68.5, 67.1, 73.9; 5001 x 24 of 64, f32:
+    // 22.9, 18.7, 18.1)
+    int split = 1;
+    while (split < 8 && split * 2 <= a.heads && a.tokens * split < 512) split *= 2;
+    int64_t tokens = 1280 / (a.heads * lanes);
+    if (tokens > a.tokens / 1024) tokens = a.tokens / 1024;
+    tokens = tokens < 1 ? 1 : tokens > kNormTokens ? kNormTokens : tokens;
+    const dim3 grid((unsigned)((a.tokens + tokens - 1) / tokens), split);
     if (a.wide) {
-        if (a.interleaved) rotary_normed_kernel<E, E::kWide, true, 1><<<grid, kThreads, 0, s>>>(a, n, lanes);
-        else rotary_normed_kernel<E, E::kWide, false, 1><<<grid, kThreads, 0, s>>>(a, n, lanes);
+        if (a.interleaved) rotary_normed_kernel<E, E::kWide, true, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
+        else rotary_normed_kernel<E, E::kWide, false, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
     } else {
-        if (a.interleaved) rotary_normed_kernel<E, 1, true, 4><<<grid, kThreads, 0, s>>>(a, n, lanes);
-        else rotary_normed_kernel<E, 1, false, 4><<<grid, kThreads, 0, s>>>(a, n, lanes);
+        if (a.interleaved) rotary_normed_kernel<E, 1, true, 4><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
+        else rotary_normed_kernel<E, 1, false, 4><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
     }
     return hipGetLastError();
 }
