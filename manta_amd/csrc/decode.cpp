@@ -5,10 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
-#include <cmath>
-#include <cstring>
 #include <new>
-#include <vector>
 
 #include "decode_kernels.hpp"
 #include "decode_layout.hpp"
@@ -73,39 +70,24 @@ int manta_rocm_weight_bind(MantaRocm* rt, const int8_t* codes, const float* scal
     if (rc) return rc;
     const bool gated = gate != MANTA_ROCM_GATE_NONE;
     const int64_t pitch = manta::product_pitch(width), rows = manta::weight_rows(n, gated);
-    const size_t bytes = (size_t)pitch * (size_t)rows;
-    std::vector<int8_t> laid;
-    std::vector<float> by_row;
+    const size_t bytes = (size_t)pitch * (size_t)rows, tail = (size_t)rows * sizeof(float);
+    const int64_t columns = gated ? 2 * n : n;
     MantaRocmWeight* w = new (std::nothrow) MantaRocmWeight();
     if (!w) return fail(err, MANTA_ROCM_ERROR, "weight_bind: out of memory");
-    try {
-        laid.assign(bytes, 0);
-        by_row.assign((size_t)rows, 0.0f);
-    } catch (const std::bad_alloc&) {
-        return give_up(w, fail(err, MANTA_ROCM_ERROR, "weight_bind: out of memory"));
-    }
-    const int64_t columns = gated ? 2 * n : n;
-    // 16 summed columns of 16 output columns at a time: a run of the block
-    for (int64_t j0 = 0; j0 < columns;) {
-        const int half = j0 >= n;
-        const int64_t c = j0 - half * n;
-        const int64_t j1 = std::min<int64_t>(std::min<int64_t>(j0 - c % 16 + 16, half ? columns : n), columns);
-        const int64_t r = manta::weight_row(c, half, gated);
-        for (int64_t j = j0; j < j1; j++) by_row[(size_t)(r + (j - j0))] = scales[j];
-        for (int64_t k0 = 0; k0 < width; k0 += 16) {
-            const int64_t k1 = std::min<int64_t>(k0 + 16, width);
-            int8_t* run = laid.data() + manta::product_at(pitch, r, k0);
-            for (int64_t k = k0; k < k1; k++) {
-                const int8_t* src = codes + k * columns;
-                for (int64_t j = j0; j < j1; j++) run[(j - j0) * 16 + (k - k0)] = src[j];
-            }
-        }
-        j0 = j1;
-    }
-    const size_t tail = (size_t)rows * sizeof(float);
+    // laid out on the device, from a copy as it came
+    const size_t raw = (size_t)width * (size_t)columns, raw_tail = (size_t)columns * sizeof(float);
+    const size_t raw_scales = (raw + 255) / 256 * 256;
+    void* came = nullptr;
+    const hipStream_t s = (hipStream_t)manta_rt::runtime_stream(rt);
     hipError_t e = hipMalloc(&w->memory, bytes + tail);
-    if (e == hipSuccess) e = hipMemcpy(w->memory, laid.data(), bytes, hipMemcpyHostToDevice);
-    if (e == hipSuccess) e = hipMemcpy((char*)w->memory + bytes, by_row.data(), tail, hipMemcpyHostToDevice);
+    if (e == hipSuccess) e = hipMalloc(&came, raw_scales + raw_tail);
+    if (e == hipSuccess) e = hipMemcpyAsync(came, codes, raw, hipMemcpyHostToDevice, s);
+    if (e == hipSuccess) e = hipMemcpyAsync((char*)came + raw_scales, scales, raw_tail, hipMemcpyHostToDevice, s);
+    if (e == hipSuccess)
+        e = manta::launch_weight_layout((const int8_t*)came, (const float*)((char*)came + raw_scales), width, n, gated,
+                                        (int8_t*)w->memory, (float*)((char*)w->memory + bytes), s);
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    if (came) (void)hipFree(came);
     if (e != hipSuccess)
         return give_up(w, fail(err, MANTA_ROCM_ERROR, "weight_bind: %s (%s)", hipGetErrorName(e), hipGetErrorString(e)));
     w->codes = (int8_t*)w->memory;

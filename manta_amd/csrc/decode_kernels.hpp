@@ -24,6 +24,11 @@ struct QuantizeArgs {
 };
 hipError_t launch_quantize_rows(const QuantizeArgs& a, hipStream_t s);
 
+// codes [width, columns] and their scales as the products read them (columns n,
+// or n and n when gated)
+hipError_t launch_weight_layout(const int8_t* codes, const float* scales, int64_t width, int64_t n, bool gated,
+                                int8_t* out, float* out_scales, hipStream_t s);
+
 struct ProductArgs {
     const int8_t* x;  // quantised rows
     const float* x_scales;

@@ -26,12 +26,8 @@ MANTA_HD int64_t product_rows(int64_t rows) { return (rows + 15) / 16 * 16; }
 MANTA_HD int64_t product_at(int64_t pitch, int64_t r, int64_t c) {
     return ((r >> 4) * (pitch >> 6) + (c >> 6)) * 1024 + ((c & 63) >> 4) * 256 + (r & 15) * 16 + (c & 15);
 }
-// The row of a bound weight that holds output column c: a gated weight's G
-// (half 0) and U (half 1) take turns in blocks of 16, so that a wave has both
-// factors of a result.
-MANTA_HD int64_t weight_row(int64_t c, int half, bool gated) {
-    return gated ? (c >> 4) * 32 + half * 16 + (c & 15) : c;
-}
+// Rows of a bound weight: a gated weight's G and U take turns in blocks of 16,
+// so that a wave has both factors of a result.
 MANTA_HD int64_t weight_rows(int64_t n, bool gated) { return product_rows(n) * (gated ? 2 : 1); }
 
 inline const char* check_weight(int64_t width, int64_t n, int gate) {
@@ -70,10 +66,11 @@ inline const char* check_beams(int64_t groups, int64_t beams, int64_t best) {
 // ---- reorder ----
 constexpr int64_t kMaxReorder = 4096, kMaxReorderGroup = 1024;
 constexpr int kReorderInts = 8192;   // table entries that a workgroup holds
-// columns of the tables that a workgroup takes
+// columns of the tables that a workgroup takes: a power of two
 MANTA_HD int reorder_columns(int64_t group) {
-    const int64_t c = kReorderInts / group;
-    return c >= 256 ? 256 : c >= 128 ? 128 : c >= 64 ? 64 : c >= 32 ? 32 : c >= 16 ? 16 : 8;
+    int c = 64;
+    while (c > 8 && c * group > kReorderInts) c /= 2;
+    return c;
 }
 
 }  // namespace manta

@@ -611,17 +611,18 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(CacheView c, const in
         parent[i] = parents[base + i];
     }
     __syncthreads();
-    const int c0 = blockIdx.x * columns, width = min(columns, c.table_pages - c0);
-    for (int e = tid; e < group * width; e += kThreads)
-        held[e] = c.tables[(int64_t)slot[e / width] * c.table_pages + c0 + e % width];
+    const int shift = __builtin_ctz(columns), col = tid & (columns - 1);
+    const int64_t at = (int64_t)blockIdx.x * columns + col;
+    const bool in = at < c.table_pages;
+    for (int i = tid >> shift; i < group && in; i += kThreads >> shift)
+        held[(i << shift) + col] = c.tables[(int64_t)slot[i] * c.table_pages + at];
     if (blockIdx.x == 0)
         for (int i = tid; i < group; i += kThreads) length[i] = c.lengths[slot[i]];
     __syncthreads();
-    for (int e = tid; e < group * width; e += kThreads) {
-        const int i = e / width, col = e % width, p = parent[i];
-        const int before = held[e], after = p < 0 ? -1 : held[p * width + col];
+    for (int i = tid >> shift; i < group && in; i += kThreads >> shift) {
+        const int p = parent[i], before = held[(i << shift) + col], after = p < 0 ? -1 : held[(p << shift) + col];
         if (before == after) continue;
-        c.tables[(int64_t)slot[i] * c.table_pages + c0 + col] = after;
+        c.tables[(int64_t)slot[i] * c.table_pages + at] = after;
         if ((unsigned)before < (unsigned)c.pages) atomicSub(&c.refs[before], 1);
         if ((unsigned)after < (unsigned)c.pages) atomicAdd(&c.refs[after], 1);
     }

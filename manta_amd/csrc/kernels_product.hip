@@ -219,6 +219,33 @@ hipError_t quantize_of(const QuantizeArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// --------------------------------------------------------- a weight's layout
+
+// A wave lays out blocks: lane l takes 16 of the summed columns of weight row
+// l % 16, whose codes lie a row of `columns` apart (16 lanes read 16 bytes of
+// each; the caches join the rest).
+__global__ __launch_bounds__(kThreads) void weight_layout_kernel(const int8_t* codes, const float* scales, int64_t width,
+                                                                 int64_t n, int gated, int64_t steps, int64_t blocks,
+                                                                 int8_t* out, float* out_scales) {
+    const int lane = threadIdx.x & 63;
+    const int64_t columns = gated ? 2 * n : n, waves = (int64_t)gridDim.x * (kThreads / 64);
+    for (int64_t b = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); b < blocks * steps; b += waves) {
+        // neighbouring waves take neighbouring columns of the same rows
+        const int64_t wb = b % blocks, step = b / blocks;
+        const int64_t r = wb * 16 + (lane & 15);
+        const int64_t c = gated ? (wb >> 1) * 16 + (lane & 15) : r;
+        const int64_t from = gated && (wb & 1) ? n + c : c;
+        const int64_t k0 = step * 64 + (lane >> 4) * 16;
+        uint32_t word[4] = {0, 0, 0, 0};
+        if (c < n)
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                if (k0 + k < width) word[k / 4] |= (uint32_t)(uint8_t)codes[(k0 + k) * columns + from] << (8 * (k % 4));
+        *(uint4*)(out + (wb * steps + step) * 1024 + lane * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+        if (step == 0 && lane < 16) out_scales[r] = c < n ? scales[from] : 0.0f;
+    }
+}
+
 // ----------------------------------------------------------------- product
 
 __device__ __forceinline__ float activate(float v, int gate) {
@@ -599,6 +626,15 @@ hipError_t launch_quantize_rows(const QuantizeArgs& a, hipStream_t s) {
     if (a.dtype == MANTA_ROCM_F32) return norm ? quantize_of<F32, true>(a, s) : quantize_of<F32, false>(a, s);
     if (a.dtype == MANTA_ROCM_F16) return norm ? quantize_of<F16, true>(a, s) : quantize_of<F16, false>(a, s);
     return norm ? quantize_of<Bf16, true>(a, s) : quantize_of<Bf16, false>(a, s);
+}
+
+hipError_t launch_weight_layout(const int8_t* codes, const float* scales, int64_t width, int64_t n, bool gated,
+                                int8_t* out, float* out_scales, hipStream_t s) {
+    const int64_t steps = product_pitch(width) / 64, blocks = weight_rows(n, gated) / 16;
+    const int64_t groups = (steps * blocks + kThreads / 64 - 1) / (kThreads / 64);
+    weight_layout_kernel<<<(unsigned)(groups < 65536 ? groups : 65536), kThreads, 0, s>>>(codes, scales, width, n, gated,
+                                                                                        steps, blocks, out, out_scales);
+    return hipGetLastError();
 }
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t s) {

@@ -244,13 +244,13 @@ hipError_t launch_normed(const RotaryArgs& a, const RotaryNorms& n, hipStream_t 
     int lanes = 1;
     while (lanes < pieces && lanes < 64) lanes *= 2;  // pieces <= 255, <= 64 when wide
     // few tokens: a token's heads over several workgroups, so that the card is
-    // full; many: as many a workgroup as give it about five rounds of its
+    // full; many: as many a workgroup as give it about six rounds of its
     // lanes, while there are 1,024 workgroups (8192 x 40 heads of 128: bf16 1
     // token 39.3 us, 2 33.7, 4 31.3; f32 68.5, 67.1, 73.9; 5001 x 24 of 64, f32:
     // 22.9, 18.7, 18.1)
     int split = 1;
     while (split < 8 && split * 2 <= a.heads && a.tokens * split < 512) split *= 2;
-    int64_t tokens = 1280 / (a.heads * lanes);
+    int64_t tokens = 1536 / (a.heads * lanes);
     if (tokens > a.tokens / 1024) tokens = a.tokens / 1024;
     tokens = tokens < 1 ? 1 : tokens > kNormTokens ? kNormTokens : tokens;
     const dim3 grid((unsigned)((a.tokens + tokens - 1) / tokens), split);
