@@ -104,14 +104,16 @@ void manta_rocm_beams_destroy(MantaRocmBeams* b);
  * that of its logits.  out_scores_dev may be scores_dev where best is beams.
  * ended_dev, when given: int32 [groups, beams]; a beam whose entry is not 0
  * has one continuation, end_token, of total scores[g, b], and its logits are
- * not read.
+ * not read.  out_ended_dev, when given: int32 [groups, best], 1 where the
+ * continuation is end_token, else 0: the next call's ended_dev (which it may
+ * be, where best is beams).
  * A total that is -inf or NaN is no continuation (a masked token; a beam of
  * score -inf; every one of a beam with a NaN or +inf among its logits); where
  * a group has too few, the rest is parent -1, token -1, -inf. */
 int manta_rocm_beam_select(MantaRocm* rt, MantaRocmBeams* b, int dtype, const void* logits_dev, int64_t logits_row,
                            int64_t groups, int64_t beams, int64_t vocab, const float* scores_dev,
                            const int32_t* ended_dev, int64_t end_token, int64_t best, int32_t* out_parents_dev,
-                           int32_t* out_tokens_dev, float* out_scores_dev, char** err);
+                           int32_t* out_tokens_dev, float* out_scores_dev, int32_t* out_ended_dev, char** err);
 
 /* Beams that go on from others: seqs_dev (int32 [n], distinct slots) holds
  * n / group groups, and its entry i takes over what entry parents_dev[i] (0

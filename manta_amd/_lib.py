@@ -229,7 +229,7 @@ SIGNATURES = {
     "manta_rocm_beams_create": (C.c_int, [_p, _i64, _i64, _i64, C.POINTER(_p), _err]),
     "manta_rocm_beams_destroy": (None, [_p]),
     "manta_rocm_beam_select": (
-        C.c_int, [_p, _p, C.c_int, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _err]),
+        C.c_int, [_p, _p, C.c_int, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _err]),
     "manta_rocm_cache_reorder": (C.c_int, [_p, _p, _p, _p, _i64, _i64, _err]),
     "manta_rocm_embed_pooled": (
         C.c_int,

@@ -222,7 +222,7 @@ void manta_rocm_beams_destroy(MantaRocmBeams* b) {
 int manta_rocm_beam_select(MantaRocm* rt, MantaRocmBeams* b, int dtype, const void* logits, int64_t logits_row,
                            int64_t groups, int64_t beams, int64_t vocab, const float* scores, const int32_t* ended,
                            int64_t end_token, int64_t best, int32_t* parents, int32_t* tokens, float* totals,
-                           char** err) {
+                           int32_t* now_ended, char** err) {
     if (!b) return fail(err, MANTA_ROCM_ERROR, "beam_select: nil beams");
     if (!b->rt) return fail(err, MANTA_ROCM_ERROR, "beam_select: the beams' runtime is destroyed");
     if (b->rt != rt) return fail(err, MANTA_ROCM_ERROR, "beam_select: the beams belong to another runtime");
@@ -238,7 +238,7 @@ int manta_rocm_beam_select(MantaRocm* rt, MantaRocmBeams* b, int dtype, const vo
     if (logits_row < 0 || (groups * beams > 1 && logits_row < vocab))
         return fail(err, MANTA_ROCM_ERROR, "beam_select: rows of %lld logits are %lld elements apart", (long long)vocab,
                     (long long)logits_row);
-    if (ended && (end_token < 0 || end_token >= vocab))
+    if ((ended || now_ended) && (end_token < 0 || end_token >= vocab))
         return fail(err, MANTA_ROCM_ERROR, "beam_select: end token %lld of %lld", (long long)end_token, (long long)vocab);
     if (groups > 0 && (!logits || !scores || !parents || !tokens || !totals))
         return fail(err, MANTA_ROCM_ERROR, "beam_select: nil pointer");
@@ -260,6 +260,7 @@ int manta_rocm_beam_select(MantaRocm* rt, MantaRocmBeams* b, int dtype, const vo
     a.parents = parents;
     a.tokens = tokens;
     a.totals = totals;
+    a.now_ended = now_ended;
     a.work = (uint64_t*)b->memory;
     a.tickets = (uint32_t*)((char*)b->memory + b->words * 8);
     a.dtype = dtype;

@@ -59,6 +59,7 @@ struct BeamArgs {
     int32_t* parents;
     int32_t* tokens;
     float* totals;
+    int32_t* now_ended;  // or nullptr
     uint64_t* work;     // [groups * beams][parts][beam_part_words(best)]
     uint32_t* tickets;  // [groups], zero between calls
     int dtype;

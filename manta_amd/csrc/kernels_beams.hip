@@ -195,6 +195,7 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
         a.parents[at] = c.total ? (int)(c.place >> 32) : -1;
         a.tokens[at] = c.total ? (int)(uint32_t)c.place : -1;
         a.totals[at] = c.total ? (float)order_total(c.total) : -__builtin_inff();
+        if (a.now_ended) a.now_ended[at] = c.total && (int)(uint32_t)c.place == a.end_token ? 1 : 0;
     };
     if (found <= kFound) {
         for (int i = tid; i < found; i += kThreads) {
@@ -455,6 +456,7 @@ hipError_t launch_type(const BeamArgs& a, hipStream_t s) {
         p.parents += (int64_t)g0 * a.best;
         p.tokens += (int64_t)g0 * a.best;
         p.totals += (int64_t)g0 * a.best;
+        if (a.now_ended) p.now_ended += (int64_t)g0 * a.best;
         p.work += rows * a.parts * beam_part_words(a.best);
         p.tickets += g0;
         beam_kernel<E><<<dim3(a.parts, p.groups * a.beams), kThreads, 0, s>>>(p);

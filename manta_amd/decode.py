@@ -141,11 +141,12 @@ class Beams:
             pass
 
     def select(self, logits, scores, parents, tokens, totals, ended=None, end_token: int = 0,
-               dtype: Optional[str] = None) -> None:
+               dtype: Optional[str] = None, out_ended=None) -> None:
         """The best continuations: logits [groups, beams, vocab], scores f32
         [groups, beams] (their sums of log probabilities), results [groups,
         best]: parents and tokens int32, totals f32; ended: int32 [groups,
-        beams], not 0 for beams whose only continuation is end_token."""
+        beams], not 0 for beams whose only continuation is end_token;
+        out_ended: the same [groups, best] for the next call."""
         kind = _kind(logits, dtype)
         if len(logits.shape) != 3:
             raise ValueError("logits must be [groups, beams, vocab] (got %s)" % (logits.shape,))
@@ -160,10 +161,12 @@ class Beams:
                                    ("parents", parents, (groups, best), np.int32),
                                    ("tokens", tokens, (groups, best), np.int32),
                                    ("totals", totals, (groups, best), np.float32),
-                                   ("ended", ended, (groups, beams), np.int32)):
+                                   ("ended", ended, (groups, beams), np.int32),
+                                   ("out_ended", out_ended, (groups, best), np.int32)):
             if a is not None and (a.dtype != dt or tuple(a.shape) != shape or a.strides is not None):
                 raise ValueError("%s must be a whole %s array %s (got %s %s)"
                                  % (name, np.dtype(dt).name, shape, a.dtype, a.shape))
         call("manta_rocm_beam_select", self.rt.handle, self.handle, kind, logits.addr,
              vocab if strides is None else strides[1], groups, beams, vocab, scores.addr,
-             None if ended is None else ended.addr, end_token, best, parents.addr, tokens.addr, totals.addr)
+             None if ended is None else ended.addr, end_token, best, parents.addr, tokens.addr, totals.addr,
+             None if out_ended is None else out_ended.addr)

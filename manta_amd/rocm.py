@@ -393,10 +393,13 @@ class Runtime:
         return ids, vals
 
     # ------------------------------------------------------------ embed
-    def gather_rows_f16(self, table: DeviceArray, idx: DeviceArray) -> DeviceArray:
+    def gather_rows_f16(self, table: DeviceArray, idx: DeviceArray, out: Optional[DeviceArray] = None) -> DeviceArray:
         vocab, d = table.shape
         nidx = int(np.prod(idx.shape))
-        out = self.empty((nidx, d), np.uint16)
+        if out is None:
+            out = self.empty((nidx, d), np.uint16)
+        elif tuple(out.shape) != (nidx, d) or out.dtype.itemsize != 2 or out.strides is not None:
+            raise ValueError("gather out must be a whole f16 array (%d, %d) (got %s %s)" % (nidx, d, out.dtype, out.shape))
         call("manta_rocm_gather_rows_f16", self.handle, table.ptr, C.c_int64(vocab), C.c_int64(d),
              idx.ptr, C.c_int64(nidx), out.ptr)
         return out
