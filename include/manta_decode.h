@@ -47,7 +47,7 @@ void manta_rocm_weight_unbind(MantaRocmWeight* w);
  * width rounded up to 128.  They lie in blocks of 16 rows and 64 columns, as
  * the matrix cores take them: the code of (r, c) is byte
  *   ((r / 16) * (pitch / 64) + c / 64) * 1024 + (c % 64) / 16 * 256 + r % 16 * 16 + c % 16.
- * -1 where rows or width is out of range. */
+ * The first starts on 16 bytes.  -1 where rows or width is out of range. */
 int64_t manta_rocm_quantized_bytes(int64_t rows, int64_t width);
 
 /* Quantise rows x [rows, width] (row r at x + r * x_row elements; f32, f16 or

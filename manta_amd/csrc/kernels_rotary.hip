@@ -116,124 +116,126 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
     const int pieces = turned + rest;
     const int per = (a.heads + gridDim.y - 1) / gridDim.y;
     const int h0 = blockIdx.y * per, heads = min(a.heads, h0 + per) - h0;
-    const int64_t t0 = (int64_t)blockIdx.x * tokens;
-    const int count = (int)min((int64_t)tokens, a.tokens - t0), all = count * heads;
     const int gl = threadIdx.x & (lanes - 1), g0 = threadIdx.x / lanes, step = kThreads / lanes;
-
-    // a head's elements as this lane has them
-    Pack<E, V> lo[NP], hi[NP];
-    T* out = nullptr;
-    int token = 0, part = 0;
-    auto fetch = [&](int i) {
-        token = i / heads;
-        int h = h0 + i - token * heads;
-        // (the parts' fields are picked with constant indices: they stay in
-        // scalar registers, where a lane's own index would read them from memory)
-        part = 0;
-        const T* src = (const T*)a.part[0].x + (t0 + token) * a.part[0].x_token + h * a.part[0].x_head;
-        out = (T*)a.part[0].out + (t0 + token) * a.part[0].out_token + h * a.part[0].out_head;
-#pragma unroll
-        for (int k = 1; k < kRotaryParts; k++) {
-            if (k >= a.parts || h < a.part[k - 1].heads) break;
-            h -= a.part[k - 1].heads;
-            part = k;
-            src = (const T*)a.part[k].x + (t0 + token) * a.part[k].x_token + h * a.part[k].x_head;
-            out = (T*)a.part[k].out + (t0 + token) * a.part[k].out_token + h * a.part[k].out_head;
-        }
-#pragma unroll
-        for (int p = 0; p < NP; p++) {
-            const int piece = gl + lanes * p, at = piece * V;
-            if (piece < turned) {
-                lo[p] = *(const Pack<E, V>*)(src + (INTERLEAVED ? 2 * at : at));
-                hi[p] = *(const Pack<E, V>*)(src + (INTERLEAVED ? 2 * at + V : half + at));
-            } else if (piece < pieces) {
-                lo[p] = *(const Pack<E, V>*)(src + a.rot + (piece - turned) * V);
-            }
-        }
-    };
-#pragma unroll
-    for (int p = 0; p < NP; p++) lo[p] = hi[p] = Pack<E, V>{};  // (what is not fetched counts as 0)
-    if (g0 < all) fetch(g0);
     for (int k = 0; k < a.parts; k++)
         if (n.weight[k])
             for (int c = threadIdx.x; c < a.head_dim; c += kThreads) weight[k][c] = n.weight[k][c];
-    for (int e = threadIdx.x; e < count * half; e += kThreads) {
-        const int token = e / half, p = e - token * half;
-        const double t = (double)a.positions[t0 + token] * a.turns[p];
-        const float r = (float)(t - rint(t));
-        float s, c;
-        sincospif(2.0f * r, &s, &c);
-        cs[token][p] = a.magnitude * c;
-        sn[token][p] = a.magnitude * s;
-    }
-    __syncthreads();
-    for (int base = 0; base < all; base += step) {  // (all lanes stay for the exchange)
-        const bool live = base + g0 < all;
-        double sum = 0.0;
+    for (int64_t t0 = (int64_t)blockIdx.x * tokens; t0 < a.tokens; t0 += (int64_t)gridDim.x * tokens) {
+        const int count = (int)min((int64_t)tokens, a.tokens - t0), all = count * heads;
+
+        // a head's elements as this lane has them
+        Pack<E, V> lo[NP], hi[NP];
+        T* out = nullptr;
+        int token = 0, part = 0;
+        auto fetch = [&](int i) {
+            token = i / heads;
+            int h = h0 + i - token * heads;
+            // (the parts' fields are picked with constant indices: they stay in
+            // scalar registers, where a lane's own index would read them from memory)
+            part = 0;
+            const T* src = (const T*)a.part[0].x + (t0 + token) * a.part[0].x_token + h * a.part[0].x_head;
+            out = (T*)a.part[0].out + (t0 + token) * a.part[0].out_token + h * a.part[0].out_head;
 #pragma unroll
-        for (int p = 0; p < NP; p++)
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const double u = E::load(lo[p].v[j]), v = E::load(hi[p].v[j]);
-                sum = fma(u, u, sum);
-                sum = fma(v, v, sum);
+            for (int k = 1; k < kRotaryParts; k++) {
+                if (k >= a.parts || h < a.part[k - 1].heads) break;
+                h -= a.part[k - 1].heads;
+                part = k;
+                src = (const T*)a.part[k].x + (t0 + token) * a.part[k].x_token + h * a.part[k].x_head;
+                out = (T*)a.part[k].out + (t0 + token) * a.part[k].out_token + h * a.part[k].out_head;
             }
-        for (int s = lanes >> 1; s; s >>= 1) sum += __shfl_xor(sum, s);
-        bool norm = n.weight[0] != nullptr;
 #pragma unroll
-        for (int k = 1; k < kRotaryParts; k++)
-            if (part == k) norm = n.weight[k] != nullptr;
-        // the hardware's 2^-23 and a step of Newton's, of the error squared
-        const double mean = fma(sum, n.inv_dim, n.eps), r0 = __builtin_amdgcn_rsq(mean);
-        const float r = norm ? (float)fma(0.5 * r0, fma(-mean * r0, r0, 1.0), r0) : 1.0f;
-        const float* w = weight[part];
-        if (live) {
-#pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const int piece = gl + lanes * i;
-                if (piece >= pieces) continue;
-                if (piece >= turned) {
-                    const int at = a.rot + (piece - turned) * V;
-                    Pack<E, V> o;
-#pragma unroll
-                    for (int j = 0; j < V; j++)
-                        o.v[j] = norm ? E::store(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
-                    *(Pack<E, V>*)(out + at) = o;
-                    continue;
+            for (int p = 0; p < NP; p++) {
+                const int piece = gl + lanes * p, at = piece * V;
+                if (piece < turned) {
+                    lo[p] = *(const Pack<E, V>*)(src + (INTERLEAVED ? 2 * at : at));
+                    hi[p] = *(const Pack<E, V>*)(src + (INTERLEAVED ? 2 * at + V : half + at));
+                } else if (piece < pieces) {
+                    lo[p] = *(const Pack<E, V>*)(src + a.rot + (piece - turned) * V);
                 }
-                const int p = piece * V;
-                // the run of columns that lo holds, and hi
-                const int at0 = INTERLEAVED ? 2 * p : p, at1 = INTERLEAVED ? 2 * p + V : half + p;
-                float u[2 * V];
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    u[j] = E::load(lo[i].v[j]);
-                    u[V + j] = E::load(hi[i].v[j]);
-                    if (norm) {
-                        u[j] = u[j] * r * w[at0 + j];
-                        u[V + j] = u[V + j] * r * w[at1 + j];
-                    }
-                }
-                T o[2 * V];
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    // pair p + j: elements 2j and 2j + 1 of the run, or j of each half
-                    const int e1 = INTERLEAVED ? 2 * j : j, e2 = INTERLEAVED ? 2 * j + 1 : V + j;
-                    const float c = cs[token][p + j], s = sn[token][p + j];
-                    o[e1] = E::store(u[e1] * c - u[e2] * s);
-                    o[e2] = E::store(u[e2] * c + u[e1] * s);
-                }
-                Pack<E, V> ylo, yhi;
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    ylo.v[j] = o[j];
-                    yhi.v[j] = o[V + j];
-                }
-                *(Pack<E, V>*)(out + at0) = ylo;
-                *(Pack<E, V>*)(out + at1) = yhi;
             }
+        };
+#pragma unroll
+        for (int p = 0; p < NP; p++) lo[p] = hi[p] = Pack<E, V>{};  // (what is not fetched counts as 0)
+        if (g0 < all) fetch(g0);
+        for (int e = threadIdx.x; e < count * half; e += kThreads) {
+            const int token = e / half, p = e - token * half;
+            const double t = (double)a.positions[t0 + token] * a.turns[p];
+            const float r = (float)(t - rint(t));
+            float s, c;
+            sincospif(2.0f * r, &s, &c);
+            cs[token][p] = a.magnitude * c;
+            sn[token][p] = a.magnitude * s;
         }
-        if (base + step + g0 < all) fetch(base + step + g0);
+        __syncthreads();
+        for (int base = 0; base < all; base += step) {  // (all lanes stay for the exchange)
+            const bool live = base + g0 < all;
+            double sum = 0.0;
+#pragma unroll
+            for (int p = 0; p < NP; p++)
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const double u = E::load(lo[p].v[j]), v = E::load(hi[p].v[j]);
+                    sum = fma(u, u, sum);
+                    sum = fma(v, v, sum);
+                }
+            for (int s = lanes >> 1; s; s >>= 1) sum += __shfl_xor(sum, s);
+            bool norm = n.weight[0] != nullptr;
+#pragma unroll
+            for (int k = 1; k < kRotaryParts; k++)
+                if (part == k) norm = n.weight[k] != nullptr;
+            // the hardware's 2^-23 and a step of Newton's, of the error squared
+            const double mean = fma(sum, n.inv_dim, n.eps), r0 = __builtin_amdgcn_rsq(mean);
+            const float r = norm ? (float)fma(0.5 * r0, fma(-mean * r0, r0, 1.0), r0) : 1.0f;
+            const float* w = weight[part];
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    const int piece = gl + lanes * i;
+                    if (piece >= pieces) continue;
+                    if (piece >= turned) {
+                        const int at = a.rot + (piece - turned) * V;
+                        Pack<E, V> o;
+#pragma unroll
+                        for (int j = 0; j < V; j++)
+                            o.v[j] = norm ? E::store(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
+                        *(Pack<E, V>*)(out + at) = o;
+                        continue;
+                    }
+                    const int p = piece * V;
+                    // the run of columns that lo holds, and hi
+                    const int at0 = INTERLEAVED ? 2 * p : p, at1 = INTERLEAVED ? 2 * p + V : half + p;
+                    float u[2 * V];
+#pragma unroll
+                    for (int j = 0; j < V; j++) {
+                        u[j] = E::load(lo[i].v[j]);
+                        u[V + j] = E::load(hi[i].v[j]);
+                        if (norm) {
+                            u[j] = u[j] * r * w[at0 + j];
+                            u[V + j] = u[V + j] * r * w[at1 + j];
+                        }
+                    }
+                    T o[2 * V];
+#pragma unroll
+                    for (int j = 0; j < V; j++) {
+                        // pair p + j: elements 2j and 2j + 1 of the run, or j of each half
+                        const int e1 = INTERLEAVED ? 2 * j : j, e2 = INTERLEAVED ? 2 * j + 1 : V + j;
+                        const float c = cs[token][p + j], s = sn[token][p + j];
+                        o[e1] = E::store(u[e1] * c - u[e2] * s);
+                        o[e2] = E::store(u[e2] * c + u[e1] * s);
+                    }
+                    Pack<E, V> ylo, yhi;
+#pragma unroll
+                    for (int j = 0; j < V; j++) {
+                        ylo.v[j] = o[j];
+                        yhi.v[j] = o[V + j];
+                    }
+                    *(Pack<E, V>*)(out + at0) = ylo;
+                    *(Pack<E, V>*)(out + at1) = yhi;
+                }
+            }
+            if (base + step + g0 < all) fetch(base + step + g0);
+        }
+        __syncthreads();  // the angles have been used
     }
 }
 
@@ -253,7 +255,8 @@ hipError_t launch_normed(const RotaryArgs& a, const RotaryNorms& n, hipStream_t 
     int64_t tokens = 1536 / (a.heads * lanes);
     if (tokens > a.tokens / 1024) tokens = a.tokens / 1024;
     tokens = tokens < 1 ? 1 : tokens > kNormTokens ? kNormTokens : tokens;
-    const dim3 grid((unsigned)((a.tokens + tokens - 1) / tokens), split);
+    const int64_t runs = (a.tokens + tokens - 1) / tokens;
+    const dim3 grid((unsigned)(runs < (1 << 20) ? runs : 1 << 20), split);
     if (a.wide) {
         if (a.interleaved) rotary_normed_kernel<E, E::kWide, true, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
         else rotary_normed_kernel<E, E::kWide, false, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
