@@ -1,5 +1,6 @@
 // code_common.hpp -- 8-bit codes of numbers by their largest, shared by the
-// cache's append and the quantised rows.
+// cache's append and the quantised rows; and accesses of 16 bytes at any
+// alignment of their elements.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -8,6 +9,20 @@
 #pragma clang fp contract(off)
 
 namespace manta {
+
+// As one vector: of a struct's elements the compiler makes several accesses.
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+typedef Words4 Words4Any __attribute__((aligned(2)));
+template <class P>
+__device__ __forceinline__ P load16_any(const void* p) {
+    static_assert(sizeof(P) == 16, "16 bytes");
+    return __builtin_bit_cast(P, (Words4)*(const Words4Any*)p);
+}
+template <class P>
+__device__ __forceinline__ void store16_any(void* p, const P& v) {
+    static_assert(sizeof(P) == 16, "16 bytes");
+    *(Words4Any*)p = __builtin_bit_cast(Words4, v);
+}
 
 // Four codes, t[j] / max rounded half to even, the division left out where it
 // cannot matter: t * (1 / max) is within 127 * 3 * 2^-24 < 2^-15 of it (three

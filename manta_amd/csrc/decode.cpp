@@ -12,8 +12,6 @@
 #include "launch_common.hpp"
 #include "runtime_internal.hpp"
 
-using manta_rt::aligned;
-using manta_rt::aligned16;
 using manta_rt::element_size;
 using manta_rt::fail;
 using manta_rt::launch;
@@ -125,6 +123,8 @@ int manta_rocm_quantize_rows(MantaRocm* rt, int dtype, const void* x, int64_t x_
         if (const char* bad = manta::check_eps(eps)) return fail(err, MANTA_ROCM_ERROR, "quantize_rows: %s", bad);
     if (rows > 0 && (!x || !codes || !scales)) return fail(err, MANTA_ROCM_ERROR, "quantize_rows: nil pointer");
     if ((uintptr_t)codes % 16 != 0) return fail(err, MANTA_ROCM_ERROR, "quantize_rows: codes must start on 16 bytes");
+    if ((uintptr_t)x % element_size(dtype) != 0)
+        return fail(err, MANTA_ROCM_ERROR, "quantize_rows: rows are not aligned to their elements");
     int rc = manta_rt::use(rt, err);
     if (rc || rows == 0) return rc;
     manta::QuantizeArgs a{};
@@ -138,7 +138,6 @@ int manta_rocm_quantize_rows(MantaRocm* rt, int dtype, const void* x, int64_t x_
     a.codes = codes;
     a.scales = scales;
     a.dtype = dtype;
-    a.wide = aligned16(x, rows > 1 ? x_row : 0, 0, element_size(dtype));
     return launch(rt, "quantize_rows", err, [&](hipStream_t s) { return manta::launch_quantize_rows(a, s); });
 }
 
@@ -156,6 +155,8 @@ int manta_rocm_matmul_q8(MantaRocm* rt, const MantaRocmWeight* w, const int8_t* 
     if (out_row < 0 || add_row < 0 || (rows > 1 && (out_row < w->n || (add && add_row < w->n))))
         return fail(err, MANTA_ROCM_ERROR, "matmul_q8: rows of %lld columns are %lld and %lld elements apart",
                     (long long)w->n, (long long)out_row, (long long)add_row);
+    if ((uintptr_t)out % element_size(dtype) != 0 || (uintptr_t)add % element_size(dtype) != 0)
+        return fail(err, MANTA_ROCM_ERROR, "matmul_q8: results are not aligned to their elements");
     if (add && w->gate != MANTA_ROCM_GATE_NONE)
         return fail(err, MANTA_ROCM_ERROR, "matmul_q8: nothing is added to a gated product");
     if (add && add == out && rows > 1 && add_row != out_row)
@@ -177,10 +178,6 @@ int manta_rocm_matmul_q8(MantaRocm* rt, const MantaRocmWeight* w, const int8_t* 
     a.w_blocks = (int)(manta::weight_rows(w->n, w->gate != MANTA_ROCM_GATE_NONE) / 16);
     a.dtype = dtype;
     a.gate = w->gate;
-    const int size = element_size(dtype);
-    a.wide = aligned(out, rows > 1 ? out_row : 0, 0, size, 4 * size) &&
-             (!add || aligned(add, rows > 1 ? add_row : 0, 0, size, 4 * size));
-    a.wide16 = aligned16(out, rows > 1 ? out_row : 0, 0, size) && (!add || aligned16(add, rows > 1 ? add_row : 0, 0, size));
     a.cus = manta_rt::runtime_cus(rt);
     return launch(rt, "matmul_q8", err, [&](hipStream_t s) { return manta::launch_product(a, s); });
 }

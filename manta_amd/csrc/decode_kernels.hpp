@@ -20,7 +20,6 @@ struct QuantizeArgs {
     int8_t* codes;
     float* scales;
     int dtype;
-    int wide;  // every row starts on 16 bytes
 };
 hipError_t launch_quantize_rows(const QuantizeArgs& a, hipStream_t s);
 
@@ -42,8 +41,6 @@ struct ProductArgs {
     int steps;        // blocks of 64 summed columns
     int w_blocks;     // blocks of 16 weight rows
     int dtype, gate;
-    int wide;    // four columns of out (and add) are one aligned access
-    int wide16;  // 16 bytes of out (and add) are
     int cus;
 };
 hipError_t launch_product(const ProductArgs& a, hipStream_t s);

@@ -47,11 +47,12 @@ constexpr int kBeamPiece = 4096;  // logits that a workgroup holds at a time
 constexpr int kBeamParts = 64;    // workgroups of a row, at most
 // 64-bit words of a part: its best keys, its largest logit, its sum
 MANTA_HD int64_t beam_part_words(int64_t best) { return best + 2; }
-// Workgroups of a row: 1,024 in all fill the card (4 a compute unit), and past
-// that a longer part finds more of its logits below its best ones so far.
+// Workgroups of a row: 1,024 in all are what the card holds at a time (4 a
+// compute unit), and a longer part finds more of its logits below its best ones
+// so far.
 MANTA_HD int beam_parts(int64_t rows, int64_t vocab) {
     const int64_t pieces = (vocab + kBeamPiece - 1) / kBeamPiece;
-    int64_t parts = (1024 + rows - 1) / rows;
+    int64_t parts = rows < 1024 ? 1024 / rows : 1;
     parts = parts < pieces ? parts : pieces;
     return (int)(parts < kBeamParts ? parts : kBeamParts);
 }

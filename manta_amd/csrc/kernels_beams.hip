@@ -416,10 +416,11 @@ __global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
             wave_sum[wave] = none && seen.sum == seen.sum ? 0.0 : seen.sum;
         }
         // the waves' lists by rank
-        S.best.keys[tid] = lane < a.best ? kept.key : 0ull;
+        if (lane < a.best) S.best.keys[wave * a.best + lane] = kept.key;
         __syncthreads();
-        const uint64_t key = S.best.keys[tid];
-        const int rank = key ? rank_in(S.best.keys, kThreads, key) : a.best;
+        const int listed = kThreads / 64 * a.best;
+        const uint64_t key = tid < listed ? S.best.keys[tid] : 0ull;
+        const int rank = key ? rank_in(S.best.keys, listed, key) : a.best;
         if (rank < a.best) store_part(dst + rank, key);
         const int live = __syncthreads_count(key != 0);
         for (int i = live + tid; i < a.best; i += kThreads) store_part(dst + i, 0ull);

@@ -83,9 +83,10 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantizeArgs a) {
     }
 }
 
-// The same results for rows that start on 16 bytes, each read once: 16 columns
+// The same results for rows of up to 32768 columns, each read once: 16 columns
 // a piece, NP pieces a thread, held in registers from the load until they are
-// coded.  WAVES waves a row; the rows of a block of 16 are taken on one XCD
+// coded.  Rows may start anywhere (16-byte loads take any alignment of their
+// elements).  WAVES waves a row; the rows of a block of 16 are taken on one XCD
 // (workgroup i runs on XCD i % 8), whose L2 joins their 16-byte runs into whole
 // lines.
 template <class E, bool NORM, int WAVES, int NP>
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void quantize_wide_kernel(QuantizeArgs a)
             held[p][l] = Pack16{};
             const int c = c0 + l * V;
             if (!live || c >= a.width) continue;
-            if (c + V <= a.width) held[p][l] = *(const Pack16*)(x + c);
+            if (c + V <= a.width) held[p][l] = load16_any<Pack16>(x + c);
             else {
 #pragma unroll
                 for (int j = 0; j < V; j++)
@@ -130,10 +131,10 @@ __global__ __launch_bounds__(kThreads) void quantize_wide_kernel(QuantizeArgs a)
             for (int e = 0; e < 16; e += 4) {
                 const int c = (tid + 64 * WAVES * p) * 16 + e;
                 if (c + 4 <= a.width) {
-                    struct alignas(4) F4 {
+                    struct alignas(16) F4 {
                         float v[4];
                     };
-                    const F4 f = *(const F4*)(a.norm + c);
+                    const F4 f = load16_any<F4>(a.norm + c);
 #pragma unroll
                     for (int j = 0; j < 4; j++) w[p][NORM ? e + j : 0] = f.v[j];
                 } else {
@@ -205,9 +206,9 @@ template <class E, bool NORM>
 hipError_t quantize_of(const QuantizeArgs& a, hipStream_t s) {
     const int64_t blocks = (a.rows + 127) / 128;
     // a wave a row up to 1024 columns, a workgroup a row up to 32768
-    if (a.wide && a.width <= 1024) {
+    if (a.width <= 1024) {
         quantize_wide_kernel<E, NORM, 1, 1><<<(unsigned)(blocks * 32), kThreads, 0, s>>>(a);
-    } else if (a.wide && a.width <= 32768 && blocks < (1 << 16)) {
+    } else if (a.width <= 32768 && blocks < (1 << 16)) {
         const dim3 grid((unsigned)(blocks * 128));
         if (a.width <= 4096) quantize_wide_kernel<E, NORM, 4, 1><<<grid, kThreads, 0, s>>>(a);
         else if (a.width <= 8192) quantize_wide_kernel<E, NORM, 4, 2><<<grid, kThreads, 0, s>>>(a);
@@ -259,17 +260,16 @@ __device__ __forceinline__ float activate(float v, int gate) {
 template <class E>
 __device__ __forceinline__ void store4(const ProductArgs& a, int64_t row, int c, const float* y) {
     typedef typename E::T T;
-    struct alignas(4 * sizeof(T)) Four {
-        T v[4];
-    };
+    typedef typename E::T Four __attribute__((ext_vector_type(4)));
+    typedef Four FourAny __attribute__((aligned(sizeof(T))));  // (one access at any alignment)
     T* out = (T*)a.out + row * a.out_row + c;
     const T* add = a.add ? (const T*)a.add + row * a.add_row + c : nullptr;
-    if (a.wide && c + 3 < a.n) {
+    if (c + 3 < a.n) {
         Four o, p{};
-        if (add) p = *(const Four*)add;
+        if (add) p = *(const FourAny*)add;
 #pragma unroll
-        for (int j = 0; j < 4; j++) o.v[j] = E::store(add ? y[j] + E::load(p.v[j]) : y[j]);
-        *(Four*)out = o;
+        for (int j = 0; j < 4; j++) o[j] = E::store(add ? y[j] + E::load(p[j]) : y[j]);
+        *(FourAny*)out = o;
         return;
     }
 #pragma unroll
@@ -296,25 +296,28 @@ struct BlockScales {
 };
 
 // The results of NT weight blocks from block wb on for this lane's token
-// (row; stored if it is one).  Where rows allow 16-byte accesses of 16-bit
-// elements, two blocks' halves change places between neighbouring rows of 16
-// lanes, so that a lane has 8 columns in a row and a row of lanes 32 bytes of
-// each token: half as many stores, of whole 64-byte pieces.
+// (row; stored if it is one).  Of 16-bit elements, two blocks' halves change
+// places between neighbouring rows of 16 lanes, so that a lane has 8 columns in
+// a row and a row of lanes 32 bytes of each token: half as many stores, of whole
+// 64-byte pieces where rows are aligned (they need not be).
 template <class E, bool GATED, int NT>
 struct Added {  // what such a lane adds, asked for ahead
     static constexpr int NR = NT / (GATED ? 2 : 1);  // result blocks
     static constexpr bool kPairs = E::kWide == 8 && NR % 2 == 0;
-    struct alignas(16) Eight {
+    struct alignas(8 * sizeof(typename E::T)) Eight {
         typename E::T v[8];
     };
     Eight v[NR / 2 + 1];
     __device__ __forceinline__ void fetch(const ProductArgs& a, int64_t row, int wb) {
-        if (GATED || !kPairs || !a.wide16 || !a.add || row >= a.rows) return;
-        const int g = (threadIdx.x & 63) >> 4;
+        if constexpr (!GATED && kPairs) {
+            if (!a.add || row >= a.rows) return;
+            const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-        for (int r = 0; r + 1 < NR; r += 2) {
-            const int c = (wb + r + (g & 1)) * 16 + (g >> 1) * 8;
-            if (c + 8 <= a.n) v[r / 2] = *(const Eight*)((const typename E::T*)a.add + row * a.add_row + c);
+            for (int r = 0; r + 1 < NR; r += 2) {
+                const int c = (wb + r + (g & 1)) * 16 + (g >> 1) * 8;
+                if (c + 8 <= a.n) 
+                    v[r / 2] = load16_any<Eight>((const typename E::T*)a.add + row * a.add_row + c);
+            }
         }
     }
 };
@@ -337,37 +340,35 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t row, float 
         }
     }
     if constexpr (Added<E, GATED, NT>::kPairs) {
-        if (a.wide16) {
-            typedef typename E::T T;
-            typedef typename Added<E, GATED, NT>::Eight Eight;
+        typedef typename E::T T;
+        typedef typename Added<E, GATED, NT>::Eight Eight;
 #pragma unroll
-            for (int r = 0; r < NR; r += 2) {
-                float z[8];
+        for (int r = 0; r < NR; r += 2) {
+            float z[8];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(y[r][j]), __float_as_uint(y[r + 1][j]),
-                                                                    false, false);
-                    z[j] = __uint_as_float(p[0]);
-                    z[4 + j] = __uint_as_float(p[1]);
-                }
-                const int c = (first + r + (g & 1)) * 16 + (g >> 1) * 8;
-                if (row >= a.rows || first + r + (g & 1) >= end) continue;
-                T* out = (T*)a.out + row * a.out_row + c;
-                const T* add = a.add ? (const T*)a.add + row * a.add_row + c : nullptr;
-                if (c + 8 <= a.n) {
-                    Eight o;
-                    const Eight& q = added.v[r / 2];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) o.v[j] = E::store(add ? z[j] + E::load(q.v[j]) : z[j]);
-                    *(Eight*)out = o;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (c + j < a.n) out[j] = E::store(add ? z[j] + E::load(add[j]) : z[j]);
-                }
+            for (int j = 0; j < 4; j++) {
+                const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(y[r][j]), __float_as_uint(y[r + 1][j]),
+                                                                false, false);
+                z[j] = __uint_as_float(p[0]);
+                z[4 + j] = __uint_as_float(p[1]);
             }
-            return;
+            const int c = (first + r + (g & 1)) * 16 + (g >> 1) * 8;
+            if (row >= a.rows || first + r + (g & 1) >= end) continue;
+            T* out = (T*)a.out + row * a.out_row + c;
+            const T* add = a.add ? (const T*)a.add + row * a.add_row + c : nullptr;
+            if (c + 8 <= a.n) {
+                Eight o;
+                const Eight& q = added.v[r / 2];
+#pragma unroll
+                for (int j = 0; j < 8; j++) o.v[j] = E::store(add ? z[j] + E::load(q.v[j]) : z[j]);
+                store16_any(out, o);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (c + j < a.n) out[j] = E::store(add ? z[j] + E::load(add[j]) : z[j]);
+            }
         }
+        return;
     }
     if (row >= a.rows) return;
 #pragma unroll

@@ -27,10 +27,9 @@ int launch(MantaRocm* rt, const char* what, char** err, F f) {
     return MANTA_ROCM_OK;
 }
 
-inline bool aligned(const void* p, int64_t a, int64_t b, int size, int bytes) {
-    return ((uintptr_t)p % bytes) == 0 && (a * size) % bytes == 0 && (b * size) % bytes == 0;
+inline bool aligned16(const void* p, int64_t a, int64_t b, int size) {
+    return ((uintptr_t)p % 16) == 0 && (a * size) % 16 == 0 && (b * size) % 16 == 0;
 }
-inline bool aligned16(const void* p, int64_t a, int64_t b, int size) { return aligned(p, a, b, size, 16); }
 
 inline int element_size(int dtype) { return dtype == MANTA_ROCM_F32 ? 4 : 2; }
 

@@ -80,7 +80,8 @@ def test_parts_of_rows(lib):
             assert 1 <= n <= min(64, pieces)
             cuts = [pieces * k // n for k in range(n + 1)]  # as the workgroups take them
             assert cuts[0] == 0 and cuts[-1] == pieces and all(a < b for a, b in zip(cuts, cuts[1:]))
-            assert rows * n >= min(1024, rows * min(64, pieces))
+            assert rows * n <= max(1024, rows)
+            assert n == 1 or n == min(64, pieces) or rows * (n + 1) > 1024
 
 
 def test_columns_of_tables(lib):
