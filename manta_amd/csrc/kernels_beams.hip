@@ -22,6 +22,7 @@
 // f32 here.
 #include "best_common.hpp"
 #include "cache_kernels.hpp"
+#include "code_common.hpp"
 #include "decode_kernels.hpp"
 
 namespace manta {
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
     // alone, so that rows of equal logits have equal sums to the last bit and
     // their totals tie; rows start anywhere, and the loads are 16 bytes all the
     // same (memory takes them at any alignment).
-    struct alignas(sizeof(T)) Pack16 {
+    struct alignas(16) Pack16 {
         T v[V];
     };
     __shared__ union Shared {
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
             for (int l = 0; l < LOADS; l++) {
                 const int64_t v = p * kBeamPiece + mine + (l * 64 + lane) * V;
                 if (v + V <= end) {
-                    held[l] = *(const Pack16*)(src + v);
+                    held[l] = load16_any<Pack16>(src + v);
                 } else {
 #pragma unroll
                     for (int k = 0; k < V; k++)

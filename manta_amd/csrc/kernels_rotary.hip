@@ -11,6 +11,7 @@
 // copy reaches 4.75).  The turns are reduced to [-1/2, 1/2] in f64: at position
 // 10^6 an f32 product is off by 0.06 radians, the f64 one by 1e-10.
 #include "cache_kernels.hpp"
+#include "code_common.hpp"
 
 namespace manta {
 
@@ -102,17 +103,22 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 // of squares is one exchange among them.  Sums of squares are f64: no number
 // of f32 leaves its range.  The weights are fetched into LDS once for a
 // workgroup's `tokens`, whose heads it takes as one run, the first ones' data
-// on their way while the angles are worked out.  Bytes bound: 8192 tokens of 40
+// on their way while the angles are worked out.  With PARTS heads may start
+// anywhere and the rotated columns end anywhere: pieces are 16 bytes at any
+// alignment, and the last of the pairs and of the rest can be a part of one.  Bytes bound: 8192 tokens of 40
 // heads of 128, bf16 31 us, 5.4 TB/s (rotary alone 26).
 constexpr int kNormTokens = 8;
-template <class E, int V, bool INTERLEAVED, int NP>
+template <class E, bool INTERLEAVED, bool PARTS, int NP>
 __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, RotaryNorms n, int lanes, int tokens) {
     typedef typename E::T T;
-    __shared__ alignas(16) float cs[kNormTokens][kMaxHeadDim / 2], sn[kNormTokens][kMaxHeadDim / 2];
-    __shared__ alignas(16) float weight[kRotaryParts][kMaxHeadDim];
+    constexpr int V = E::kWide;
+    typedef Pack<E, V> Piece;
+    // (a last piece reads on past what there is, and stores none of it)
+    __shared__ alignas(16) float cs[kNormTokens][kMaxHeadDim / 2 + V], sn[kNormTokens][kMaxHeadDim / 2 + V];
+    __shared__ alignas(16) float weight[kRotaryParts][kMaxHeadDim + 2 * V];
     const int half = a.rot >> 1;
-    const int turned = half / V;                // pieces of V pairs
-    const int rest = (a.head_dim - a.rot) / V;  // pieces of V columns past them
+    const int turned = (half + V - 1) / V;                // pieces of V pairs
+    const int rest = (a.head_dim - a.rot + V - 1) / V;    // pieces of V columns past them
     const int pieces = turned + rest;
     const int per = (a.heads + gridDim.y - 1) / gridDim.y;
     const int h0 = blockIdx.y * per, heads = min(a.heads, h0 + per) - h0;
@@ -124,7 +130,7 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
         const int count = (int)min((int64_t)tokens, a.tokens - t0), all = count * heads;
 
         // a head's elements as this lane has them
-        Pack<E, V> lo[NP], hi[NP];
+        Piece lo[NP], hi[NP];
         T* out = nullptr;
         int token = 0, part = 0;
         auto fetch = [&](int i) {
@@ -147,15 +153,36 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
             for (int p = 0; p < NP; p++) {
                 const int piece = gl + lanes * p, at = piece * V;
                 if (piece < turned) {
-                    lo[p] = *(const Pack<E, V>*)(src + (INTERLEAVED ? 2 * at : at));
-                    hi[p] = *(const Pack<E, V>*)(src + (INTERLEAVED ? 2 * at + V : half + at));
+                    const T *from0 = src + (INTERLEAVED ? 2 * at : at), *from1 = src + (INTERLEAVED ? 2 * at + V : half + at);
+                    if constexpr (!PARTS) {
+                        lo[p] = *(const Piece*)from0;
+                        hi[p] = *(const Piece*)from1;
+                    } else if (at + V <= half) {
+                        lo[p] = load16_any<Piece>(from0);
+                        hi[p] = load16_any<Piece>(from1);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; j++) {
+                            if (INTERLEAVED ? 2 * at + j < a.rot : at + j < half) lo[p].v[j] = from0[j];
+                            if (INTERLEAVED ? 2 * at + V + j < a.rot : at + j < half) hi[p].v[j] = from1[j];
+                        }
+                    }
                 } else if (piece < pieces) {
-                    lo[p] = *(const Pack<E, V>*)(src + a.rot + (piece - turned) * V);
+                    const int c = a.rot + (piece - turned) * V;
+                    if constexpr (!PARTS) {
+                        lo[p] = *(const Piece*)(src + c);
+                    } else if (c + V <= a.head_dim) {
+                        lo[p] = load16_any<Piece>(src + c);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; j++)
+                            if (c + j < a.head_dim) lo[p].v[j] = src[c + j];
+                    }
                 }
             }
         };
 #pragma unroll
-        for (int p = 0; p < NP; p++) lo[p] = hi[p] = Pack<E, V>{};  // (what is not fetched counts as 0)
+        for (int p = 0; p < NP; p++) lo[p] = hi[p] = Piece{};  // (what is not fetched counts as 0)
         if (g0 < all) fetch(g0);
         for (int e = threadIdx.x; e < count * half; e += kThreads) {
             const int token = e / half, p = e - token * half;
@@ -194,11 +221,19 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                     if (piece >= pieces) continue;
                     if (piece >= turned) {
                         const int at = a.rot + (piece - turned) * V;
-                        Pack<E, V> o;
+                        Piece o;
 #pragma unroll
                         for (int j = 0; j < V; j++)
                             o.v[j] = norm ? E::store(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
-                        *(Pack<E, V>*)(out + at) = o;
+                        if constexpr (!PARTS) {
+                            *(Piece*)(out + at) = o;
+                        } else if (at + V <= a.head_dim) {
+                            store16_any(out + at, o);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < V; j++)
+                                if (at + j < a.head_dim) out[at + j] = o.v[j];
+                        }
                         continue;
                     }
                     const int p = piece * V;
@@ -223,14 +258,25 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                         o[e1] = E::store(u[e1] * c - u[e2] * s);
                         o[e2] = E::store(u[e2] * c + u[e1] * s);
                     }
-                    Pack<E, V> ylo, yhi;
+                    Piece ylo, yhi;
 #pragma unroll
                     for (int j = 0; j < V; j++) {
                         ylo.v[j] = o[j];
                         yhi.v[j] = o[V + j];
                     }
-                    *(Pack<E, V>*)(out + at0) = ylo;
-                    *(Pack<E, V>*)(out + at1) = yhi;
+                    if constexpr (!PARTS) {
+                        *(Piece*)(out + at0) = ylo;
+                        *(Piece*)(out + at1) = yhi;
+                    } else if (p + V <= half) {
+                        store16_any(out + at0, ylo);
+                        store16_any(out + at1, yhi);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; j++) {
+                            if (INTERLEAVED ? at0 + j < a.rot : p + j < half) out[at0 + j] = ylo.v[j];
+                            if (INTERLEAVED ? at1 + j < a.rot : p + j < half) out[at1 + j] = yhi.v[j];
+                        }
+                    }
                 }
             }
             if (base + step + g0 < all) fetch(base + step + g0);
@@ -241,10 +287,10 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
 
 template <class E>
 hipError_t launch_normed(const RotaryArgs& a, const RotaryNorms& n, hipStream_t s) {
-    const int v = a.wide ? E::kWide : 1;
-    const int pieces = (a.rot / 2 + a.head_dim - a.rot) / v;
+    constexpr int V = E::kWide;
+    const int pieces = (a.rot / 2 + V - 1) / V + (a.head_dim - a.rot + V - 1) / V;  // 65 at most
     int lanes = 1;
-    while (lanes < pieces && lanes < 64) lanes *= 2;  // pieces <= 255, <= 64 when wide
+    while (lanes < pieces && lanes < 64) lanes *= 2;
     // few tokens: a token's heads over several workgroups, so that the card is
     // full; many: as many a workgroup as give it about six rounds of its
     // lanes, while there are 1,024 workgroups (8192 x 40 heads of 128: bf16 1
@@ -257,12 +303,18 @@ hipError_t launch_normed(const RotaryArgs& a, const RotaryNorms& n, hipStream_t 
     tokens = tokens < 1 ? 1 : tokens > kNormTokens ? kNormTokens : tokens;
     const int64_t runs = (a.tokens + tokens - 1) / tokens;
     const dim3 grid((unsigned)(runs < (1 << 20) ? runs : 1 << 20), split);
-    if (a.wide) {
-        if (a.interleaved) rotary_normed_kernel<E, E::kWide, true, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
-        else rotary_normed_kernel<E, E::kWide, false, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
+    // (with PARTS where there are none: 49.7 us against 42 for 8192 tokens of 40
+    // heads of 128, bf16, out of memory)
+    const int t = (int)tokens;
+    if (a.wide) {  // 64 pieces at most
+        if (a.interleaved) rotary_normed_kernel<E, true, false, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        else rotary_normed_kernel<E, false, false, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+    } else if (pieces <= 64) {
+        if (a.interleaved) rotary_normed_kernel<E, true, true, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        else rotary_normed_kernel<E, false, true, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
     } else {
-        if (a.interleaved) rotary_normed_kernel<E, 1, true, 4><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
-        else rotary_normed_kernel<E, 1, false, 4><<<grid, kThreads, 0, s>>>(a, n, lanes, (int)tokens);
+        if (a.interleaved) rotary_normed_kernel<E, true, true, 2><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        else rotary_normed_kernel<E, false, true, 2><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
     }
     return hipGetLastError();
 }
