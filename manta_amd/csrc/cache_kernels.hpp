@@ -34,6 +34,7 @@ hipError_t launch_rotary(const RotaryArgs& a, hipStream_t s);
 struct RotaryNorms {
     const float* weight[kRotaryParts];  // [head_dim] each, or nullptr: not normed
     double eps, inv_dim;  // 1 / head_dim
+    int past;  // write past the caches (the launcher's)
 };
 hipError_t launch_rotary_normed(const RotaryArgs& a, const RotaryNorms& n, hipStream_t s);
 

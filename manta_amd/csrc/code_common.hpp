@@ -23,6 +23,12 @@ __device__ __forceinline__ void store16_any(void* p, const P& v) {
     static_assert(sizeof(P) == 16, "16 bytes");
     *(Words4Any*)p = __builtin_bit_cast(Words4, v);
 }
+// Of data that is too large to be found in a cache afterwards.
+template <class P>
+__device__ __forceinline__ void store16_past(void* p, const P& v) {
+    static_assert(sizeof(P) == 16, "16 bytes");
+    __builtin_nontemporal_store(__builtin_bit_cast(Words4, v), (Words4Any*)p);
+}
 
 // Four codes, t[j] / max rounded half to even, the division left out where it
 // cannot matter: t * (1 / max) is within 127 * 3 * 2^-24 < 2^-15 of it (three

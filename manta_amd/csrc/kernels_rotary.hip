@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 // on their way while the angles are worked out.  With PARTS heads may start
 // anywhere and the rotated columns end anywhere: pieces are 16 bytes at any
 // alignment, and the last of the pairs and of the rest can be a part of one.  Bytes bound: 8192 tokens of 40
-// heads of 128, bf16 31 us, 5.4 TB/s (rotary alone 26).
+// heads of 128, bf16, out of memory: 29 to 35 us, 4.8 to 5.7 TB/s.
 constexpr int kNormTokens = 8;
 template <class E, bool INTERLEAVED, bool PARTS, int NP>
 __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, RotaryNorms n, int lanes, int tokens) {
@@ -123,6 +123,10 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
     const int per = (a.heads + gridDim.y - 1) / gridDim.y;
     const int h0 = blockIdx.y * per, heads = min(a.heads, h0 + per) - h0;
     const int gl = threadIdx.x & (lanes - 1), g0 = threadIdx.x / lanes, step = kThreads / lanes;
+    auto put = [&](T* p, Piece v) {
+        if (n.past) store16_past(p, v);
+        else *(Piece*)p = v;
+    };
     for (int k = 0; k < a.parts; k++)
         if (n.weight[k])
             for (int c = threadIdx.x; c < a.head_dim; c += kThreads) weight[k][c] = n.weight[k][c];
@@ -226,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                         for (int j = 0; j < V; j++)
                             o.v[j] = norm ? E::store(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
                         if constexpr (!PARTS) {
-                            *(Piece*)(out + at) = o;
+                            put(out + at, o);
                         } else if (at + V <= a.head_dim) {
                             store16_any(out + at, o);
                         } else {
@@ -265,8 +269,8 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                         yhi.v[j] = o[V + j];
                     }
                     if constexpr (!PARTS) {
-                        *(Piece*)(out + at0) = ylo;
-                        *(Piece*)(out + at1) = yhi;
+                        put(out + at0, ylo);
+                        put(out + at1, yhi);
                     } else if (p + V <= half) {
                         store16_any(out + at0, ylo);
                         store16_any(out + at1, yhi);
@@ -286,7 +290,12 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
 }
 
 template <class E>
-hipError_t launch_normed(const RotaryArgs& a, const RotaryNorms& n, hipStream_t s) {
+hipError_t launch_normed(const RotaryArgs& a, RotaryNorms n, hipStream_t s) {
+    // results past the 32 MB of the L2s are not found there by what reads them
+    // next: written past them, they leave the room to what is being read
+    // (8192 x 40 heads of 128, bf16, out of memory and back: 42 us, 35 so; with
+    // a rotary that reads it 73, 70)
+    n.past = a.tokens * a.heads * a.head_dim * (int64_t)sizeof(typename E::T) > ((int64_t)32 << 20);
     constexpr int V = E::kWide;
     const int pieces = (a.rot / 2 + V - 1) / V + (a.head_dim - a.rot + V - 1) / V;  // 65 at most
     int lanes = 1;
