@@ -11,7 +11,7 @@
 // is done.  The last workgroup of a group (a ticket) joins the parts of each
 // beam, and takes the best of the beams' candidates.
 //
-// 64 groups of 8 beams of 130001 logits: f32 96 us, 2.8 TB/s, bf16 93; what
+// 64 groups of 8 beams of 130001 logits: f32 90 us, 3.0 TB/s, bf16 85; what
 // bounds it are the exponentials, 22 of about 34 vector instructions a logit,
 // which fill two thirds of the SIMDs' cycles.
 //
@@ -20,6 +20,8 @@
 // of a sum) would exchange two of them once in 10^5 choices, and this one
 // (below 1e-11) does not.  A vector instruction of f64 takes as long as one of
 // f32 here.
+#include <type_traits>
+
 #include "best_common.hpp"
 #include "cache_kernels.hpp"
 #include "code_common.hpp"
@@ -77,15 +79,51 @@ __device__ __forceinline__ double order_total(uint64_t o) {
     return __longlong_as_double((long long)(o >> 63 ? o & 0x7FFFFFFFFFFFFFFFull : ~o));
 }
 
-struct Joined {  // of a row or a part: exp(largest) * sum
-    double largest, sum;
-};
-// Both may be empty (sum 0); a NaN in either stays.
-__device__ __forceinline__ Joined join(Joined a, Joined b) {
-    if (b.sum == 0.0) return a;
-    if (a.sum == 0.0) return b;
-    const double m = fmax(a.largest, b.largest);
-    return {m, a.sum * exp_neg(a.largest - m) + b.sum * exp_neg(b.largest - m)};
+// Sums and maxima over a wave's 64 lanes, all of them active, in every lane:
+// row shifts by 1, 2, 4 and 8, after which lane 15 of a row has its row's, and
+// two broadcasts, after which lane 63 has the wave's.  A lane whose source lies
+// outside takes `none`.  (A tenth of the cycles of exchanges through LDS.)
+template <class F>
+__device__ __forceinline__ void wave_steps(F step) {
+    step(std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xf>());
+    step(std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xf>());
+    step(std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xf>());
+    step(std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xf>());
+    step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());
+    step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());
+}
+__device__ __forceinline__ float wave_max(float x) {
+    const int none = (int)0xFF800000u;  // -inf
+    wave_steps([&](auto ctrl, auto rows) {
+        x = fmaxf(x, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(none, (int)__float_as_uint(x), ctrl(), rows(),
+                                                                           0xf, false)));
+    });
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
+}
+template <class Op>
+__device__ __forceinline__ double wave_join(double x, double none, Op op) {
+    const int nlo = __double2loint(none), nhi = __double2hiint(none);
+    wave_steps([&](auto ctrl, auto rows) {
+        const int lo = __builtin_amdgcn_update_dpp(nlo, __double2loint(x), ctrl(), rows(), 0xf, false);
+        const int hi = __builtin_amdgcn_update_dpp(nhi, __double2hiint(x), ctrl(), rows(), 0xf, false);
+        x = op(x, __hiloint2double(hi, lo));
+    });
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), 63), __builtin_amdgcn_readlane(__double2loint(x), 63));
+}
+__device__ __forceinline__ double wave_sum(double x) {
+    return wave_join(x, 0.0, [](double a, double b) { return a + b; });
+}
+__device__ __forceinline__ double wave_max(double x) {
+    return wave_join(x, -HUGE_VAL, [](double a, double b) { return fmax(a, b); });
+}
+
+// A wave's lanes' shares exp(largest) * sum of one total (sum 0: none; a NaN in
+// any stays), joined: *largest and the sum, in every lane.
+__device__ __forceinline__ double joined(double sum, double* largest) {
+    const double most = wave_max(sum == 0.0 ? -HUGE_VAL : *largest);
+    sum = sum == 0.0 ? 0.0 : sum * exp_neg(*largest - most);
+    *largest = most;
+    return wave_sum(sum);
 }
 
 struct Candidate {
@@ -137,14 +175,11 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
             largest = __longlong_as_double((long long)load_part(part));
             sum = __longlong_as_double((long long)load_part(part + 1));
         }
-        double most = sum == 0.0 ? -HUGE_VAL : largest;
-        for (int s = 32; s; s >>= 1) most = fmax(most, __shfl_xor(most, s));
-        sum = sum == 0.0 ? 0.0 : sum * exp_neg(largest - most);
-        for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
+        sum = joined(sum, &largest);
         if (lane == 0) {
             M.score[b] = (double)a.scores[row];
             M.ended[b] = over;
-            M.largest[b] = most;
+            M.largest[b] = largest;
             M.log_sum[b] = log(sum);
         }
     }
@@ -229,22 +264,6 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
     }
 }
 
-// The largest of a wave's 64 numbers, in every lane (all of them active).
-__device__ __forceinline__ float wave_max(float x) {
-    auto step = [&](float y) { x = fmaxf(x, y); };
-    const int low = (int)0xFF800000u;  // -inf where a shift has no source
-#define MANTA_DPP(ctrl, rows) \
-    step(__uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(low, (int)__float_as_uint(x), ctrl, rows, 0xf, false)))
-    MANTA_DPP(0x111, 0xf);  // row_shr 1, 2, 4, 8: lane 15 of a row has its row's
-    MANTA_DPP(0x112, 0xf);
-    MANTA_DPP(0x114, 0xf);
-    MANTA_DPP(0x118, 0xf);
-    MANTA_DPP(0x142, 0xa);  // row_bcast 15, 31: lane 63 has the wave's
-    MANTA_DPP(0x143, 0xc);
-#undef MANTA_DPP
-    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
-}
-
 // What a wave has seen: the largest, and a lane's sum of exp(x - largest).
 struct Seen {
     float top = -__builtin_inff();
@@ -282,7 +301,7 @@ struct Kept {
     // Begin with the lanes' own largest of the first piece, sorted by counting
     // (and taken out of x): few others are left to come in one by one.
     template <int N, class Token>
-    __device__ __forceinline__ void start(float (&x)[N], Token token, int best) {
+    __device__ __forceinline__ void start(float (&x)[N], Token token, int best, uint64_t* room) {
         const uint32_t lane = threadIdx.x & 63;
         float high = x[0];
         int at = 0;
@@ -299,13 +318,10 @@ struct Kept {
         for (int j = 0; j < N; j++)
             if (j == at) t = token(j);
         const uint64_t mine = none ? (uint64_t)(63 - lane) : make_key(high, (uint32_t)t, 0);
-        int rank = 0;
-#pragma unroll 8
-        for (int i = 0; i < 64; i++) {
-            const uint64_t one = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(mine >> 32), i) << 32) |
-                                 (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, i);
-            rank += one > mine ? 1 : 0;
-        }
+        room[lane] = mine;  // (the wave's own 64: its accesses are in order)
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int rank = rank_in(room, 64, mine);
         const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(uint32_t)mine);
         const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_permute(rank * 4, (int)(uint32_t)(mine >> 32));
         key = hi && (int)lane < best ? ((uint64_t)hi << 32) | lo : 0ull;
@@ -361,7 +377,7 @@ __global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
         MergeShared merge;
         __device__ Shared() {}
     } S;
-    __shared__ double wave_largest[kThreads / 64], wave_sum[kThreads / 64];
+    __shared__ double tops[kThreads / 64], sums[kThreads / 64];
     __shared__ int last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x, row = blockIdx.y;
     const int g = row / a.beams;
@@ -403,20 +419,21 @@ __global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
             }
             if (p + 1 < p1) fetch(p + 1);
             const float top = seen.add(x, exp);
-            if (p == p0) kept.start(x, at, a.best);
+            if (p == p0) kept.start(x, at, a.best, S.best.keys + wave * 64);
             if (top >= kept.tau && top > -__builtin_inff()) {
 #pragma unroll
                 for (int j = 0; j < kHeld; j++)
                     kept.offer(x[j], [&] { return at(j); }, a.best);
             }
         }
-        for (int s = 32; s; s >>= 1) seen.sum += __shfl_xor(seen.sum, s);
+        const double sum = wave_sum(seen.sum);
         if (lane == 0) {
             const bool none = seen.top == -__builtin_inff();
-            wave_largest[wave] = none ? 0.0 : (double)seen.top;
-            wave_sum[wave] = none && seen.sum == seen.sum ? 0.0 : seen.sum;
+            tops[wave] = none ? 0.0 : (double)seen.top;
+            sums[wave] = none && sum == sum ? 0.0 : sum;
         }
         // the waves' lists by rank
+        __syncthreads();  // (the lists take the room where the first pieces were ranked)
         if (lane < a.best) S.best.keys[wave * a.best + lane] = kept.key;
         __syncthreads();
         const int listed = kThreads / 64 * a.best;
@@ -425,11 +442,13 @@ __global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
         if (rank < a.best) store_part(dst + rank, key);
         const int live = __syncthreads_count(key != 0);
         for (int i = live + tid; i < a.best; i += kThreads) store_part(dst + i, 0ull);
-        if (tid == 0) {
-            Joined all{0.0, 0.0};
-            for (int w = 0; w < kThreads / 64; w++) all = join(all, {wave_largest[w], wave_sum[w]});
-            store_part(dst + a.best, (uint64_t)__double_as_longlong(all.largest));
-            store_part(dst + a.best + 1, (uint64_t)__double_as_longlong(all.sum));
+        if (wave == kThreads / 64 - 1) {
+            double largest = lane < kThreads / 64 ? tops[lane] : 0.0;
+            const double all = joined(lane < kThreads / 64 ? sums[lane] : 0.0, &largest);
+            if (lane == 0) {
+                store_part(dst + a.best, (uint64_t)__double_as_longlong(largest));
+                store_part(dst + a.best + 1, (uint64_t)__double_as_longlong(all));
+            }
         }
     }
     // Publication: agent-scope stores, retired before the ticket.
