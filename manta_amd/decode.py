@@ -19,6 +19,7 @@ from . import _lib
 from ._lib import call, load
 from .cache import _kind
 
+_F32 = np.dtype(np.float32)
 _EMPTY = {"f32": np.float32, "f16": np.uint16, "bf16": np.uint16}
 
 
@@ -82,13 +83,18 @@ def _matrix(name: str, a, rows: Optional[int] = None, columns: Optional[int] = N
         raise ValueError("%s must be [%s, %s] (got %s)" % (name, "rows" if rows is None else rows,
                                                            "columns" if columns is None else columns, a.shape))
     strides = a.strides
-    return a.addr, a.shape[0], a.shape[1], a.shape[1] if strides is None else strides[0]
+    r, c = a.shape
+    return a.addr, r, c, c if strides is None else strides[0]
+
+
+def _f32_row(a, width: int) -> bool:
+    return (a.dtype is _F32 or a.dtype == _F32) and a.shape == (width,) and (a.strides is None or a.strides == (1,))
 
 
 def quantize_rows(rt, x, out, norm, eps: float, dtype: Optional[str]):
     kind = _kind(x, dtype)
     addr, rows, width, stride = _matrix("x", x)
-    if norm is not None and (norm.dtype != np.float32 or tuple(norm.shape) != (width,) or norm.strides not in (None, (1,))):
+    if norm is not None and not _f32_row(norm, width):
         raise ValueError("norm must be f32 [%d] (got %s %s)" % (width, norm.dtype, norm.shape))
     if out is None:
         out = Quantized(rt, rows, width)

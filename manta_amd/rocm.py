@@ -14,7 +14,7 @@ from typing import Optional
 
 import numpy as np
 
-from . import _lib
+from . import _lib, cache, decode
 from ._lib import call, load
 
 DTYPES = {np.dtype(np.float32), np.dtype(np.uint16), np.dtype(np.int8), np.dtype(np.uint8),
@@ -191,8 +191,6 @@ class Runtime:
     def rotary_bind(self, freqs, layout: str = "half", magnitude: float = 1.0):
         """Frequencies (radians a token, one a pair; rotary_freqs) as rotary
         takes them; layout "half" or "interleaved"."""
-        from . import cache
-
         return cache.Rotary(self, freqs, layout, magnitude)
 
     def rotary(self, rot, positions: DeviceArray, parts, inverse: bool = False, dtype: Optional[str] = None) -> None:
@@ -200,23 +198,17 @@ class Runtime:
         head_dim] (out may be x), by the tokens' positions (int32);
         inverse=True is the gradient.  dtype "f32", "f16" or "bf16" (by default
         the array's; 16-bit arrays are f16)."""
-        from . import cache
-
         cache.rotary(self, rot, positions, parts, inverse, dtype)
 
     def rotary_normed(self, rot, positions: DeviceArray, parts, norms, eps: float = 1e-6,
                       dtype: Optional[str] = None) -> None:
         """rotary of tensors whose heads are RMS normed first: norms[i], f32
         [head_dim] (None: not normed), belongs to parts[i]."""
-        from . import cache
-
         cache.rotary_normed(self, rot, positions, parts, norms, eps, dtype)
 
     def cache(self, pages: int, kv_heads: int, head_dim: int, seqs: int, table_pages: int, page_tokens: int = 64,
               layers: int = 1):
         """An empty 8-bit key/value cache of pages (cache.Cache)."""
-        from . import cache
-
         return cache.Cache(self, layers, pages, page_tokens, kv_heads, head_dim, seqs, table_pages)
 
     # ------------------------------------------- products in 8 bits, beams
@@ -224,36 +216,26 @@ class Runtime:
         """A weight of int8 codes [width, n] with an f32 scale a column, as
         matmul_q8 takes it; gate "silu" or "gelu": [width, 2 n], the columns of
         the gate first."""
-        from . import decode
-
         return decode.Weight(self, codes, scales, gate)
 
     def quantized(self, rows: int, width: int):
         """Memory for rows in 8 bits (decode.Quantized)."""
-        from . import decode
-
         return decode.Quantized(self, rows, width)
 
     def quantize_rows(self, x: DeviceArray, out=None, norm: Optional[DeviceArray] = None, eps: float = 1e-6,
                       dtype: Optional[str] = None):
         """x [rows, width] in 8 bits with a scale a row, after an RMS norm when
         its weights (f32 [width]) are given.  Returns out."""
-        from . import decode
-
         return decode.quantize_rows(self, x, out, norm, eps, dtype)
 
     def matmul_q8(self, weight, x, out: Optional[DeviceArray] = None, add: Optional[DeviceArray] = None,
                   dtype: Optional[str] = None) -> DeviceArray:
         """Quantised rows times a weight (plus add), [rows, n] of dtype (that
         of out; "f16" without one).  Returns out."""
-        from . import decode
-
         return decode.matmul_q8(self, weight, x, out, add, dtype)
 
     def beams(self, groups: int, beams: int, best: int):
         """The choice of the next beams, for up to so many (decode.Beams)."""
-        from . import decode
-
         return decode.Beams(self, groups, beams, best)
 
     # ------------------------------------------------------------ binding
