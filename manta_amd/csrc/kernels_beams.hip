@@ -11,14 +11,14 @@
 // is done.  The last workgroup of a group (a ticket) joins the parts of each
 // beam, and takes the best of the beams' candidates.
 //
-// 64 groups of 8 beams of 130001 logits: f32 90 us, 3.0 TB/s, bf16 85; what
-// bounds it are the exponentials, 22 of about 34 vector instructions a logit,
-// which fill two thirds of the SIMDs' cycles.
+// 64 groups of 8 beams of 130001 logits: f32 73 us, 3.7 TB/s, bf16 69; what
+// bounds it are the exponentials, 16 of about 30 vector instructions a logit,
+// which fill two thirds of the SIMDs' cycles (with 22 of them, to 1e-11, 90).
 //
 // Sums and totals are f64: totals of different beams lie a few 1e-2 apart
 // where `best` of them are taken from a vocabulary, so an error of f32 (1e-7
 // of a sum) would exchange two of them once in 10^5 choices, and this one
-// (below 1e-11) does not.  A vector instruction of f64 takes as long as one of
+// (below 1e-10) does not.  A vector instruction of f64 takes as long as one of
 // f32 here.
 #include <type_traits>
 
@@ -36,25 +36,25 @@ constexpr int kHeld = kBeamPiece / kThreads;  // logits a thread holds
 constexpr int kAhead = 4;                     // candidates that a thread of it holds
 constexpr int kFound = 512;                   // candidates that the last workgroup ranks at once
 
-// exp(d) for -700 <= d <= 0 (NaN stays), within 1e-11 of it: d = k ln 2 + r, |r|
-// <= ln(2) / 2, and the series of exp(r) to r^9 / 9!.  Adding 1.5 * 2^52 rounds
-// to k and leaves it in the low word, and k goes into the exponent by an
-// addition.  The constants stay in scalar registers: as literals each would
-// cost two moves a use.
+// exp(d) for -700 <= d <= 0 (NaN stays), within 1e-10 of it: d = k ln 2 + r, |r|
+// <= ln(2) / 2, and exp(r) as 1 + r + r^2 / 2 + r^3 times a polynomial of degree
+// 4, whose coefficients make the largest relative error over that range the
+// least (reweighted least squares; 9.6e-11.  The series to r^9 / 9! has 7e-12
+// and two steps more).  Adding 1.5 * 2^52 rounds to k and leaves it in the low
+// word, and k goes into the exponent by an addition.  The constants stay in
+// scalar registers: as literals each would cost two moves a use.
 struct Exp {
     double magic = 6755399441055744.0, log2e = 1.4426950408889634, ln2 = -0x1.62e42fefa39efp-1;
-    double c9 = 1.0 / 362880.0, c8 = 1.0 / 40320.0, c7 = 1.0 / 5040.0, c6 = 1.0 / 720.0, c5 = 1.0 / 120.0,
-           c4 = 1.0 / 24.0, c3 = 1.0 / 6.0;
+    double c7 = 0.0001973345940007819, c6 = 0.0013935234389446138, c5 = 0.008333586300566968,
+           c4 = 0.041666461302453994, c3 = 0.1666666558083848;
     __device__ __forceinline__ Exp() {
-        asm("" : "+s"(magic), "+s"(log2e), "+s"(ln2), "+s"(c9), "+s"(c8));
+        asm("" : "+s"(magic), "+s"(log2e), "+s"(ln2));
         asm("" : "+s"(c7), "+s"(c6), "+s"(c5), "+s"(c4), "+s"(c3));
     }
     __device__ __forceinline__ double operator()(double d) const {
         const double t = fma(d, log2e, magic);
         const double r = fma(t - magic, ln2, d);
-        double p = fma(c9, r, c8);
-        p = fma(p, r, c7);
-        p = fma(p, r, c6);
+        double p = fma(c7, r, c6);
         p = fma(p, r, c5);
         p = fma(p, r, c4);
         p = fma(p, r, c3);
@@ -268,23 +268,25 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
 struct Seen {
     float top = -__builtin_inff();
     double sum = 0.0;
+    unsigned long long odd = 0;  // lanes that have met a NaN, or +inf
     // Returns the wave's largest of these.
     template <int N>
     __device__ __forceinline__ float add(const float (&x)[N], const Exp& exp) {
         float now = x[0];
 #pragma unroll
-        for (int j = 1; j < N; j++) now = fmaxf(now, x[j]);  // (a NaN shows in the sum)
+        for (int j = 1; j < N; j++) now = fmaxf(now, x[j]);  // (a NaN shows below)
         now = wave_max(now);
         if (now > top) {
             sum *= exp_neg((double)top - (double)now);
             top = now;
         }
         // (all masked: 0 stands in for -inf, and the sum does not count)
-        const float from = top == -__builtin_inff() ? 0.0f : top, least = from - 600.0f;
+        const float from = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
         for (int j = 0; j < N; j++) {
             const double d = (double)x[j] - (double)from;
-            sum += exp(x[j] < least ? -600.0 : d);  // (1e-261 of the largest for less)
+            odd |= __ballot(!(d == d));
+            sum += exp(fmax(d, -600.0));  // (1e-261 of the largest for less)
             // four at a time: sixteen at once do not fit the registers
             if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
@@ -422,11 +424,15 @@ __global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
             if (p == p0) kept.start(x, at, a.best, S.best.keys + wave * 64);
             if (top >= kept.tau && top > -__builtin_inff()) {
 #pragma unroll
-                for (int j = 0; j < kHeld; j++)
-                    kept.offer(x[j], [&] { return at(j); }, a.best);
+                for (int q = 0; q < kHeld / 4; q++) {
+                    const float most = fmaxf(fmaxf(x[4 * q], x[4 * q + 1]), fmaxf(x[4 * q + 2], x[4 * q + 3]));
+                    if (!__ballot(most >= kept.tau)) continue;
+#pragma unroll
+                    for (int j = 4 * q; j < 4 * q + 4; j++) kept.offer(x[j], [&] { return at(j); }, a.best);
+                }
             }
         }
-        const double sum = wave_sum(seen.sum);
+        const double sum = seen.odd ? __builtin_nan("") : wave_sum(seen.sum);
         if (lane == 0) {
             const bool none = seen.top == -__builtin_inff();
             tops[wave] = none ? 0.0 : (double)seen.top;
