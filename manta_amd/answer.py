@@ -86,6 +86,8 @@ class Answerer:
 
     def __init__(self, rt: Runtime, model: Model, questions: int, beams: int, tokens: int, end_token: int,
                  page_tokens: int = 16):
+        if beams > model.vocab:
+            raise ValueError("%d beams of a vocabulary of %d" % (beams, model.vocab))
         self.rt, self.model, self.beams, self.tokens, self.end_token = rt, model, beams, tokens, end_token
         self.questions = questions
         n = questions * beams

@@ -198,7 +198,7 @@ int manta_rocm_beams_create(MantaRocm* rt, int64_t groups, int64_t beams, int64_
     b->groups = groups;
     b->beams = beams;
     b->best = best;
-    b->words = (size_t)(groups * beams * manta::kBeamParts * manta::beam_part_words(best));
+    b->words = (size_t)(manta::beam_parts_in_all(groups * beams) * manta::beam_part_words(best));
     hipError_t e = hipMalloc(&b->memory, b->words * 8 + (size_t)groups * 4);
     if (e == hipSuccess) e = hipMemset((char*)b->memory + b->words * 8, 0, (size_t)groups * 4);
     if (e == hipSuccess) e = hipDeviceSynchronize();
@@ -239,6 +239,9 @@ int manta_rocm_beam_select(MantaRocm* rt, MantaRocmBeams* b, int dtype, const vo
         return fail(err, MANTA_ROCM_ERROR, "beam_select: end token %lld of %lld", (long long)end_token, (long long)vocab);
     if (groups > 0 && (!logits || !scores || !parents || !tokens || !totals))
         return fail(err, MANTA_ROCM_ERROR, "beam_select: nil pointer");
+    if (best != beams && groups > 0 && (totals == scores || (ended && now_ended == ended)))
+        return fail(err, MANTA_ROCM_ERROR, "beam_select: in place needs as many results as beams (%lld, %lld)",
+                    (long long)best, (long long)beams);
     if ((uintptr_t)logits % element_size(dtype) != 0)
         return fail(err, MANTA_ROCM_ERROR, "beam_select: logits are not aligned to their elements");
     int rc = manta_rt::use(rt, err);

@@ -56,6 +56,11 @@ MANTA_HD int beam_parts(int64_t rows, int64_t vocab) {
     parts = parts < pieces ? parts : pieces;
     return (int)(parts < kBeamParts ? parts : kBeamParts);
 }
+// Parts that any call of up to so many rows has.
+MANTA_HD int64_t beam_parts_in_all(int64_t rows) {
+    if (rows >= 1024) return rows;
+    return rows * kBeamParts < 1024 ? rows * kBeamParts : 1024;
+}
 
 inline const char* check_beams(int64_t groups, int64_t beams, int64_t best) {
     if (groups < 0 || beams < 1 || beams > kMaxBeams) return "1 to 64 beams";

@@ -158,7 +158,8 @@ class Beams:
             raise ValueError("logits must be [groups, beams, vocab] (got %s)" % (logits.shape,))
         groups, beams, vocab = logits.shape
         strides = logits.strides
-        if strides is not None and groups > 1 and strides[0] != beams * strides[1]:
+        row = vocab if strides is None else strides[0 if beams == 1 else 1]
+        if strides is not None and groups > 1 and strides[0] != beams * row:
             raise ValueError("logits of a group must follow those of the group before (strides %s)" % (strides,))
         if len(parents.shape) != 2 or parents.shape[0] != groups:
             raise ValueError("parents must be [%d, best] (got %s)" % (groups, parents.shape))
@@ -173,6 +174,6 @@ class Beams:
                 raise ValueError("%s must be a whole %s array %s (got %s %s)"
                                  % (name, np.dtype(dt).name, shape, a.dtype, a.shape))
         call("manta_rocm_beam_select", self.rt.handle, self.handle, kind, logits.addr,
-             vocab if strides is None else strides[1], groups, beams, vocab, scores.addr,
+             row, groups, beams, vocab, scores.addr,
              None if ended is None else ended.addr, end_token, best, parents.addr, tokens.addr, totals.addr,
              None if out_ended is None else out_ended.addr)

@@ -19,6 +19,7 @@ long long pitch(long long w) { return product_pitch(w); }
 long long at(long long p, long long r, long long c) { return product_at(p, r, c); }
 long long rows(long long n, int gated) { return weight_rows(n, gated); }
 int parts(long long rows, long long vocab) { return beam_parts(rows, vocab); }
+long long all_parts(long long rows) { return beam_parts_in_all(rows); }
 int columns(long long group) { return reorder_columns(group); }
 int ints() { return kReorderInts; }
 int piece() { return kBeamPiece; }
@@ -40,6 +41,7 @@ def lib(tmp_path_factory):
     L.at.argtypes = [C.c_longlong] * 3
     L.rows.argtypes = [C.c_longlong, C.c_int]
     L.parts.argtypes = [C.c_longlong] * 2
+    L.all_parts.argtypes, L.all_parts.restype = [C.c_longlong], C.c_longlong
     L.columns.argtypes = [C.c_longlong]
     return L
 
@@ -82,6 +84,14 @@ def test_parts_of_rows(lib):
             assert cuts[0] == 0 and cuts[-1] == pieces and all(a < b for a, b in zip(cuts, cuts[1:]))
             assert rows * n <= max(1024, rows)
             assert n == 1 or n == min(64, pieces) or rows * (n + 1) > 1024
+
+
+def test_scratch_holds_every_smaller_call(lib):
+    for made in (1, 2, 15, 16, 17, 100, 512, 1023, 1024, 1025, 5000):
+        have = lib.all_parts(made)
+        for rows in range(1, made + 1):
+            for vocab in (1, 5000, 100000, 2 ** 31 - 17):
+                assert rows * lib.parts(rows, vocab) <= have
 
 
 def test_columns_of_tables(lib):

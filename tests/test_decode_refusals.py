@@ -125,6 +125,14 @@ def test_shapes_of_beams():
         b.select(*good, ended=_Array((2, 8), i32))
 
 
+def test_no_more_beams_than_tokens():
+    from manta_amd import answer
+
+    model = type("Model", (), {"vocab": 3})()
+    with pytest.raises(ValueError, match="4 beams of a vocabulary of 3"):
+        answer.Answerer(None, model, 1, 4, 16, 0)
+
+
 def test_reorder_without_a_cache():
     with pytest.raises(_lib.MantaRocmError, match="nil cache"):
         call("manta_rocm_cache_reorder", None, None, P, P, 4, 2)

@@ -1,11 +1,15 @@
 """The choice of the next beams: parents and tokens equal to those of 64 bits,
-totals within their one rounding (2^-24; the sums' own error is some 1e-15)."""
+totals within their one rounding, 2^-24, and the sums' error.  Each term of a
+sum is within 1e-10 of it but the largest, exp(0), which is exact: with p the
+largest's share the sum is off by 1e-10 (1 - p) of itself at most, its logarithm
+by as much, and 1 - p <= -log p, which is no more than |total| where scores are
+not positive.  So 1e-10 |total|; that of f64 additions is some 1e-15."""
 import numpy as np
 import pytest
 
 from cache_oracle import from_bits, to_bits
 from decode_oracle import beams
-from manta_amd import rocm
+from manta_amd import _lib, rocm
 
 pytestmark = pytest.mark.gpu
 
@@ -29,7 +33,7 @@ def _run(rt, logits, scores, best, dtype, ended=None, end_token=0, stride=None, 
     np.testing.assert_array_equal(tokens, wt)
     live = wp >= 0
     assert np.isneginf(totals[~live]).all()
-    assert (np.abs(totals[live] - ws[live]) <= np.abs(ws[live]) * 2.0 ** -24 * 1.0001 + 1e-30).all()
+    assert (np.abs(totals[live] - ws[live]) <= np.abs(ws[live]) * (2.0 ** -24 + 1e-10) * 1.0001 + 1e-30).all()
     return parents, tokens, totals
 
 
@@ -129,3 +133,42 @@ def test_a_handle_serves_smaller_calls_and_repeats(rt):
     np.testing.assert_array_equal(out[0].download(), wp)
     np.testing.assert_array_equal(out[1].download(), wt)
     np.testing.assert_allclose(s.download(), ws, rtol=2.0 ** -23)
+
+
+def test_one_beam_a_group_at_any_stride(rt):
+    """The middle axis of a view has one entry: its stride says nothing."""
+    rng = np.random.default_rng(12)
+    logits = rng.standard_normal((5, 900)).astype(np.float32)
+    whole = rt.to_device(logits)
+    scores = rt.to_device(np.zeros((5, 1), np.float32))
+    h = rt.beams(5, 1, 3)
+    for stride in (900, 1, 7):
+        out = [rt.empty((5, 3), np.int32), rt.empty((5, 3), np.int32), rt.empty((5, 3), np.float32)]
+        h.select(rocm.View(whole, (5, 1, 700), (900, stride, 1), 20), scores, *out)
+        parents, tokens, _ = (x.download() for x in out)
+        wp, wt, _ = beams(logits[:, None, 20:720], np.zeros((5, 1), np.float32), 3)
+        np.testing.assert_array_equal(parents, wp)
+        np.testing.assert_array_equal(tokens, wt)
+
+
+def test_in_place(rt):
+    """scores and ended are the results' own memory: as many results as beams,
+    or the call is refused."""
+    rng = np.random.default_rng(13)
+    logits, scores = rng.standard_normal((6, 4, 5000)).astype(np.float32), -rng.random((6, 4)).astype(np.float32)
+    ended = (rng.random((6, 4)) < 0.3).astype(np.int32)
+    want = beams(logits, scores, 4, ended, 9)
+    s, e, d = rt.to_device(scores), rt.to_device(ended), rt.to_device(logits)
+    p, t = rt.empty((6, 4), np.int32), rt.empty((6, 4), np.int32)
+    h = rt.beams(6, 4, 8)
+    h.select(d, s, p, t, s, ended=e, end_token=9, out_ended=e)
+    np.testing.assert_array_equal(p.download(), want[0])
+    np.testing.assert_array_equal(t.download(), want[1])
+    np.testing.assert_array_equal(e.download(), want[1] == 9)
+    assert (np.abs(s.download() - want[2]) <= np.abs(want[2]) * (2.0 ** -24 + 1e-10) * 1.0001).all()
+    other = rt.empty((24,), np.float32)
+    for totals, now in ((s.addr, None), (other.addr, e.addr)):
+        with pytest.raises(_lib.MantaRocmError, match="in place"):
+            _lib.call("manta_rocm_beam_select", rt.handle, h.handle, 32, d.addr, 5000, 6, 4, 5000, s.addr, e.addr, 9, 3,
+                      p.addr, t.addr, totals, now)
+    np.testing.assert_array_equal(t.download(), want[1])
