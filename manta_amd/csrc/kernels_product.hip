@@ -470,8 +470,8 @@ __global__ __launch_bounds__(WAVES * 64) void product_few_kernel(ProductArgs a) 
 
 // Many rows: a workgroup of WM x WN waves takes 16 WM MT tokens and 16 WN NT
 // weight rows, a wave MT x NT tiles of 16 x 16.  Blocks of both operands
-// stream through LDS, ST of the summed columns' steps ahead of the products,
-// by direct-to-LDS loads: a block is 1 KB in a row where it lies and where it
+// stream through LDS, ST stages of SUB steps of the summed columns ahead of the
+// products, by direct-to-LDS loads: a block is 1 KB in a row where it lies and where it
 // goes, and a wave reads it back 16 bytes a lane in order, so neither side
 // has a bank conflict.
 //
@@ -480,13 +480,14 @@ __global__ __launch_bounds__(WAVES * 64) void product_few_kernel(ProductArgs a) 
 // of a 256 x 256 tile's 67 us when the whole card works on random codes (the
 // clock falls with the matrix cores' load: 43 us on 16 compute units), the
 // fill of 32 KB a step about 45 bytes a clock.
-template <class E, bool GATED, int WM, int WN, int MT, int NT, int ST>
+template <class E, bool GATED, int WM, int WN, int MT, int NT, int ST, int SUB>
 __global__ __launch_bounds__(WM* WN * 64) void product_tile_kernel(
     ProductArgs a, int row_tiles, int w_tiles) {
     constexpr int TM = WM * MT, TN = WN * NT, WAVES = WM * WN;
-    constexpr int LPW = (TM + TN) / WAVES;  // blocks that a wave loads a step
-    static_assert(LPW * WAVES == TM + TN, "a step's blocks split evenly over the waves");
-    constexpr int STAGE = (TM + TN) * 1024;
+    constexpr int LPW = (TM + TN) * SUB / WAVES;  // blocks that a wave loads a stage
+    static_assert(LPW * WAVES == (TM + TN) * SUB && SUB <= 2, "a stage's blocks split evenly over the waves");
+    constexpr int STAGE = (TM + TN) * SUB * 1024;
+    const int stages = a.steps / SUB;  // (steps is even)
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -505,11 +506,11 @@ __global__ __launch_bounds__(WM* WN * 64) void product_tile_kernel(
     const int8_t* src[LPW];
 #pragma unroll
     for (int i = 0; i < LPW; i++) {
-        const int b = wave * LPW + i;
+        const int b = (wave * LPW + i) / SUB;
         // (blocks past the operand read its last one; nothing of theirs is stored)
         const int8_t* p = b < TM ? a.x + min((int64_t)rt * TM + b, x_blocks - 1) * a.steps * 1024
                                  : a.w + (int64_t)min(wt * TN + b - TM, a.w_blocks - 1) * a.steps * 1024;
-        src[i] = p + lane * 16;
+        src[i] = p + (wave * LPW + i) % SUB * 1024 + lane * 16;
     }
     const uint32_t base = lds_addr(smem) + wave * LPW * 1024;
     auto issue = [&](int k) {
@@ -517,49 +518,54 @@ __global__ __launch_bounds__(WM* WN * 64) void product_tile_kernel(
 #pragma unroll
         for (int i = 0; i < LPW; i++) {
             lds_load16(src[i], dst + i * 1024);
-            src[i] += 1024;
+            src[i] += SUB * 1024;
         }
     };
 #pragma unroll
     for (int k = 0; k < ST; k++)
-        if (k < a.steps) issue(k);
+        if (k < stages) issue(k);
     v4i sums[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int t = 0; t < NT; t++) sums[m][t] = v4i{0, 0, 0, 0};
     const int m0 = wave % WM * MT, t0 = wave / WM * NT;  // this wave's blocks of the tile
-    v4i wv[2][NT], xv[2][MT];
+    v4i wv[2][SUB][NT], xv[2][SUB][MT];
     auto read = [&](int k, int into) {
         const uint8_t* stage = smem + (k % ST) * STAGE + lane * 16;
 #pragma unroll
-        for (int t = 0; t < NT; t++) wv[into][t] = *(const v4i*)(stage + (TM + t0 + t) * 1024);
+        for (int u = 0; u < SUB; u++) {
 #pragma unroll
-        for (int m = 0; m < MT; m++) xv[into][m] = *(const v4i*)(stage + (m0 + m) * 1024);
+            for (int t = 0; t < NT; t++) wv[into][u][t] = *(const v4i*)(stage + ((TM + t0 + t) * SUB + u) * 1024);
+#pragma unroll
+            for (int m = 0; m < MT; m++) xv[into][u][m] = *(const v4i*)(stage + ((m0 + m) * SUB + u) * 1024);
+        }
     };
     auto multiply = [&](int from) {
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int u = 0; u < SUB; u++)
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-                sums[m][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[from][t], xv[from][m], sums[m][t], 0, 0, 0);
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                    sums[m][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[from][u][t], xv[from][u][m], sums[m][t], 0, 0, 0);
     };
-    // Step k's products run while step k + 1's operands come out of LDS.  At
-    // the barrier step k + 1 has arrived and every wave holds step k, whose
-    // place step k + ST takes.
+    // Stage k's products run while stage k + 1's operands come out of LDS.  At
+    // the barrier stage k + 1 has arrived and every wave holds stage k, whose
+    // place stage k + ST takes.
     auto step = [&](int k, int now) {
-        if (k + 1 < a.steps) {
-            mq_wait_barrier<LPW, ST - 2>(a.steps - 2 - k);
-            if (k + ST < a.steps) issue(k + ST);
+        if (k + 1 < stages) {
+            mq_wait_barrier<LPW, ST - 2>(stages - 2 - k);
+            if (k + ST < stages) issue(k + ST);
             read(k + 1, now ^ 1);
         }
         multiply(now);
     };
-    mq_wait_barrier<LPW, ST - 1>(a.steps - 1);
+    mq_wait_barrier<LPW, ST - 1>(stages - 1);
     read(0, 0);
-    for (int k = 0; k < a.steps; k += 2) {  // (steps is even)
+    for (int k = 0; k < stages; k += 2) {
         step(k, 0);
-        step(k + 1, 1);
+        if (SUB == 1 || k + 1 < stages) step(k + 1, 1);
     }
     const int64_t row0 = ((int64_t)rt * TM + m0) * 16 + (lane & 15);
     const BlockScales<NT> scales(a, wt * TN + t0);
@@ -575,21 +581,21 @@ __global__ __launch_bounds__(WM* WN * 64) void product_tile_kernel(
     }
 }
 
-template <class E, bool GATED, int WM, int WN, int MT, int NT, int ST>
+template <class E, bool GATED, int WM, int WN, int MT, int NT, int ST, int SUB>
 hipError_t product_tiles(const ProductArgs& a, hipStream_t s) {
     constexpr int TM = WM * MT, TN = WN * NT;
-    const size_t lds = (size_t)ST * (TM + TN) * 1024;
+    const size_t lds = (size_t)ST * (TM + TN) * SUB * 1024;
     int device = 0;
     if (const hipError_t e = hipGetDevice(&device)) return e;
     static std::atomic<uint64_t> set{0};  // devices whose kernel may use that much LDS
     if (!(set.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
-        const hipError_t e = hipFuncSetAttribute((const void*)product_tile_kernel<E, GATED, WM, WN, MT, NT, ST>,
+        const hipError_t e = hipFuncSetAttribute((const void*)product_tile_kernel<E, GATED, WM, WN, MT, NT, ST, SUB>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
         set.fetch_or(1ull << (device & 63), std::memory_order_relaxed);
     }
     const int64_t row_tiles = (a.rows + 16 * TM - 1) / (16 * TM), w_tiles = (a.w_blocks + TN - 1) / TN;
-    product_tile_kernel<E, GATED, WM, WN, MT, NT, ST>
+    product_tile_kernel<E, GATED, WM, WN, MT, NT, ST, SUB>
         <<<(unsigned)(row_tiles * w_tiles), WM * WN * 64, lds, s>>>(a, (int)row_tiles, (int)w_tiles);
     return hipGetLastError();
 }
@@ -608,8 +614,8 @@ hipError_t product_of(const ProductArgs& a, hipStream_t s) {
     auto few = [&](int mt, int nt) { return ((rb + mt - 1) / mt) * ((wb + nt - 1) / nt); };
     // The smallest tile that still is a workgroup a compute unit or less: more
     // of them share the reading of the weight, and its latency (32 rows x 4096
-    // columns: 16 x 32 tiles 5.9, 32 x 32 7.3; 64 x 4096: 64 x 32 9.1, tiles
-    // through LDS 14.9)
+    // columns: 16 x 32 tiles 5.9, 32 x 32 7.3; 64 x 4096: 64 x 32 9.1, tiles of
+    // 64 x 64 through LDS 14.9)
     if constexpr (!GATED)
         if (few(1, 1) <= a.cus) return product_few<E, GATED, 8, 1, 1, 4>(a, s);
     if (few(1, 2) <= a.cus) return product_few<E, GATED, 8, 1, 2, 2>(a, s);
@@ -620,17 +626,28 @@ hipError_t product_of(const ProductArgs& a, hipStream_t s) {
     if (rb == 1) return product_few<E, GATED, 8, 1, 2, 2>(a, s);
     if (rb == 2) return product_few<E, GATED, 8, 2, 2, 2>(a, s);
     // Tiles of 64 x 64 while those are few: a larger tile of a unit's own takes
-    // as long as several of them (512 x 4096: 17.5, 128 x 128 26.9; 1024 x 4096
-    // 29.0, 30.8; 512 x 12288 40.2, 37.9)
+    // as long as several of them (512 x 4096: 15.1, 128 x 128 26.9; 1024 x 4096
+    // 27.1, 30.8; 512 x 12288 40.2, 37.9)
     const int64_t t64 = ((a.rows + 63) / 64) * ((wb + 3) / 4), t128 = ((a.rows + 127) / 128) * ((wb + 7) / 8);
-    if (t64 <= 4 * a.cus) return product_tiles<E, GATED, 2, 2, 2, 2, 4>(a, s);
+    if (t64 <= 4 * a.cus) {
+        // a tile a unit or less: a deep ring, 128 columns a barrier (589 x 832 of
+        // 7936 summed: 19.4, two stages 28.5, four of 64 columns 23.9)
+        if (t64 <= a.cus) return product_tiles<E, GATED, 2, 2, 2, 2, 4, 2>(a, s);
+        // one row of tiles reads its weight out of memory (48 rows x 2 x 12288:
+        // 18.3, and 19.1 with less LDS)
+        if (rb <= 4) return product_tiles<E, GATED, 2, 2, 2, 2, 4, 1>(a, s);
+        // several a unit wait for each other's data with little LDS each (512 x
+        // 4096: 15.1, four stages 16.4, of 64 columns 18.3; 1024 x 4096: 27.1,
+        // 30.5, 29.6)
+        return product_tiles<E, GATED, 2, 2, 2, 2, 2, 2>(a, s);
+    }
     // 256 x 256 needs half of the operands' reads of 128 x 128, but comes in
     // whole rounds of a tile a unit, 57 each, against 17.5 for a 128 x 128 tile
     // a unit and 10 (1024 x 12288: 60.1 and 66.0; 2048 x 4096: 57.7 and 43;
     // 8192 x 4096: 121 and 158)
     const int64_t t256 = ((a.rows + 255) / 256) * ((wb + 15) / 16);
-    if ((t256 + a.cus - 1) / a.cus * 13 <= t128 * 4 / a.cus + 2) return product_tiles<E, GATED, 2, 4, 8, 4, 2>(a, s);
-    return product_tiles<E, GATED, 2, 2, 4, 4, 2>(a, s);
+    if ((t256 + a.cus - 1) / a.cus * 13 <= t128 * 4 / a.cus + 2) return product_tiles<E, GATED, 2, 4, 8, 4, 2, 1>(a, s);
+    return product_tiles<E, GATED, 2, 2, 4, 4, 2, 1>(a, s);
 }
 
 template <class E>
