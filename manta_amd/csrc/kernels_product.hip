@@ -471,9 +471,9 @@ __global__ __launch_bounds__(WAVES * 64) void product_few_kernel(ProductArgs a) 
 // Many rows: a workgroup of WM x WN waves takes 16 WM MT tokens and 16 WN NT
 // weight rows, a wave MT x NT tiles of 16 x 16.  Blocks of both operands
 // stream through LDS, ST stages of SUB steps of the summed columns ahead of the
-// products, by direct-to-LDS loads: a block is 1 KB in a row where it lies and where it
-// goes, and a wave reads it back 16 bytes a lane in order, so neither side
-// has a bank conflict.
+// products, by direct-to-LDS loads: a block is 1 KB in a row where it lies and
+// where it goes, and a wave reads it back 16 bytes a lane in order, so neither
+// side has a bank conflict.
 //
 // 8192 x 4096 x 4096 bf16: 121 us, 2.27 POP/s (torch's int8 product of that
 // size, without scales: 130).  What bounds it: a step's products alone take 54
@@ -642,11 +642,12 @@ hipError_t product_of(const ProductArgs& a, hipStream_t s) {
         return product_tiles<E, GATED, 2, 2, 2, 2, 2, 2>(a, s);
     }
     // 256 x 256 needs half of the operands' reads of 128 x 128, but comes in
-    // whole rounds of a tile a unit, 57 each, against 17.5 for a 128 x 128 tile
-    // a unit and 10 (1024 x 12288: 60.1 and 66.0; 2048 x 4096: 57.7 and 43;
-    // 8192 x 4096: 121 and 158)
+    // whole rounds of a tile a unit, 57 each, against 17.5 a tile for the unit
+    // that has most of 128 x 128, and 9 (1024 x 12288: 60.1 and 66.0; 2048 x 4096:
+    // 57.7 and 43; 8192 x 4096: 121 and 158; 16384 x 640: 54.8 and 63.8)
     const int64_t t256 = ((a.rows + 255) / 256) * ((wb + 15) / 16);
-    if ((t256 + a.cus - 1) / a.cus * 13 <= t128 * 4 / a.cus + 2) return product_tiles<E, GATED, 2, 4, 8, 4, 2, 1>(a, s);
+    if ((t256 + a.cus - 1) / a.cus * 13 <= (t128 + a.cus - 1) / a.cus * 4 + 2)
+        return product_tiles<E, GATED, 2, 4, 8, 4, 2, 1>(a, s);
     return product_tiles<E, GATED, 2, 2, 4, 4, 2, 1>(a, s);
 }
 
