@@ -103,12 +103,21 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 // of squares is one exchange among them.  Sums of squares are f64: no number
 // of f32 leaves its range.  The weights are fetched into LDS once for a
 // workgroup's `tokens`, whose heads it takes as one run, the first ones' data
-// on their way while the angles are worked out.  With PARTS heads may start
-// anywhere and the rotated columns end anywhere: pieces are 16 bytes at any
-// alignment, and the last of the pairs and of the rest can be a part of one.  Bytes bound: 8192 tokens of 40
+// on their way while the angles are worked out.  Bytes bound: 8192 tokens of 40
 // heads of 128, bf16, out of memory: 29 to 35 us, 4.8 to 5.7 TB/s.
+//
+// PIECES says how a head splits into pieces of 16 bytes:
+//   kEven   whole ones at their alignment, pairs and rest alike;
+//   kShared at any alignment, the last one of the pairs and of the rest ending
+//           where they do: it shares its first elements with the piece before,
+//           which works out the same for them (the sum takes them once);
+//   kShort  as kShared where there are too few for one piece: the last is taken
+//           element by element.
+// (4169 tokens of 36 heads of 80, 50 of them rotated, bf16: kShared 22 us, kShort
+// 33.)
+enum { kEven, kShared, kShort };
 constexpr int kNormTokens = 8;
-template <class E, bool INTERLEAVED, bool PARTS, int NP>
+template <class E, bool INTERLEAVED, int PIECES, int NP>
 __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, RotaryNorms n, int lanes, int tokens) {
     typedef typename E::T T;
     constexpr int V = E::kWide;
@@ -120,6 +129,12 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
     const int turned = (half + V - 1) / V;                // pieces of V pairs
     const int rest = (a.head_dim - a.rot + V - 1) / V;    // pieces of V columns past them
     const int pieces = turned + rest;
+    // the first pair of a piece, or column past the pairs
+    auto start = [&](int piece) {
+        if (piece < turned) return PIECES == kShared ? min(piece * V, half - V) : piece * V;
+        const int c = a.rot + (piece - turned) * V;
+        return PIECES == kShared ? min(c, a.head_dim - V) : c;
+    };
     const int per = (a.heads + gridDim.y - 1) / gridDim.y;
     const int h0 = blockIdx.y * per, heads = min(a.heads, h0 + per) - h0;
     const int gl = threadIdx.x & (lanes - 1), g0 = threadIdx.x / lanes, step = kThreads / lanes;
@@ -155,38 +170,33 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
             }
 #pragma unroll
             for (int p = 0; p < NP; p++) {
-                const int piece = gl + lanes * p, at = piece * V;
-                if (piece < turned) {
-                    const T *from0 = src + (INTERLEAVED ? 2 * at : at), *from1 = src + (INTERLEAVED ? 2 * at + V : half + at);
-                    if constexpr (!PARTS) {
-                        lo[p] = *(const Piece*)from0;
-                        hi[p] = *(const Piece*)from1;
-                    } else if (at + V <= half) {
-                        lo[p] = load16_any<Piece>(from0);
-                        hi[p] = load16_any<Piece>(from1);
-                    } else {
+                const int piece = gl + lanes * p, at = start(piece);
+                const T* from0 = src + (INTERLEAVED && piece < turned ? 2 * at : at);
+                const T* from1 = src + (INTERLEAVED ? 2 * at + V : half + at);
+                const bool whole = PIECES != kShort || at + V <= (piece < turned ? half : a.head_dim);
+                if (whole && piece < pieces) lo[p] = PIECES == kEven ? *(const Piece*)from0 : load16_any<Piece>(from0);
+                if (whole && piece < turned) hi[p] = PIECES == kEven ? *(const Piece*)from1 : load16_any<Piece>(from1);
+                if constexpr (PIECES == kShort) {
+                    if (whole || piece >= pieces) continue;
 #pragma unroll
-                        for (int j = 0; j < V; j++) {
-                            if (INTERLEAVED ? 2 * at + j < a.rot : at + j < half) lo[p].v[j] = from0[j];
-                            if (INTERLEAVED ? 2 * at + V + j < a.rot : at + j < half) hi[p].v[j] = from1[j];
-                        }
-                    }
-                } else if (piece < pieces) {
-                    const int c = a.rot + (piece - turned) * V;
-                    if constexpr (!PARTS) {
-                        lo[p] = *(const Piece*)(src + c);
-                    } else if (c + V <= a.head_dim) {
-                        lo[p] = load16_any<Piece>(src + c);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < V; j++)
-                            if (c + j < a.head_dim) lo[p].v[j] = src[c + j];
+                    for (int j = 0; j < V; j++) {
+                        const bool pairs = piece < turned;
+                        const int end = !pairs ? a.head_dim : INTERLEAVED ? a.rot - at : half;
+                        if (at + j < end) lo[p].v[j] = from0[j];
+                        if (pairs && at + (INTERLEAVED ? V + j : j) < end) hi[p].v[j] = from1[j];
                     }
                 }
             }
         };
+        int twice[NP];  // elements of a piece that the piece before it has too
 #pragma unroll
-        for (int p = 0; p < NP; p++) lo[p] = hi[p] = Piece{};  // (what is not fetched counts as 0)
+        for (int p = 0; p < NP; p++) {
+            lo[p] = hi[p] = Piece{};  // (what is not fetched counts as 0)
+            const int piece = gl + lanes * p;
+            twice[p] = PIECES != kShared || piece >= pieces ? 0
+                       : piece < turned                     ? (INTERLEAVED ? 2 : 1) * (piece * V - start(piece))
+                                                            : a.rot + (piece - turned) * V - start(piece);
+        }
         if (g0 < all) fetch(g0);
         for (int e = threadIdx.x; e < count * half; e += kThreads) {
             const int token = e / half, p = e - token * half;
@@ -205,9 +215,13 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
             for (int p = 0; p < NP; p++)
 #pragma unroll
                 for (int j = 0; j < V; j++) {
-                    const double u = E::load(lo[p].v[j]), v = E::load(hi[p].v[j]);
-                    sum = fma(u, u, sum);
-                    sum = fma(v, v, sum);
+                    float u = E::load(lo[p].v[j]), v = E::load(hi[p].v[j]);
+                    if (PIECES == kShared) {
+                        u = j < twice[p] ? 0.0f : u;
+                        v = (INTERLEAVED ? V + j : j) < twice[p] ? 0.0f : v;
+                    }
+                    sum = fma((double)u, (double)u, sum);
+                    sum = fma((double)v, (double)v, sum);
                 }
             for (int s = lanes >> 1; s; s >>= 1) sum += __shfl_xor(sum, s);
             bool norm = n.weight[0] != nullptr;
@@ -224,23 +238,23 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                     const int piece = gl + lanes * i;
                     if (piece >= pieces) continue;
                     if (piece >= turned) {
-                        const int at = a.rot + (piece - turned) * V;
+                        const int at = start(piece);
                         Piece o;
 #pragma unroll
                         for (int j = 0; j < V; j++)
                             o.v[j] = norm ? E::store(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
-                        if constexpr (!PARTS) {
+                        if constexpr (PIECES == kEven) {
                             put(out + at, o);
-                        } else if (at + V <= a.head_dim) {
+                        } else if (PIECES == kShared || at + V <= a.head_dim) {
                             store16_any(out + at, o);
-                        } else {
+                        } else if constexpr (PIECES == kShort) {
 #pragma unroll
                             for (int j = 0; j < V; j++)
                                 if (at + j < a.head_dim) out[at + j] = o.v[j];
                         }
                         continue;
                     }
-                    const int p = piece * V;
+                    const int p = start(piece);
                     // the run of columns that lo holds, and hi
                     const int at0 = INTERLEAVED ? 2 * p : p, at1 = INTERLEAVED ? 2 * p + V : half + p;
                     float u[2 * V];
@@ -268,13 +282,13 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                         ylo.v[j] = o[j];
                         yhi.v[j] = o[V + j];
                     }
-                    if constexpr (!PARTS) {
+                    if constexpr (PIECES == kEven) {
                         put(out + at0, ylo);
                         put(out + at1, yhi);
-                    } else if (p + V <= half) {
+                    } else if (PIECES == kShared || p + V <= half) {
                         store16_any(out + at0, ylo);
                         store16_any(out + at1, yhi);
-                    } else {
+                    } else if constexpr (PIECES == kShort) {
 #pragma unroll
                         for (int j = 0; j < V; j++) {
                             if (INTERLEAVED ? at0 + j < a.rot : p + j < half) out[at0 + j] = ylo.v[j];
@@ -312,18 +326,21 @@ hipError_t launch_normed(const RotaryArgs& a, RotaryNorms n, hipStream_t s) {
     tokens = tokens < 1 ? 1 : tokens > kNormTokens ? kNormTokens : tokens;
     const int64_t runs = (a.tokens + tokens - 1) / tokens;
     const dim3 grid((unsigned)(runs < (1 << 20) ? runs : 1 << 20), split);
-    // (with PARTS where there are none: 49.7 us against 42 for 8192 tokens of 40
-    // heads of 128, bf16, out of memory)
-    const int t = (int)tokens;
+    // (pieces at any alignment where all are aligned: 49.7 us against 42 for 8192
+    // tokens of 40 heads of 128, bf16, out of memory)
+    const int t = (int)tokens, over = a.head_dim - a.rot;
     if (a.wide) {  // 64 pieces at most
-        if (a.interleaved) rotary_normed_kernel<E, true, false, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
-        else rotary_normed_kernel<E, false, false, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        if (a.interleaved) rotary_normed_kernel<E, true, kEven, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        else rotary_normed_kernel<E, false, kEven, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+    } else if (a.rot / 2 >= V && (over == 0 || over >= V)) {  // 64 as well: 4 pairs take two pieces' columns
+        if (a.interleaved) rotary_normed_kernel<E, true, kShared, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        else rotary_normed_kernel<E, false, kShared, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
     } else if (pieces <= 64) {
-        if (a.interleaved) rotary_normed_kernel<E, true, true, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
-        else rotary_normed_kernel<E, false, true, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
-    } else {
-        if (a.interleaved) rotary_normed_kernel<E, true, true, 2><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
-        else rotary_normed_kernel<E, false, true, 2><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        if (a.interleaved) rotary_normed_kernel<E, true, kShort, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        else rotary_normed_kernel<E, false, kShort, 1><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+    } else if constexpr (V == 4) {  // a pair and 254 columns of f32
+        if (a.interleaved) rotary_normed_kernel<E, true, kShort, 2><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
+        else rotary_normed_kernel<E, false, kShort, 2><<<grid, kThreads, 0, s>>>(a, n, lanes, t);
     }
     return hipGetLastError();
 }

@@ -21,7 +21,8 @@ def _check(got, x, norm, eps, pos, freqs, layout, magnitude, dtype):
 @pytest.mark.parametrize("tokens,heads,d,rot", [
     (1, (1,), 2, 2), (1, (6, 6), 64, 64), (3, (32, 8), 128, 128), (7, (5, 1), 96, 32), (600, (4, 2), 64, 16),
     (2, (3,), 80, 80), (5, (2, 1, 1, 3), 33, 22), (4, (12, 2), 256, 256), (9, (7,), 192, 50), (1, (3, 1), 255, 2), (3, (2, 1), 256, 2), (70, (3, 3), 80, 50), (5, (4,), 77, 44),
-    (1100, (9, 3), 128, 64), (2, (70, 5), 128, 96)])
+    (1100, (9, 3), 128, 64), (2, (70, 5), 128, 96), (6, (3, 2), 128, 126), (3, (2, 1), 80, 8), (2, (1,), 20, 4),
+    (65, (7, 2), 47, 40), (4, (3,), 24, 16)])
 def test_sizes_layouts_types(rt, dtype, layout, tokens, heads, d, rot):
     print("rotary_normed", dtype, layout, tokens, heads, d, rot, flush=True)
     rng = np.random.default_rng(tokens + 10 * d + rot)
