@@ -6,8 +6,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#pragma clang fp contract(off)
-
 namespace manta {
 
 // As one vector: of a struct's elements the compiler makes several accesses.
@@ -37,6 +35,7 @@ __device__ __forceinline__ void store16_past(void* p, const P& v) {
 // for t beyond the largest number; `exact`: there may be such a t (max >= 2^121;
 // its code is 127 or -127), or 1 / max is not a normal number.
 __device__ __forceinline__ uint32_t ratio_codes(const float* t, float max, float inv, bool exact) {
+#pragma clang fp contract(off)  // (here, not in the file: what includes it has its own rule)
     constexpr float kRound = 12582912.0f;
     uint32_t b[4];
     float far = 0.0f;

@@ -24,6 +24,15 @@ struct alignas(sizeof(typename E::T) * V) Pack {
     typename E::T v[V];
 };
 
+// The part of a turn that pos * turns leaves, in [-1/2, 1/2]: of the exact
+// product, whose f64 rounding is 3e-8 turns off at position 2^31.
+__device__ __forceinline__ float turn_left(double pos, double turns) {
+    return (float)fma(pos, turns, -rint(pos * turns));
+}
+// A pair turned: a product and a fused one, so two roundings.
+__device__ __forceinline__ float turn_1(float x1, float x2, float c, float s) { return fmaf(x1, c, -(x2 * s)); }
+__device__ __forceinline__ float turn_2(float x1, float x2, float c, float s) { return fmaf(x2, c, x1 * s); }
+
 // V elements at once: V pairs of a head, or V columns past the rotated ones.
 template <class E, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
@@ -34,8 +43,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         __syncthreads();  // an earlier token's angles have been used
         const double pos = (double)a.positions[token];
         for (int p = threadIdx.x; p < half; p += kThreads) {
-            const double t = pos * a.turns[p];
-            const float r = (float)(t - rint(t));
+            const float r = turn_left(pos, a.turns[p]);
             float s, c;
             sincospif(2.0f * r, &s, &c);
             cs[p] = a.magnitude * c;
@@ -77,7 +85,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
                 const T t1 = !INTERLEAVED ? lo.v[j] : e < V ? lo.v[e % V] : hi.v[e % V];
                 const T t2 = !INTERLEAVED ? hi.v[j] : e + 1 < V ? lo.v[(e + 1) % V] : hi.v[(e + 1) % V];
                 const float x1 = E::load(t1), x2 = E::load(t2), c = cs[p + j], s = sn[p + j];
-                const T y1 = E::store(x1 * c - x2 * s), y2 = E::store(x2 * c + x1 * s);
+                const T y1 = E::store(turn_1(x1, x2, c, s)), y2 = E::store(turn_2(x1, x2, c, s));
                 if (!INTERLEAVED) {
                     ylo.v[j] = y1;
                     yhi.v[j] = y2;
@@ -200,8 +208,7 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
         if (g0 < all) fetch(g0);
         for (int e = threadIdx.x; e < count * half; e += kThreads) {
             const int token = e / half, p = e - token * half;
-            const double t = (double)a.positions[t0 + token] * a.turns[p];
-            const float r = (float)(t - rint(t));
+            const float r = turn_left((double)a.positions[t0 + token], a.turns[p]);
             float s, c;
             sincospif(2.0f * r, &s, &c);
             cs[token][p] = a.magnitude * c;
@@ -273,8 +280,8 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                         // pair p + j: elements 2j and 2j + 1 of the run, or j of each half
                         const int e1 = INTERLEAVED ? 2 * j : j, e2 = INTERLEAVED ? 2 * j + 1 : V + j;
                         const float c = cs[token][p + j], s = sn[token][p + j];
-                        o[e1] = E::store(u[e1] * c - u[e2] * s);
-                        o[e2] = E::store(u[e2] * c + u[e1] * s);
+                        o[e1] = E::store(turn_1(u[e1], u[e2], c, s));
+                        o[e2] = E::store(turn_2(u[e1], u[e2], c, s));
                     }
                     Piece ylo, yhi;
 #pragma unroll
