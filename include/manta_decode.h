@@ -53,7 +53,8 @@ int64_t manta_rocm_quantized_bytes(int64_t rows, int64_t width);
 /* Quantise rows x [rows, width] (row r at x + r * x_row elements; f32, f16 or
  * bf16) to 8 bits with a scale a row:
  *   z = x, or x * norm[c] rounded to f32 with norm_dev (f32 [width]);
- *   code = round_half_even(z * 127 / max|z|) in f32, scale = max|z| / 127,
+ *   code = round_half_even(z * 127 / max|z|) in f32 (also where z * 127 is past
+ *   its range), scale = max|z| / 127,
  *   times 1 / sqrt(mean(x^2) + eps) with norm_dev: the RMS norm's factor
  *   cancels in the codes.
  * A row whose max|z| is below 2^-126 has codes and scale 0, one with a z that

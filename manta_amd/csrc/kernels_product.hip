@@ -18,10 +18,14 @@ constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------- quantise
 
-__device__ __forceinline__ int row_code(float z, float max) {
-    const float r = __builtin_rintf(__fdiv_rn(z * 127.0f, max));
-    return (int)fminf(127.0f, fmaxf(-127.0f, r));
-}
+// A row's codes are (z by) / low, `by` 127 and `low` the row's largest |z|; from
+// 2^121 on both are 2^-7 times that, the same quotient of numbers in range.
+struct Ratio {
+    float by, low;
+    __device__ __forceinline__ explicit Ratio(float big)
+        : by(big >= 0x1p121f ? 127.0f * 0x1p-7f : 127.0f), low(big >= 0x1p121f ? big * 0x1p-7f : big) {}
+    __device__ __forceinline__ int code(float z) const { return (int)__builtin_rintf(__fdiv_rn(z * by, low)); }
+};
 
 // One row a workgroup at a time.
 template <class E>
@@ -62,6 +66,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantizeArgs a) {
             else if (!zero) scale = a.norm ? (float)((double)big / 127.0 / sqrt(sum / a.width + a.eps)) : __fdiv_rn(big, 127.0f);
             a.scales[row] = scale;
         }
+        const Ratio ratio(big);
         for (int c0 = tid * 16; c0 < a.pitch; c0 += kThreads * 16) {
             uint32_t words[4];
             for (int k = 0; k < 4; k++) {
@@ -71,7 +76,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantizeArgs a) {
                     int code = 0;
                     if (!zero && c < a.width) {
                         const float v = E::load(x[c]);
-                        code = row_code(a.norm ? v * a.norm[c] : v, big);
+                        code = ratio.code(a.norm ? v * a.norm[c] : v);
                     }
                     word |= (uint32_t)(code & 0xFF) << (8 * j);
                 }
@@ -184,8 +189,8 @@ __global__ __launch_bounds__(kThreads) void quantize_wide_kernel(QuantizeArgs a)
         else if (!zero) scale = NORM ? (float)((double)big / 127.0 / sqrt(sum / a.width + a.eps)) : __fdiv_rn(big, 127.0f);
         a.scales[row] = scale;
     }
-    const float inv = 1.0f / big;
-    const bool exact = big >= 0x1p121f;
+    const Ratio ratio(big);
+    const float inv = 1.0f / ratio.low;
 #pragma unroll
     for (int p = 0; p < NP; p++) {
         const int c0 = (tid + 64 * WAVES * p) * 16;
@@ -195,8 +200,8 @@ __global__ __launch_bounds__(kThreads) void quantize_wide_kernel(QuantizeArgs a)
         for (int k = 0; k < 4; k++) {
             float t[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) t[j] = z(p, 4 * k + j) * 127.0f;
-            word[k] = zero ? 0 : ratio_codes(t, big, inv, exact);
+            for (int j = 0; j < 4; j++) t[j] = z(p, 4 * k + j) * ratio.by;
+            word[k] = zero ? 0 : ratio_codes(t, ratio.low, inv, false);
         }
         *(uint4*)(a.codes + product_at(a.pitch, row, c0)) = make_uint4(word[0], word[1], word[2], word[3]);
     }
