@@ -79,6 +79,15 @@ class _Rows:
         self.x8, self.a8, self.f8 = (rt.quantized(rows, w) for w in (m.width, q * d, m.blocks[0].feed.n))
 
 
+def pool_pages(questions: int, beams: int, tokens: int, page_tokens: int) -> int:
+    """Pages that any course of the beams finds enough: each beam's own, and of
+    beams of one page one more for every two.  (Several beams that go on from
+    one take a copy each of its last page before that page is free; of more
+    than one page they share the others, and have as many to spare.)"""
+    each = (tokens + page_tokens - 1) // page_tokens
+    return questions * (beams * each + (beams // 2 if each == 1 else 0))
+
+
 class Answerer:
     """Answers up to `questions` questions at once with `beams` beams each;
     a question and its answer have at most `tokens` tokens.  Sequence
@@ -92,8 +101,9 @@ class Answerer:
         self.questions = questions
         n = questions * beams
         each = (tokens + page_tokens - 1) // page_tokens
-        self.cache = rt.cache(pages=n * each, kv_heads=model.kv_heads, head_dim=model.head_dim, seqs=n,
-                              table_pages=each, page_tokens=page_tokens, layers=len(model.blocks))
+        self.cache = rt.cache(pages=pool_pages(questions, beams, tokens, page_tokens), kv_heads=model.kv_heads,
+                              head_dim=model.head_dim, seqs=n, table_pages=each, page_tokens=page_tokens,
+                              layers=len(model.blocks))
         self.rot = rt.rotary_bind(rotary_freqs(model.head_dim))
         self.choice = rt.beams(questions, beams, beams)
         self.seqs, self.ones = self._ints(range(n)), self._ints([1] * n)
