@@ -116,6 +116,11 @@ int manta_rocm_beam_select(MantaRocm* rt, MantaRocmBeams* b, int dtype, const vo
                            const int32_t* ended_dev, int64_t end_token, int64_t best, int32_t* out_parents_dev,
                            int32_t* out_tokens_dev, float* out_scores_dev, int32_t* out_ended_dev, char** err);
 
+/* What the next step reads: out[i] = tokens[i], or `instead` where that is
+ * negative (no continuation).  out_dev may be tokens_dev; n is at most 2^25. */
+int manta_rocm_beam_inputs(MantaRocm* rt, const int32_t* tokens_dev, int64_t n, int64_t instead, int32_t* out_dev,
+                           char** err);
+
 /* Beams that go on from others: seqs_dev (int32 [n], distinct slots) holds
  * n / group groups, and its entry i takes over what entry parents_dev[i] (0
  * to group - 1) of its own group held when the call began, sharing its pages;

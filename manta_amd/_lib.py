@@ -230,6 +230,7 @@ SIGNATURES = {
     "manta_rocm_beams_destroy": (None, [_p]),
     "manta_rocm_beam_select": (
         C.c_int, [_p, _p, C.c_int, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _err]),
+    "manta_rocm_beam_inputs": (C.c_int, [_p, _p, _i64, _i64, _p, _err]),
     "manta_rocm_cache_reorder": (C.c_int, [_p, _p, _p, _p, _i64, _i64, _err]),
     "manta_rocm_embed_pooled": (
         C.c_int,

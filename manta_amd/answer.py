@@ -166,7 +166,7 @@ class Answerer:
         """One token of every beam, and the next ones' choice: parents and
         next hold it.  Only calls that may be recorded into a HIP graph."""
         rt, r = self.rt, self.rows
-        rt.copy(self.tokens_now, self.next)
+        rt.beam_inputs(self.next, self.tokens_now, self.end_token)  # (a beam without one reads that, for nothing)
         rt.copy(self.positions, self.cache.lengths)
         self.cache.extend(self.seqs, self.ones)
         rt.gather_rows_f16(self.model.table, self.tokens_now, out=r.x)
@@ -185,7 +185,7 @@ class Answerer:
         self.ask(questions)
         chosen = [(self.parents.download(), self.next.download())]
         for _ in range(most - 1):
-            if self.ended.download().all():
+            if (self.ended.download() | (chosen[-1][0] < 0)).all():
                 break
             self.step()
             chosen.append((self.parents.download(), self.next.download()))

@@ -267,4 +267,16 @@ int manta_rocm_beam_select(MantaRocm* rt, MantaRocmBeams* b, int dtype, const vo
     return launch(rt, "beam_select", err, [&](hipStream_t s) { return manta::launch_beam_select(a, s); });
 }
 
+int manta_rocm_beam_inputs(MantaRocm* rt, const int32_t* tokens, int64_t n, int64_t instead, int32_t* out, char** err) {
+    if (n < 0 || n > manta::kMaxTokens) return fail(err, MANTA_ROCM_ERROR, "beam_inputs: bad token count %lld", (long long)n);
+    if (instead < 0 || instead > manta::kMaxInt32)
+        return fail(err, MANTA_ROCM_ERROR, "beam_inputs: token %lld", (long long)instead);
+    if (n > 0 && (!tokens || !out)) return fail(err, MANTA_ROCM_ERROR, "beam_inputs: nil pointer");
+    int rc = manta_rt::use(rt, err);
+    if (rc || n == 0) return rc;
+    return launch(rt, "beam_inputs", err, [&](hipStream_t s) {
+        return manta::launch_beam_inputs(tokens, (int)n, (int)instead, out, s);
+    });
+}
+
 }  // extern "C"

@@ -62,5 +62,6 @@ struct BeamArgs {
     int dtype;
 };
 hipError_t launch_beam_select(const BeamArgs& a, hipStream_t s);
+hipError_t launch_beam_inputs(const int32_t* tokens, int n, int instead, int32_t* out, hipStream_t s);
 
 }  // namespace manta

@@ -483,6 +483,11 @@ __global__ __launch_bounds__(kThreads, 4) void beam_kernel(BeamArgs a) {
     if (last) merge_group(a, g, S.merge);
 }
 
+__global__ __launch_bounds__(kThreads) void inputs_kernel(const int32_t* tokens, int n, int instead, int32_t* out) {
+    const int i = blockIdx.x * kThreads + threadIdx.x;
+    if (i < n) out[i] = tokens[i] < 0 ? instead : tokens[i];
+}
+
 template <class E>
 hipError_t launch_type(const BeamArgs& a, hipStream_t s) {
     // rows are a grid's second axis, 16 bits of it: whole groups at a time
@@ -511,6 +516,11 @@ hipError_t launch_beam_select(const BeamArgs& a, hipStream_t s) {
     if (a.dtype == MANTA_ROCM_F32) return launch_type<F32>(a, s);
     if (a.dtype == MANTA_ROCM_F16) return launch_type<F16>(a, s);
     return launch_type<Bf16>(a, s);
+}
+
+hipError_t launch_beam_inputs(const int32_t* tokens, int n, int instead, int32_t* out, hipStream_t s) {
+    inputs_kernel<<<(n + kThreads - 1) / kThreads, kThreads, 0, s>>>(tokens, n, instead, out);
+    return hipGetLastError();
 }
 
 }  // namespace manta

@@ -177,3 +177,10 @@ class Beams:
              row, groups, beams, vocab, scores.addr,
              None if ended is None else ended.addr, end_token, best, parents.addr, tokens.addr, totals.addr,
              None if out_ended is None else out_ended.addr)
+
+
+def beam_inputs(rt, tokens, out, instead: int) -> None:
+    for name, a in (("tokens", tokens), ("out", out)):
+        if a.dtype != np.int32 or a.strides is not None or a.nbytes != tokens.nbytes:
+            raise ValueError("%s must be a whole int32 array, one entry a token (got %s %s)" % (name, a.dtype, a.shape))
+    call("manta_rocm_beam_inputs", rt.handle, tokens.addr, tokens.nbytes // 4, instead, out.addr)

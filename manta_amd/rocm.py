@@ -238,6 +238,11 @@ class Runtime:
         """The choice of the next beams, for up to so many (decode.Beams)."""
         return decode.Beams(self, groups, beams, best)
 
+    def beam_inputs(self, tokens: DeviceArray, out: DeviceArray, instead: int = 0) -> None:
+        """What the next step reads (int32): the chosen tokens, or `instead`
+        where there is no continuation (-1)."""
+        decode.beam_inputs(self, tokens, out, instead)
+
     # ------------------------------------------------------------ binding
     def bind_q8(self, codes: np.ndarray, scales: np.ndarray) -> Candidates:
         """codes int8 [n,d] or [sets,n,d]; scales f32 [n] or [sets,n]."""

@@ -1,9 +1,11 @@
-"""The answerer's own account of its pages, on the cache's model."""
+"""The answerer's own account of its pages, on the cache's model, and what the
+next step's inputs refuse."""
 import numpy as np
 import pytest
 
 from cache_oracle import Model
 from decode_oracle import reorder
+from manta_amd import _lib, decode
 from manta_amd.answer import pool_pages
 
 
@@ -33,3 +35,19 @@ def test_no_course_of_the_beams_is_out_of_pages(questions, beams, tokens, page):
             if course % 4 == 3:
                 parents[rng.random(n) < 0.2] = -1  # some have no continuation
             reorder(m, seqs, parents, beams)
+
+
+def test_inputs_that_are_refused():
+    class Array:
+        strides = None
+
+        def __init__(self, n, dtype=np.int32):
+            self.dtype, self.shape, self.nbytes, self.addr = np.dtype(dtype), (n,), n * np.dtype(dtype).itemsize, 4096
+
+    for tokens, out in ((Array(3, np.float32), Array(3)), (Array(3), Array(4)), (Array(3), Array(3, np.uint32))):
+        with pytest.raises(ValueError, match="whole int32 array"):
+            decode.beam_inputs(None, tokens, out, 0)
+    for n, instead, p, message in ((-1, 0, 4096, "token count"), ((1 << 25) + 1, 0, 4096, "token count"),
+                                   (1, -1, 4096, "token -1"), (1, 1 << 31, 4096, "token 2147483648"), (1, 0, None, "nil")):
+        with pytest.raises(_lib.MantaRocmError, match=message):
+            _lib.call("manta_rocm_beam_inputs", None, p, n, instead, p)
