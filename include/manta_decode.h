@@ -97,12 +97,13 @@ void manta_rocm_beams_destroy(MantaRocmBeams* b);
 
 /* The best continuations of every group's beams: of the totals
  *   scores[g, b] + logits[g, b, t] - log(sum over u of exp(logits[g, b, u]))
- * the `best` largest, in descending order, equal ones by the lower (b, t):
- * the beam to out_parents, t to out_tokens, the total to out_scores, each
- * [groups, best].  logits_dev: f32, f16 or bf16 [groups * beams, vocab], rows
- * logits_row elements apart; scores_dev f32 [groups, beams].  Totals are
- * formed and compared in f64 and rounded once.  Within a beam the order is
- * that of its logits.  out_scores_dev may be scores_dev where best is beams.
+ * the `best` largest, in descending order, equal ones by the lower beam, those
+ * of one beam by the larger logit, then the lower token (so that within a beam
+ * the order is that of its logits): the beam to out_parents, t to out_tokens,
+ * the total to out_scores, each [groups, best].  logits_dev: f32, f16 or bf16
+ * [groups * beams, vocab], rows logits_row elements apart; scores_dev f32
+ * [groups, beams].  Totals are formed and compared in f64 and rounded once.
+ * out_scores_dev may be scores_dev where best is beams.
  * ended_dev, when given: int32 [groups, beams]; a beam whose entry is not 0
  * has one continuation, end_token, of total scores[g, b], and its logits are
  * not read.  out_ended_dev, when given: int32 [groups, best], 1 where the

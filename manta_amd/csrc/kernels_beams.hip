@@ -126,8 +126,16 @@ __device__ __forceinline__ double joined(double sum, double* largest) {
     return wave_sum(sum);
 }
 
+// Equal totals: the lower beam, of one beam the larger logit (a score may swallow
+// their difference), then the lower token.  Candidate i of a beam stands for its
+// token: parts lie in the tokens' order, and a part's keys too where logits are
+// equal.
+constexpr int kPlaceBits = 18;
+static_assert(kMaxBeams * kBeamParts * kMaxBest <= 1 << kPlaceBits, "i fits its bits");
 struct Candidate {
-    uint64_t total, place;  // order of the total (0: none), beam << 32 | token
+    uint64_t total, place;  // order of the total (0: none); beam, the logit's order complemented, i
+    __device__ __forceinline__ int beam() const { return (int)(place >> (32 + kPlaceBits)); }
+    __device__ __forceinline__ int index() const { return (int)(place & ((1u << kPlaceBits) - 1)); }
 };
 __device__ __forceinline__ bool better(const Candidate& a, const Candidate& b) {
     return a.total > b.total || (a.total == b.total && a.place < b.place);
@@ -147,6 +155,7 @@ struct MergeShared {
     double largest[kMaxBeams], log_sum[kMaxBeams], score[kMaxBeams];
     int ended[kMaxBeams];
     Candidate found[kFound];
+    int token[kFound];
     Candidate wave_best[kThreads / 64];
     uint32_t tops[kThreads];
     Floor floor;
@@ -200,17 +209,15 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
     __syncthreads();
     auto candidate = [&](int i, uint64_t key) {
         const int b = i / per, k = i - b * per;
-        Candidate c{0, 0};
+        Candidate c{0, (((uint64_t)b << 32) | (uint32_t)~(key >> 32)) << kPlaceBits | (uint32_t)i};
         double t;
         if (M.ended[b]) {
             if (k) return c;
             t = M.score[b];
-            c.place = ((uint64_t)b << 32) | (uint32_t)a.end_token;
         } else {
             if (!key) return c;
             // (apart: the largest may be a number that swallows the logarithm)
             t = M.score[b] + (((double)key_score(key, 0) - M.largest[b]) - M.log_sum[b]);
-            c.place = ((uint64_t)b << 32) | key_index(key);
         }
         if (t > -HUGE_VAL) c.total = total_order(t);
         return c;
@@ -222,45 +229,52 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
     auto each = [&](auto f) {
 #pragma unroll
         for (int r = 0; r < kAhead; r++)
-            if (tid + kThreads * r < n) f(candidate(tid + kThreads * r, keys[r]));
-        for (int i = tid + kThreads * kAhead; i < n; i += kThreads) f(candidate(i, key_at(i)));
+            if (tid + kThreads * r < n) f(candidate(tid + kThreads * r, keys[r]), keys[r]);
+        for (int i = tid + kThreads * kAhead; i < n; i += kThreads) {
+            const uint64_t key = key_at(i);
+            f(candidate(i, key), key);
+        }
     };
-    each([&](const Candidate& c) { top = max(top, coarse(c)); });
+    auto token_of = [&](const Candidate& c, uint64_t key) { return M.ended[c.beam()] ? a.end_token : (int)key_index(key); };
+    each([&](const Candidate& c, uint64_t) { top = max(top, coarse(c)); });
     M.tops[tid] = top;
     __syncthreads();
     find_floor<4>(M.tops, a.best, M.floor);
     __syncthreads();
     const uint32_t floor = M.floor.floor;
-    each([&](const Candidate& c) {
+    each([&](const Candidate& c, uint64_t key) {
         if (c.total && coarse(c) >= floor) {
             const int at = atomicAdd(&M.count, 1);
-            if (at < kFound) M.found[at] = c;
+            if (at < kFound) {
+                M.found[at] = c;
+                M.token[at] = token_of(c, key);
+            }
         }
     });
     __syncthreads();
     const int found = M.count;
-    auto put = [&](int k, const Candidate& c) {
+    auto put = [&](int k, const Candidate& c, int token) {
         const int64_t at = (int64_t)g * a.best + k;
-        a.parents[at] = c.total ? (int)(c.place >> 32) : -1;
-        a.tokens[at] = c.total ? (int)(uint32_t)c.place : -1;
+        a.parents[at] = c.total ? c.beam() : -1;
+        a.tokens[at] = token;
         a.totals[at] = c.total ? (float)order_total(c.total) : -__builtin_inff();
-        if (a.now_ended) a.now_ended[at] = c.total && (int)(uint32_t)c.place == a.end_token ? 1 : 0;
+        if (a.now_ended) a.now_ended[at] = token == a.end_token ? 1 : 0;
     };
     if (found <= kFound) {
         for (int i = tid; i < found; i += kThreads) {
             const Candidate mine = M.found[i];
             int rank = 0;
             for (int k = 0; k < found; k++) rank += better(M.found[k], mine) ? 1 : 0;
-            if (rank < a.best) put(rank, mine);
+            if (rank < a.best) put(rank, mine, M.token[i]);
         }
-        for (int k = found + tid; k < a.best; k += kThreads) put(k, Candidate{0, 0});
+        for (int k = found + tid; k < a.best; k += kThreads) put(k, Candidate{0, 0}, -1);
         return;
     }
     // more of them than fit (totals equal in masses): one after the other
     Candidate last{~0ull, 0};
     for (int k = 0; k < a.best; k++) {
         Candidate mine{0, ~0ull};
-        each([&](const Candidate& c) {
+        each([&](const Candidate& c, uint64_t) {
             if (c.total && better(last, c) && better(c, mine)) mine = c;
         });
         for (int s = 32; s; s >>= 1) {
@@ -271,7 +285,7 @@ __device__ __forceinline__ void merge_group(const BeamArgs& a, int g, MergeShare
         __syncthreads();
         for (int w = 0; w < kThreads / 64; w++)
             if (better(M.wave_best[w], mine)) mine = M.wave_best[w];
-        if (tid == 0) put(k, mine);
+        if (tid == 0) put(k, mine, mine.total ? token_of(mine, key_at(mine.index())) : -1);
         last = mine;
         __syncthreads();
     }
