@@ -79,7 +79,9 @@ int manta_rocm_matmul_q8(MantaRocm* rt, const MantaRocmWeight* w, const int8_t* 
  * pass: y = rotate(x / sqrt(mean(x^2) + eps) * norm), the mean over a head's
  * head_dim columns, in f32 (the sum of squares in f64), rounded once.
  * norms_dev[i], f32 [head_dim] in device memory, belongs to parts[i]; NULL:
- * that tensor is rotated only.  eps is at least 2^-126. */
+ * that tensor is rotated only.  eps is at least 2^-126.  As the formula has it,
+ * a NaN makes its whole head NaN, an infinity its own pair (or column), and the
+ * head's other columns 0. */
 int manta_rocm_rotary_normed(MantaRocm* rt, const MantaRocmRotary* rot, int dtype, const int32_t* positions_dev,
                              int64_t tokens, int64_t head_dim, const MantaRocmHeads* parts,
                              const float* const* norms_dev, int64_t nparts, double eps, char** err);

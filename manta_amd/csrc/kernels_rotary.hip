@@ -237,7 +237,9 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                 if (part == k) norm = n.weight[k] != nullptr;
             // the hardware's 2^-23 and a step of Newton's, of the error squared
             const double mean = fma(sum, n.inv_dim, n.eps), r0 = __builtin_amdgcn_rsq(mean);
-            const float r = norm ? (float)fma(0.5 * r0, fma(-mean * r0, r0, 1.0), r0) : 1.0f;
+            // (of infinity 0 as it is: the step would be 0 times infinity)
+            const double r1 = mean < HUGE_VAL ? fma(0.5 * r0, fma(-mean * r0, r0, 1.0), r0) : r0;
+            const float r = norm ? (float)r1 : 1.0f;
             const float* w = weight[part];
             if (live) {
 #pragma unroll
