@@ -60,6 +60,8 @@ class Quantized:
     """Rows in 8 bits with a scale each (Runtime.quantized): codes in blocks of
     16 rows and 64 columns, as the products read them."""
 
+    shared = False  # part of a larger one (first)
+
     def __init__(self, rt, rows: int, width: int):
         size = load().manta_rocm_quantized_bytes(rows, width)
         if size < 0:
@@ -68,13 +70,24 @@ class Quantized:
         self.codes = rt.empty((size,), np.int8)
         self.scales = rt.empty((rows,), np.float32)
 
+    def first(self, rows: int) -> "Quantized":
+        """The memory of the first `rows` rows, for a batch of so many: it is
+        this one's."""
+        if not 0 <= rows <= self.rows:
+            raise ValueError("quantized rows: %s of %d" % (rows, self.rows))
+        part = Quantized.__new__(Quantized)
+        part.rt, part.rows, part.width, part.codes, part.scales = self.rt, rows, self.width, self.codes, self.scales
+        part.shared = True
+        return part
+
     def values(self):
         """(codes int8 [rows, width], scales f32 [rows]) on the host; waits
         for the stream."""
         pitch = (self.width + 127) // 128 * 128
         c = self.codes.download().reshape(-1, pitch // 64, 4, 16, 16)
         c = c.transpose(0, 3, 1, 2, 4).reshape(-1, pitch)
-        return np.ascontiguousarray(c[:self.rows, :self.width]), self.scales.download()
+        scales = self.scales.download()
+        return np.ascontiguousarray(c[:self.rows, :self.width]), scales[:self.rows] if self.shared else scales
 
 
 def _matrix(name: str, a, rows: Optional[int] = None, columns: Optional[int] = None):

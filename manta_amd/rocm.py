@@ -219,7 +219,8 @@ class Runtime:
         return decode.Weight(self, codes, scales, gate)
 
     def quantized(self, rows: int, width: int):
-        """Memory for rows in 8 bits (decode.Quantized)."""
+        """Memory for rows in 8 bits (decode.Quantized); its first(n) serves
+        batches of fewer."""
         return decode.Quantized(self, rows, width)
 
     def quantize_rows(self, x: DeviceArray, out=None, norm: Optional[DeviceArray] = None, eps: float = 1e-6,
