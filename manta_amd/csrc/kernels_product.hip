@@ -612,48 +612,23 @@ hipError_t product_few(const ProductArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Which tile: figures are bf16, 4096 summed columns, us on 256 compute units.
+// (decode_layout.hpp has the rule)
 template <class E, bool GATED>
 hipError_t product_of(const ProductArgs& a, hipStream_t s) {
-    const int64_t rb = (a.rows + 15) / 16, wb = a.w_blocks;
-    auto few = [&](int mt, int nt) { return ((rb + mt - 1) / mt) * ((wb + nt - 1) / nt); };
-    // The smallest tile that still is a workgroup a compute unit or less: more
-    // of them share the reading of the weight, and its latency (32 rows x 4096
-    // columns: 16 x 32 tiles 5.9, 32 x 32 7.3; 64 x 4096: 64 x 32 9.1, tiles of
-    // 64 x 64 through LDS 14.9)
-    if constexpr (!GATED)
-        if (few(1, 1) <= a.cus) return product_few<E, GATED, 8, 1, 1, 4>(a, s);
-    if (few(1, 2) <= a.cus) return product_few<E, GATED, 8, 1, 2, 2>(a, s);
-    if (few(2, 2) <= a.cus) return product_few<E, GATED, 8, 2, 2, 2>(a, s);
-    if (few(4, 2) <= a.cus) return product_few<E, GATED, 4, 4, 2, 2>(a, s);
-    // Up to 32 rows of more columns, where the weight's bytes are all that
-    // counts (16 rows x 24576 columns: 16.6, tiles 18.2; 32 rows are even)
-    if (rb == 1) return product_few<E, GATED, 8, 1, 2, 2>(a, s);
-    if (rb == 2) return product_few<E, GATED, 8, 2, 2, 2>(a, s);
-    // Tiles of 64 x 64 while those are few: a larger tile of a unit's own takes
-    // as long as several of them (512 x 4096: 15.1, 128 x 128 26.9; 1024 x 4096
-    // 27.1, 30.8; 512 x 12288 40.2, 37.9)
-    const int64_t t64 = ((a.rows + 63) / 64) * ((wb + 3) / 4), t128 = ((a.rows + 127) / 128) * ((wb + 7) / 8);
-    if (t64 <= 4 * a.cus) {
-        // a tile a unit or less: a deep ring, 128 columns a barrier (589 x 832 of
-        // 7936 summed: 19.4, two stages 28.5, four of 64 columns 23.9)
-        if (t64 <= a.cus) return product_tiles<E, GATED, 2, 2, 2, 2, 4, 2>(a, s);
-        // one row of tiles reads its weight out of memory (48 rows x 2 x 12288:
-        // 18.3, and 19.1 with less LDS)
-        if (rb <= 4) return product_tiles<E, GATED, 2, 2, 2, 2, 4, 1>(a, s);
-        // several a unit wait for each other's data with little LDS each (512 x
-        // 4096: 15.1, four stages 16.4, of 64 columns 18.3; 1024 x 4096: 27.1,
-        // 30.5, 29.6)
-        return product_tiles<E, GATED, 2, 2, 2, 2, 2, 2>(a, s);
+    switch (product_form(a.rows, a.w_blocks, GATED, a.cus)) {
+        case kFew16x16:
+            if constexpr (!GATED) return product_few<E, GATED, 8, 1, 1, 4>(a, s);
+            break;  // (not of gated weights)
+        case kFew16x32: return product_few<E, GATED, 8, 1, 2, 2>(a, s);
+        case kFew32x32: return product_few<E, GATED, 8, 2, 2, 2>(a, s);
+        case kFew64x32: return product_few<E, GATED, 4, 4, 2, 2>(a, s);
+        case kTile64Deep: return product_tiles<E, GATED, 2, 2, 2, 2, 4, 2>(a, s);
+        case kTile64Row: return product_tiles<E, GATED, 2, 2, 2, 2, 4, 1>(a, s);
+        case kTile64: return product_tiles<E, GATED, 2, 2, 2, 2, 2, 2>(a, s);
+        case kTile128: return product_tiles<E, GATED, 2, 2, 4, 4, 2, 1>(a, s);
+        case kTile256: return product_tiles<E, GATED, 2, 4, 8, 4, 2, 1>(a, s);
     }
-    // 256 x 256 needs half of the operands' reads of 128 x 128, but comes in
-    // whole rounds of a tile a unit, 57 each, against 17.5 a tile for the unit
-    // that has most of 128 x 128, and 9 (1024 x 12288: 60.1 and 66.0; 2048 x 4096:
-    // 57.7 and 43; 8192 x 4096: 121 and 158; 16384 x 640: 54.8 and 63.8)
-    const int64_t t256 = ((a.rows + 255) / 256) * ((wb + 15) / 16);
-    if ((t256 + a.cus - 1) / a.cus * 13 <= (t128 + a.cus - 1) / a.cus * 4 + 2)
-        return product_tiles<E, GATED, 2, 4, 8, 4, 2, 1>(a, s);
-    return product_tiles<E, GATED, 2, 2, 4, 4, 2, 1>(a, s);
+    return hipErrorInvalidValue;
 }
 
 template <class E>
