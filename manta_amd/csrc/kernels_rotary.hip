@@ -33,6 +33,16 @@ __device__ __forceinline__ float turn_left(double pos, double turns) {
 __device__ __forceinline__ float turn_1(float x1, float x2, float c, float s) { return fmaf(x1, c, -(x2 * s)); }
 __device__ __forceinline__ float turn_2(float x1, float x2, float c, float s) { return fmaf(x2, c, x1 * s); }
 
+// A result, rounded to f32 and then to its type.  (Else the compiler fuses f16's
+// rounding with the operation before it for some elements of a piece and not for
+// others: a result would depend on its place, and two lanes that work out the
+// same element could write two.)
+template <class E>
+__device__ __forceinline__ typename E::T stored(float y) {
+    asm("" : "+v"(y));
+    return E::store(y);
+}
+
 // V elements at once: V pairs of a head, or V columns past the rotated ones.
 template <class E, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
@@ -85,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
                 const T t1 = !INTERLEAVED ? lo.v[j] : e < V ? lo.v[e % V] : hi.v[e % V];
                 const T t2 = !INTERLEAVED ? hi.v[j] : e + 1 < V ? lo.v[(e + 1) % V] : hi.v[(e + 1) % V];
                 const float x1 = E::load(t1), x2 = E::load(t2), c = cs[p + j], s = sn[p + j];
-                const T y1 = E::store(turn_1(x1, x2, c, s)), y2 = E::store(turn_2(x1, x2, c, s));
+                const T y1 = stored<E>(turn_1(x1, x2, c, s)), y2 = stored<E>(turn_2(x1, x2, c, s));
                 if (!INTERLEAVED) {
                     ylo.v[j] = y1;
                     yhi.v[j] = y2;
@@ -251,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                         Piece o;
 #pragma unroll
                         for (int j = 0; j < V; j++)
-                            o.v[j] = norm ? E::store(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
+                            o.v[j] = norm ? stored<E>(E::load(lo[i].v[j]) * r * w[at + j]) : lo[i].v[j];
                         if constexpr (PIECES == kEven) {
                             put(out + at, o);
                         } else if (PIECES == kShared || at + V <= a.head_dim) {
@@ -282,8 +292,8 @@ __global__ __launch_bounds__(kThreads) void rotary_normed_kernel(RotaryArgs a, R
                         // pair p + j: elements 2j and 2j + 1 of the run, or j of each half
                         const int e1 = INTERLEAVED ? 2 * j : j, e2 = INTERLEAVED ? 2 * j + 1 : V + j;
                         const float c = cs[token][p + j], s = sn[token][p + j];
-                        o[e1] = E::store(turn_1(u[e1], u[e2], c, s));
-                        o[e2] = E::store(turn_2(u[e1], u[e2], c, s));
+                        o[e1] = stored<E>(turn_1(u[e1], u[e2], c, s));
+                        o[e2] = stored<E>(turn_2(u[e1], u[e2], c, s));
                     }
                     Piece ylo, yhi;
 #pragma unroll

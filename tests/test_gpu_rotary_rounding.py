@@ -90,17 +90,35 @@ def test_far_positions_that_are_almost_whole_turns(rt, normed):
     assert (np.abs(got - want) <= 2.0 ** -20 * np.abs(want)).all()
 
 
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-def test_narrow_results_are_those_of_f32(rt, dtype):
-    """16-bit elements: the f32 results of the same numbers, rounded once more
-    (or, fused, not even that: one unit of the last place at a tie)."""
+@pytest.mark.parametrize("d,rot", [(64, 64), (47, 40), (80, 50), (20, 4)])
+def test_narrow_results_are_those_of_f32(rt, d, rot, dtype, layout, normed):
+    """16-bit elements: the f32 results of the same numbers, rounded once more,
+    whichever kernel and lane works them out."""
+    print("rotary narrow", d, rot, dtype, layout, normed, flush=True)
     rng = np.random.default_rng(3)
-    t, d = 200, 64
-    freqs = 10000.0 ** (-np.arange(d // 2) / (d // 2))
-    pos = rng.integers(0, 100000, t)
-    bits = to_bits(rng.standard_normal((t, 2, d)), dtype)
-    wide = _call(rt, from_bits(bits, dtype), pos, freqs, "half", "f32", False)
-    got = from_bits(_call(rt, bits, pos, freqs, "half", dtype, False), dtype)
-    want = from_bits(to_bits(wide, dtype), dtype)
-    unit = np.abs(want) * {"f16": 2.0 ** -10, "bf16": 2.0 ** -7}[dtype] + 2.0 ** -24
-    assert (np.abs(got - want) <= unit).all() and (got != want).mean() < 0.001
+    t = 8199
+    freqs, pos = 10000.0 ** (-np.arange(rot // 2) / rot), rng.integers(0, 100000, t)
+    bits = to_bits(rng.standard_normal((t, 3, d)), dtype)
+    wide = _call(rt, from_bits(bits, dtype), pos, freqs, layout, "f32", normed)
+    np.testing.assert_array_equal(_call(rt, bits, pos, freqs, layout, dtype, normed), to_bits(wide, dtype))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("d,rot", [(64, 64), (47, 40), (80, 50), (20, 4)])
+def test_narrow_normed_results_are_those_of_f32(rt, d, rot, layout):
+    rng = np.random.default_rng(4)
+    t = 8199
+    r = rt.rotary_bind(10000.0 ** (-np.arange(rot // 2) / rot), layout=layout)
+    p, w = rt.to_device(rng.integers(0, 100000, t).astype(np.int32)), rt.to_device(rng.uniform(0.5, 2, d).astype(np.float32))
+    bits = to_bits(rng.standard_normal((t, 3, d)), "f16")
+    found = []
+    for x, dtype in ((bits, "f16"), (from_bits(bits, "f16"), "f32")):
+        out = rt.to_device(np.zeros_like(x))
+        rt.rotary_normed(r, p, [(rt.to_device(x), out)], [w], dtype=dtype)
+        found.append(out.download())
+    # the sums of squares come in another order of their f64 additions: one factor
+    # in 10^8 rounds to its neighbour
+    assert (found[0] != to_bits(found[1], "f16")).mean() < 1e-5
