@@ -180,6 +180,8 @@ class Answerer:
     def answer(self, questions: Sequence[Sequence[int]], most: int) -> List[List[Tuple[List[int], float]]]:
         """For each question its beams, the best first: up to `most` tokens
         (without the one that ends them) and their log probability."""
+        if most < 1:
+            raise ValueError("answers of %d tokens" % most)
         if max(len(q) for q in questions) + most - 1 > self.tokens:
             raise ValueError("question and answer have more than %d tokens" % self.tokens)
         self.ask(questions)

@@ -6,7 +6,7 @@ import pytest
 from cache_oracle import Model
 from decode_oracle import reorder
 from manta_amd import _lib, decode
-from manta_amd.answer import pool_pages
+from manta_amd.answer import Answerer, pool_pages
 
 
 @pytest.mark.parametrize("questions,beams,tokens,page", [
@@ -51,3 +51,11 @@ def test_inputs_that_are_refused():
                                    (1, -1, 4096, "token -1"), (1, 1 << 31, 4096, "token 2147483648"), (1, 0, None, "nil")):
         with pytest.raises(_lib.MantaRocmError, match=message):
             _lib.call("manta_rocm_beam_inputs", None, p, n, instead, p)
+
+
+@pytest.mark.parametrize("most", [0, -3])
+def test_answers_of_no_tokens(most):
+    a = Answerer.__new__(Answerer)
+    a.tokens = 64
+    with pytest.raises(ValueError, match="answers of %d tokens" % most):
+        a.answer([[5, 6]], most)
