@@ -480,7 +480,7 @@ __global__ __launch_bounds__(WAVES * 64) void product_few_kernel(ProductArgs a) 
 // where it goes, and a wave reads it back 16 bytes a lane in order, so neither
 // side has a bank conflict.
 //
-// 8192 x 4096 x 4096 bf16: 121 us, 2.27 POP/s (torch's int8 product of that
+// 8192 x 4096 x 4096 bf16: 121 to 124 us, 2.2 POP/s (torch's int8 product of that
 // size, without scales: 130).  What bounds it: a step's products alone take 54
 // of a 256 x 256 tile's 67 us when the whole card works on random codes (the
 // clock falls with the matrix cores' load: 43 us on 16 compute units), the
